@@ -443,6 +443,70 @@ int b200exl3_head_argmax(const uint16_t* d_x_f16, const uint16_t* d_weight_f16, 
                          uint16_t* d_logits_f16, float* d_best_value, int64_t* d_best_index, void* d_workspace,
                          size_t workspace_bytes, b200exl3_stream stream);
 
+/* ---- paged key/value cache: several sequences, any number of new tokens, 16, 8 or 4 bits ----------------------------
+ * No counterpart in the reference beyond the array operators named above (its cache is one array per sequence): the same rotary
+ * embedding, append and attention for batches, prompts and draft tokens.  Rows, positions and pages live on the device, so that a
+ * recorded call can be replayed while the sequences grow. */
+
+/* A pool of pages: keys and values each [pages, kv_heads, page_size, head_dim].  dtype (f16 or bf16) is the type of the rows of q,
+ * k, v and the outputs, and of the cache itself with bits == 16.  With bits == 8 or 4 a vector is held as integer codes round(x * m /
+ * max|x|), m = 127 or 7, one per byte, or two per byte as code + 8 with the even dimension in the low half, and one scale max|x| / m
+ * in [pages, kv_heads, page_size].  head_dim is 64 or 128; any page_size; a cache of one page of max_ctx rows per sequence is the
+ * layout of b200exl3_rope_append and b200exl3_attention_decode. */
+typedef struct {
+    void* d_k;
+    void* d_v;
+    float* d_k_scale;                /* NULL with bits == 16 */
+    float* d_v_scale;
+    int64_t pages;
+    int page_size;
+    int kv_heads;
+    int head_dim;
+    int dtype;
+    int bits;
+} b200exl3_kv_cache;
+/* The sequences of a call: sequence b brings the rows d_row_start[b] .. d_row_start[b + 1] - 1 of the row buffers, which are the last
+ * of its d_length[b] tokens (row i of n is token length - n + i), and token t lies in row t % page_size of page d_page_table[b,
+ * t / page_size].  d_row_start ascends; `rows` bounds the row buffers.  Rows that are no sequence's and tokens before the first are left
+ * as they were; tokens behind the table and pages outside the pool are never written and read as zeros (kv_read leaves their rows as
+ * they were).  No two sequences of a call may append to the same row of a page. */
+typedef struct {
+    const int32_t* d_row_start;      /* [batch + 1] */
+    const int32_t* d_length;         /* [batch] */
+    const int32_t* d_page_table;     /* [batch, table_width] */
+    int64_t rows;
+    int batch;
+    int table_width;
+} b200exl3_kv_batch;
+/* Rotary embedding of the first `rotated` dimensions of a head (a multiple of 16, 0 = none): the pairs (j, j + rotated / 2), or with
+ * `interleaved` (2j, 2j + 1), turn by 2 pi * position * d_turns[j] and are multiplied by `magnitude`.  The frequencies come as turns
+ * per position in 64 bits, theta^(-2j / rotated) / 2 pi or any scaled form of it. */
+typedef struct {
+    const double* d_turns;           /* [rotated / 2] */
+    int rotated;
+    int interleaved;
+    float magnitude;
+} b200exl3_rope;
+/* q [rows, heads, head_dim] rotated to d_q_out (may be d_q; heads == 0: no q), k [rows, kv_heads, head_dim] rotated and v as it is
+ * written to the cache; strides are elements between rows (multiples of 8, so that a row may be a part of a wider one; 0 = rows
+ * without gaps).  fp32 inside and one rounding; the position's angle, and with codes the rotated k up to its code, in 64 bits. */
+int b200exl3_kv_append(const b200exl3_kv_cache* cache, const b200exl3_kv_batch* batch, const b200exl3_rope* rope, const void* d_q,
+                       int64_t q_stride, int heads, void* d_q_out, int64_t q_out_stride, const void* d_k, int64_t k_stride,
+                       const void* d_v, int64_t v_stride, b200exl3_stream stream);
+/* What the cache holds for the rows of the batch: keys and values [rows, kv_heads, head_dim] in out_dtype (f16, bf16 or f32), rounded
+ * once; either output may be NULL. */
+int b200exl3_kv_read(const b200exl3_kv_cache* cache, const b200exl3_kv_batch* batch, int out_dtype, void* d_k_out, void* d_v_out,
+                     b200exl3_stream stream);
+/* out[row, h] = sum_j softmax_j(scale * q[row, h] . k_j) v_j over the tokens j up to the row's own, with window > 0 the last `window` of
+ * them; heads / kv_heads query heads share a key head; the row's own token has been appended before.  A row that sees no token is
+ * zero.  max_new bounds the rows of one sequence (rows beyond it are not computed; 0 = `rows`): it chooses the kernel, so say 1 for a
+ * step of single tokens.  Tokens that no row of a sequence sees are never used whatever they hold; the others have to be finite.
+ * The workspace follows the rules of the linear layer's (header of zeros; one call at a time). */
+int b200exl3_kv_attention_workspace_bytes(const b200exl3_kv_cache* cache, int heads, int64_t max_new, size_t* out_bytes);
+int b200exl3_kv_attention(const b200exl3_kv_cache* cache, const b200exl3_kv_batch* batch, const void* d_q, int64_t q_stride, int heads,
+                          float scale, int window, int64_t max_new, void* d_out, int64_t out_stride, void* d_workspace,
+                          size_t workspace_bytes, b200exl3_stream stream);
+
 /* ---- router: stable top-k ----------------------------------------------------------------------------------
  * Replaces router::topk / routes (native/src/router.rs:28-120, native/shaders/router_topk.h:1-34): values
  * [rows, experts] (fp16 = 9 or fp32 = 10, experts <= 1024) -> indices [rows, top_k] (u32) and scores

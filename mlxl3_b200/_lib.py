@@ -100,6 +100,12 @@ SIGNATURES = {
     "b200exl3_attention_decode": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "b200exl3_head_workspace_bytes": (c_int, [POINTER(c_size_t)]),
     "b200exl3_head_argmax": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "b200exl3_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                   c_void_p]),
+    "b200exl3_kv_read": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "b200exl3_kv_attention_workspace_bytes": (c_int, [c_void_p, c_int, c_int64, POINTER(c_size_t)]),
+    "b200exl3_kv_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_float, c_int, c_int64, c_void_p, c_int64, c_void_p, c_size_t,
+                                      c_void_p]),
     "b200exl3_router_topk": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "b200exl3_router_softmax_topk": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "b200exl3_router_gate": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p]),

@@ -1884,6 +1884,143 @@ int b200exl3_attention_decode(const uint16_t* d_q, const uint16_t* d_k_cache, co
                                          reinterpret_cast<__half*>(d_out), ws, as_stream(s)), "attention kernel");
 }
 
+/* ---- paged key/value cache --------------------------------------------------------------------------------------- */
+
+static int kv_args(const b200exl3_kv_cache* c, const b200exl3_kv_batch* b, KvArgs& p) {
+    if (!c) return fail("NULL argument");
+    if (c->dtype != kF16 && c->dtype != kBF16) return fail("a paged cache takes f16 or bf16 rows");
+    if (c->bits != 16 && c->bits != 8 && c->bits != 4) return fail("a paged cache holds 16, 8 or 4 bits, got %d", c->bits);
+    if (c->head_dim != 64 && c->head_dim != 128) return fail("a paged cache is built for a head dimension of 64 or 128, got %d", c->head_dim);
+    if (c->pages <= 0 || c->pages > INT32_MAX || c->page_size <= 0 || c->kv_heads <= 0 || c->kv_heads > 65535) return fail("invalid paged cache dimensions");
+    if (static_cast<double>(c->pages) * c->page_size * c->kv_heads > 1e15) return fail("invalid paged cache dimensions");
+    if (!c->d_k || !c->d_v || (c->bits != 16 && (!c->d_k_scale || !c->d_v_scale))) return fail("NULL buffer");
+    if (!aligned16(c->d_k) || !aligned16(c->d_v)) return fail("device pointers must be 16-byte aligned");
+    if (c->bits != 16 && check_places({{c->d_k_scale, sizeof(float)}, {c->d_v_scale, sizeof(float)}})) return -1;
+    p = KvArgs{};
+    p.k = c->d_k;
+    p.v = c->d_v;
+    p.k_scale = c->d_k_scale;
+    p.v_scale = c->d_v_scale;
+    p.pages = c->pages;
+    p.page_size = c->page_size;
+    p.page_shift = -1;
+    if ((c->page_size & (c->page_size - 1)) == 0)
+        for (p.page_shift = 0; (1 << p.page_shift) < c->page_size;) ++p.page_shift;
+    p.kv_heads = c->kv_heads;
+    p.head_dim = c->head_dim;
+    p.dtype = c->dtype;
+    p.bits = c->bits;
+    if (!b) return 0;
+    if (b->batch <= 0 || b->rows <= 0 || b->rows > INT32_MAX || b->table_width <= 0) return fail("invalid batch dimensions");
+    if (static_cast<int64_t>(b->table_width) * c->page_size > kKvMaxTokens) return fail("a page table may hold 2^30 tokens per sequence");
+    if (!b->d_row_start || !b->d_length || !b->d_page_table) return fail("NULL buffer");
+    if (check_places({{b->d_row_start, sizeof(int32_t)}, {b->d_length, sizeof(int32_t)}, {b->d_page_table, sizeof(int32_t)}})) return -1;
+    p.row_start = b->d_row_start;
+    p.length = b->d_length;
+    p.table = b->d_page_table;
+    p.rows = b->rows;
+    p.batch = b->batch;
+    p.table_width = b->table_width;
+    return 0;
+}
+
+// Elements between rows: 0 = rows without gaps.
+static int kv_stride(int64_t& stride, int64_t width) {
+    if (stride == 0) stride = width;
+    if (stride < width || stride % 8 || stride > (int64_t(1) << 32)) return fail("rows of %lld elements cannot lie %lld apart", static_cast<long long>(width), static_cast<long long>(stride));
+    return 0;
+}
+
+int b200exl3_kv_append(const b200exl3_kv_cache* cache, const b200exl3_kv_batch* batch, const b200exl3_rope* rope, const void* d_q,
+                       int64_t q_stride, int heads, void* d_q_out, int64_t q_out_stride, const void* d_k, int64_t k_stride,
+                       const void* d_v, int64_t v_stride, b200exl3_stream s) {
+    if (!batch) return fail("NULL argument");
+    KvArgs p;
+    if (kv_args(cache, batch, p)) return -1;
+    KvAppendArgs a{};
+    if (heads < 0 || heads > (1 << 20)) return fail("invalid attention head counts");
+    if (rope) {
+        if (rope->rotated < 0 || rope->rotated > p.head_dim || rope->rotated % 16) return fail("rotary embedding of %d of %d dimensions: a multiple of 16 is needed", rope->rotated, p.head_dim);
+        if (rope->rotated && !rope->d_turns) return fail("NULL buffer");
+        if (!std::isfinite(rope->magnitude)) return fail("invalid rotary magnitude");
+        if (check_places({{rope->d_turns, sizeof(double)}})) return -1;
+        a.turns = rope->d_turns;
+        a.rotated = rope->rotated;
+        a.interleaved = rope->interleaved != 0;
+        a.magnitude = rope->magnitude;
+    }
+    if (!d_k || !d_v || (heads && (!d_q || !d_q_out))) return fail("NULL buffer");
+    if (kv_stride(q_stride, static_cast<int64_t>(std::max(heads, 1)) * p.head_dim) || kv_stride(q_out_stride, static_cast<int64_t>(std::max(heads, 1)) * p.head_dim) ||
+        kv_stride(k_stride, static_cast<int64_t>(p.kv_heads) * p.head_dim) || kv_stride(v_stride, static_cast<int64_t>(p.kv_heads) * p.head_dim)) return -1;
+    if ((heads && (!aligned16(d_q) || !aligned16(d_q_out))) || !aligned16(d_k) || !aligned16(d_v)) return fail("device pointers must be 16-byte aligned");
+    if (heads && d_q == d_q_out && q_stride != q_out_stride) return fail("queries are rotated in place with one stride");
+    a.q = d_q;
+    a.q_out = d_q_out;
+    a.k = d_k;
+    a.v = d_v;
+    a.q_stride = q_stride;
+    a.q_out_stride = q_out_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.heads = heads;
+    return check(launch_kv_append(p, a, as_stream(s)), "cache append kernel");
+}
+
+int b200exl3_kv_read(const b200exl3_kv_cache* cache, const b200exl3_kv_batch* batch, int out_dtype, void* d_k_out, void* d_v_out,
+                     b200exl3_stream s) {
+    if (!batch) return fail("NULL argument");
+    KvArgs p;
+    if (kv_args(cache, batch, p)) return -1;
+    if (!dtype_is_float(out_dtype)) return fail("unsupported dtype %d", out_dtype);
+    if (!d_k_out && !d_v_out) return fail("NULL buffer");
+    if (!aligned16(d_k_out) || !aligned16(d_v_out)) return fail("device pointers must be 16-byte aligned");
+    return check(launch_kv_read(p, out_dtype, d_k_out, d_v_out, as_stream(s)), "cache read kernel");
+}
+
+static int kv_attention_heads(const b200exl3_kv_cache* c, int heads, int64_t max_new) {
+    if (heads <= 0 || heads > (1 << 20) || heads % c->kv_heads) return fail("invalid attention head counts");
+    if (max_new <= 0 || max_new > INT32_MAX / heads) return fail("invalid number of new tokens");
+    return 0;
+}
+
+int b200exl3_kv_attention_workspace_bytes(const b200exl3_kv_cache* cache, int heads, int64_t max_new, size_t* out_bytes) {
+    KvArgs p;
+    if (!out_bytes) return fail("NULL argument");
+    if (kv_args(cache, nullptr, p) || kv_attention_heads(cache, heads, max_new)) return -1;
+    *out_bytes = kCounterBytes + round256(kv_attention_workspace_bytes(p.bits, p.head_dim, heads / p.kv_heads, max_new));
+    return 0;
+}
+
+int b200exl3_kv_attention(const b200exl3_kv_cache* cache, const b200exl3_kv_batch* batch, const void* d_q, int64_t q_stride, int heads,
+                          float scale, int window, int64_t max_new, void* d_out, int64_t out_stride, void* ws, size_t ws_bytes,
+                          b200exl3_stream s) {
+    if (!batch) return fail("NULL argument");
+    KvArgs p;
+    if (kv_args(cache, batch, p)) return -1;
+    if (max_new == 0 || max_new > batch->rows) max_new = batch->rows;
+    if (kv_attention_heads(cache, heads, max_new)) return -1;
+    if (!std::isfinite(scale)) return fail("invalid attention scale");
+    if (window < 0) return fail("invalid attention window");
+    if (!d_q || !d_out) return fail("NULL buffer");
+    const int64_t width = static_cast<int64_t>(heads) * p.head_dim;
+    if (kv_stride(q_stride, width) || kv_stride(out_stride, width)) return -1;
+    if (!aligned16(d_q) || !aligned16(d_out) || !aligned16(ws)) return fail("device pointers must be 16-byte aligned");
+    const size_t need = kCounterBytes + round256(kv_attention_workspace_bytes(p.bits, p.head_dim, heads / p.kv_heads, max_new));
+    if (!ws || ws_bytes < need) return fail("workspace too small: %zu bytes given, %zu needed", ws_bytes, need);
+    KvAttentionArgs a{};
+    a.q = d_q;
+    a.out = d_out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.heads = heads;
+    a.window = window;
+    a.max_new = static_cast<int>(max_new);
+    a.scale_log2e = scale * 1.4426950408889634f;
+    a.arrived = static_cast<unsigned int*>(ws);
+    a.parts = reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes);
+    return check(launch_kv_attention(p, a, as_stream(s)), "cache attention kernel");
+}
+
 int b200exl3_head_workspace_bytes(size_t* out_bytes) {
     if (!out_bytes) return fail("NULL argument");
     *out_bytes = round256(static_cast<size_t>(head_candidates()) * (sizeof(float) + sizeof(long long)));

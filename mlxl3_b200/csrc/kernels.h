@@ -416,6 +416,47 @@ size_t qmm_mapped_piece_bytes();
 cudaError_t launch_qmm_mapped(QmmArgs args, const __half* xhat, int max_segments, int k, int cb, cudaStream_t stream);
 void qmm_set_tuning(int splits);   // force the number of input splits (0 = automatic)
 
+// ---- paged key/value cache (kernels_kv.cu, kernels_kv_attention.cu) ---------------------------------------
+constexpr int kKvMaxTokens = 1 << 30;      // table_width * page_size of a call; a longer length counts as this
+struct KvArgs {
+    void* k;                   // pools [pages, kv_heads, page_size, head_dim]: 16-bit values of `dtype`, or codes of 8 or 4 bits
+    void* v;
+    float* k_scale;            // [pages, kv_heads, page_size], with codes
+    float* v_scale;
+    const int* row_start;      // [batch + 1]: sequence b brings rows row_start[b] .. row_start[b + 1] - 1
+    const int* length;         // [batch]: tokens of the sequence, those rows included as its last
+    const int* table;          // [batch, table_width] pages
+    int64_t pages, rows;       // rows: of the row buffers
+    int page_size, page_shift; // page_shift: log2 of the page size, or -1
+    int kv_heads, head_dim, dtype, bits;
+    int batch, table_width;
+};
+struct KvAppendArgs {
+    const void* q;             // rows of `heads` vectors, q_stride elements from row to row; nullptr with heads == 0
+    void* q_out;
+    const void* k;
+    const void* v;
+    int64_t q_stride, q_out_stride, k_stride, v_stride;
+    const double* turns;       // [rotated / 2] turns per position
+    int heads, rotated, interleaved;
+    double magnitude;
+};
+cudaError_t launch_kv_append(const KvArgs& args, const KvAppendArgs& append, cudaStream_t stream);
+// rows [rows, kv_heads, head_dim] of `out_dtype`; either may be nullptr
+cudaError_t launch_kv_read(const KvArgs& args, int out_dtype, void* k, void* v, cudaStream_t stream);
+
+struct KvAttentionArgs {
+    const void* q;
+    void* out;
+    int64_t q_stride, out_stride;
+    int heads, window, max_new;
+    float scale_log2e;
+    unsigned int* arrived;     // [CTAs] arrival counters at the head of the workspace, zero on entry and on exit
+    float* parts;              // two places per CTA for its part of a segment that CTAs share
+};
+size_t kv_attention_workspace_bytes(int bits, int head_dim, int group, int64_t max_new);
+cudaError_t launch_kv_attention(const KvArgs& args, const KvAttentionArgs& attention, cudaStream_t stream);
+
 // ---- weight layout (kernels_codec.cu) -----------------------------------------------------------------
 // checkpoint layout [tiles_k, tiles_n, 8K] words -> quad layout [tiles_n/8, tiles_k, 2, 8K, 4]: the stream words of four
 // neighbouring tiles interleaved word by word (a quad), two quads = one row of a 128-column block (256K bytes), and

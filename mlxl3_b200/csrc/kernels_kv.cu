@@ -1,0 +1,343 @@
+// Rotary embedding with the append to a paged key/value cache, and reading the cache back.
+//
+// append: row i of a sequence's n new rows is its token at position p = length - n + i.  The pairs (a, b) of the first `rotated`
+// dimensions of every q and k head -- (j, j + rotated/2), or (2j, 2j + 1) interleaved -- turn by the angle 2 pi p f_j, f_j in turns
+// per position: (a, b) -> m (a cos - b sin, a sin + b cos).  The product p f_j is taken in 64 bits and only its fraction goes into
+// sine and cosine, so a token at position 10^6 is as exact as the first; both are computed in 64 bits once per token and pair and
+// shared by all heads.  q goes to a buffer of its own (or in place), k and v to row p % page_size of the sequence's page
+// p / page_size.
+//
+// A quantised cache holds a vector x as codes round(x m / max|x|), m = 127 or 7, and one fp32 scale max|x| / m.  The rotated k is kept
+// in 64 bits up to the code: between two codes a last bit of fp32 decides, and every element of a long cache gets its chance at it.
+// v needs no more than fp32: x m is exact there and the quotient of two 16-bit values is never closer to a border than that division
+// rounds, unless it lies on it.  4-bit codes are stored as code + 8, the even dimension in the low half of the byte.
+//
+// Both kernels are bound by memory (and short calls by the chain row_start -> length -> page table -> data): 16 or 8 lanes hold a
+// vector, 8 dimensions each, so that every access is 16 bytes (8 or 4 for codes) and a vector one coalesced piece.
+#include "kv.cuh"
+
+namespace b200exl3 {
+
+namespace {
+
+constexpr int kKvThreads = 256;
+constexpr int kKvStarts = 256;              // sequences whose first rows are searched in shared memory
+
+// Sequence of a row: the last one that starts at or before it, by bisection (rows ascend from sequence to sequence).
+template <typename Start>
+__device__ __forceinline__ int kv_find(int batch, int row, Start start) {
+    int low = 0, high = batch;              // start(low) <= row, or low == 0
+    while (high - low > 1) {
+        const int mid = (low + high) >> 1;
+        if (start(mid) <= row) low = mid; else high = mid;
+    }
+    return low;
+}
+
+struct KvRow {
+    int64_t place;          // vector of head 0, or -1: not in the cache
+    int pos;                // position, or -1: no sequence's row
+};
+
+// Where the ROWS rows from row0 on belong: one thread per row, after the first rows were brought to shared memory.
+template <int ROWS>
+__device__ __forceinline__ void kv_locate(const KvArgs& p, int64_t row0, int (&s_start)[kKvStarts + 1], KvRow (&s_row)[ROWS]) {
+    const bool shared = p.batch <= kKvStarts;
+    if (shared) {
+        for (int i = threadIdx.x; i <= p.batch; i += kKvThreads) s_start[i] = kv_clamp_row(p, __ldg(p.row_start + i));
+        __syncthreads();
+    }
+    if (threadIdx.x < ROWS) {
+        KvRow r{-1, -1};
+        if (row0 + threadIdx.x < p.rows) {
+            const int row = static_cast<int>(row0) + static_cast<int>(threadIdx.x);
+            auto start = [&](int b) { return shared ? s_start[b] : kv_clamp_row(p, __ldg(p.row_start + b)); };
+            int b = kv_find(p.batch, row, start);
+            const int first = start(b), end = start(b + 1);
+            if (row >= first && row < end) {
+                const int pos = kv_clamp_length(__ldg(p.length + b)) - end + row;
+                if (pos >= 0) {
+                    r.pos = pos;
+                    r.place = kv_place(p, b, pos);
+                }
+            }
+        }
+        s_row[threadIdx.x] = r;
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ double kv_abs_max(double m, double x) { x = fabs(x); return x > m || x != x ? x : m; }
+__device__ __forceinline__ float kv_abs_max(float m, float x) { x = fabsf(x); return x > m || x != x ? x : m; }
+__device__ __forceinline__ double kv_divide(double a, double b) { return __ddiv_rn(a, b); }
+__device__ __forceinline__ float kv_divide(float a, float b) { return __fdiv_rn(a, b); }
+__device__ __forceinline__ int kv_round(double x) { return __double2int_rn(x); }
+__device__ __forceinline__ int kv_round(float x) { return __float2int_rn(x); }
+
+// Codes of eight dimensions of a vector that LANES neighbouring lanes hold, and its scale.  A NaN or an infinity anywhere is the
+// scale, with codes of 0: the whole vector reads as NaN.
+template <int BITS, int LANES, typename F>
+__device__ __forceinline__ void kv_quantise(const F (&x)[8], uint32_t (&words)[2], float& scale) {
+    constexpr int M = BITS == 8 ? 127 : 7;
+    F top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = kv_abs_max(top, x[i]);
+#pragma unroll
+    for (int d = LANES / 2; d >= 1; d >>= 1) top = kv_abs_max(top, __shfl_xor_sync(0xffffffffu, top, d));
+    scale = static_cast<float>(kv_divide(top, static_cast<F>(M)));
+    words[0] = words[1] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        int code = top > 0 && top < static_cast<F>(INFINITY) ? kv_round(kv_divide(x[i] * static_cast<F>(M), top)) : 0;
+        code = max(-M, min(M, code));
+        if constexpr (BITS == 8) words[i >> 2] |= static_cast<uint32_t>(code & 0xff) << (8 * (i & 3));
+        else words[0] |= static_cast<uint32_t>(code + 8) << (4 * i);
+    }
+}
+
+template <int BITS, int D>
+__device__ __forceinline__ void kv_store_codes(void* pool, float* scales, int64_t vector, int lane, const uint32_t (&words)[2], float scale) {
+    char* dst = static_cast<char*>(pool) + vector * (D * BITS / 8) + lane * BITS;
+    if constexpr (BITS == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(words[0], words[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = words[0];
+    if (lane == 0) scales[vector] = scale;
+}
+
+template <typename T, int BITS, int D, int ROWS>
+__global__ void __launch_bounds__(kKvThreads)
+kv_append_kernel(const KvArgs p, const KvAppendArgs a) {
+    constexpr int LANES = D / 8, kGroups = kKvThreads / LANES;
+    __shared__ int s_start[kKvStarts + 1];
+    __shared__ KvRow s_row[ROWS];
+    __shared__ double s_cos[ROWS][D / 2], s_sin[ROWS][D / 2];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * ROWS;
+    kv_locate<ROWS>(p, row0, s_start, s_row);
+    const int pairs = a.rotated / 2;
+    for (int i = threadIdx.x; i < ROWS * pairs; i += kKvThreads) {
+        const int r = i / pairs, j = i - r * pairs;
+        const double turns = static_cast<double>(s_row[r].pos) * __ldg(a.turns + j);
+        double sn, cs;
+        sincospi(2.0 * (turns - rint(turns)), &sn, &cs);
+        s_cos[r][j] = cs * a.magnitude;
+        s_sin[r][j] = sn * a.magnitude;
+    }
+    __syncthreads();
+    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const int vectors = a.heads + 2 * p.kv_heads;
+    const int d0 = lane * 8;
+    // this lane's partner in the half layout: the same place of the other half of the rotated dimensions
+    const int half_lanes = a.rotated / 16;
+    const bool rotates = d0 < a.rotated, upper = lane >= half_lanes;
+    const int partner = !rotates || a.interleaved ? lane : (upper ? lane - half_lanes : lane + half_lanes);
+    const int pair0 = a.interleaved ? d0 / 2 : (upper ? d0 - pairs : d0);
+    // whole warps go round together (the shuffles); a group without a vector holds zeros and stores nothing
+    const int total = ROWS * vectors;
+    for (int first = 0; first < total; first += kGroups) {
+        const int item = first + group;
+        const int r = min(item / vectors, ROWS - 1), vec = item - r * vectors;
+        const KvRow at = s_row[r];
+        const int64_t row = row0 + r;
+        const bool is_q = vec < a.heads, is_k = !is_q && vec < a.heads + p.kv_heads;
+        const int head = is_q ? vec : (is_k ? vec - a.heads : vec - a.heads - p.kv_heads);
+        const bool live = item < total && at.pos >= 0 && (is_q || at.place >= 0);
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (live) {
+            const T* src = is_q ? static_cast<const T*>(a.q) + row * a.q_stride
+                                : (is_k ? static_cast<const T*>(a.k) + row * a.k_stride : static_cast<const T*>(a.v) + row * a.v_stride);
+            w = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(head) * D + d0);
+        }
+        uint32_t own[4] = {w.x, w.y, w.z, w.w}, other[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) other[i] = __shfl_sync(0xffffffffu, own[i], partner, LANES);
+        // x[i] of dimension d0 + i turned, in F
+        auto turn = [&](auto zero, auto (&x)[8]) {
+            using F = decltype(zero);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = KvType<T>::unpack(own[i]);
+                x[2 * i] = f.x;
+                x[2 * i + 1] = f.y;
+            }
+            if (!rotates || pairs == 0) return;
+            if (a.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const F c = static_cast<F>(s_cos[r][pair0 + i]), s = static_cast<F>(s_sin[r][pair0 + i]), u = x[2 * i], v = x[2 * i + 1];
+                    x[2 * i] = u * c - v * s;
+                    x[2 * i + 1] = u * s + v * c;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = KvType<T>::unpack(other[i]);
+                    const F y[2] = {f.x, f.y};
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const F c = static_cast<F>(s_cos[r][pair0 + 2 * i + e]), s = static_cast<F>(s_sin[r][pair0 + 2 * i + e]), u = x[2 * i + e];
+                        x[2 * i + e] = upper ? y[e] * s + u * c : u * c - y[e] * s;
+                    }
+                }
+            }
+        };
+        const int64_t vector = at.place + static_cast<int64_t>(head) * p.page_size;
+        auto store = [&](T* dst, const float (&x)[8]) {
+            *reinterpret_cast<uint4*>(dst) = make_uint4(KvType<T>::pack(x[0], x[1]), KvType<T>::pack(x[2], x[3]), KvType<T>::pack(x[4], x[5]),
+                                                        KvType<T>::pack(x[6], x[7]));
+        };
+        if constexpr (BITS == 16) {
+            if (!live) continue;
+            if (is_q || is_k) {
+                float x[8];
+                turn(0.0f, x);
+                store(is_q ? static_cast<T*>(a.q_out) + row * a.q_out_stride + static_cast<int64_t>(head) * D + d0 : static_cast<T*>(p.k) + vector * D + d0, x);
+            } else {
+                *reinterpret_cast<uint4*>(static_cast<T*>(p.v) + vector * D + d0) = w;
+            }
+        } else {
+            if (is_q) {
+                if (live) {
+                    float x[8];
+                    turn(0.0f, x);
+                    store(static_cast<T*>(a.q_out) + row * a.q_out_stride + static_cast<int64_t>(head) * D + d0, x);
+                }
+            }
+            // a warp may hold vectors of several kinds: all its lanes go through the shuffles of both
+            uint32_t words[2];
+            float scale;
+            if (__any_sync(0xffffffffu, is_k && live)) {
+                double x[8];
+                turn(0.0, x);
+                kv_quantise<BITS, LANES>(x, words, scale);
+                if (is_k && live) kv_store_codes<BITS, D>(p.k, p.k_scale, vector, lane, words, scale);
+            }
+            if (__any_sync(0xffffffffu, !is_q && !is_k && live)) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = KvType<T>::unpack(own[i]);
+                    x[2 * i] = f.x;
+                    x[2 * i + 1] = f.y;
+                }
+                kv_quantise<BITS, LANES>(x, words, scale);
+                if (!is_q && !is_k && live) kv_store_codes<BITS, D>(p.v, p.v_scale, vector, lane, words, scale);
+            }
+        }
+    }
+}
+
+template <typename O>
+__device__ __forceinline__ void kv_store8(O* dst, const float (&x)[8]) {
+    if constexpr (sizeof(O) == 4) {
+        reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(KvType<O>::pack(x[0], x[1]), KvType<O>::pack(x[2], x[3]), KvType<O>::pack(x[4], x[5]),
+                                                    KvType<O>::pack(x[6], x[7]));
+    }
+}
+
+// T: type of a 16-bit cache (any for codes); O: type of the rows
+template <typename T, int BITS, int D, typename O, int ROWS>
+__global__ void __launch_bounds__(kKvThreads)
+kv_read_kernel(const KvArgs p, O* __restrict__ k_out, O* __restrict__ v_out) {
+    constexpr int LANES = D / 8, kGroups = kKvThreads / LANES;
+    __shared__ int s_start[kKvStarts + 1];
+    __shared__ KvRow s_row[ROWS];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * ROWS;
+    kv_locate<ROWS>(p, row0, s_start, s_row);
+    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const int vectors = 2 * p.kv_heads, total = ROWS * vectors;
+#pragma unroll 4
+    for (int item = group; item < total; item += kGroups) {
+        const int r = item / vectors, vec = item - r * vectors;
+        const bool is_k = vec < p.kv_heads;
+        const int head = is_k ? vec : vec - p.kv_heads;
+        const KvRow at = s_row[r];
+        O* out = is_k ? k_out : v_out;
+        if (at.place < 0 || out == nullptr) continue;
+        const int64_t vector = at.place + static_cast<int64_t>(head) * p.page_size;
+        const char* src = static_cast<const char*>(is_k ? p.k : p.v) + vector * (D * BITS / 8) + lane * BITS;
+        float x[8];
+        if constexpr (BITS == 16) {
+            const uint4 w = __ldcs(reinterpret_cast<const uint4*>(src));
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = KvType<T>::unpack(words[i]);
+                x[2 * i] = f.x;
+                x[2 * i + 1] = f.y;
+            }
+        } else {
+            const float scale = __ldg((is_k ? p.k_scale : p.v_scale) + vector);
+            if constexpr (BITS == 8) {
+                const uint2 w = __ldcs(reinterpret_cast<const uint2*>(src));
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[i] = scale * static_cast<float>(static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3))));
+            } else {
+                const uint32_t w = __ldcs(reinterpret_cast<const uint32_t*>(src));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = scale * static_cast<float>(static_cast<int>((w >> (4 * i)) & 15u) - 8);
+            }
+        }
+        kv_store8(out + ((row0 + r) * p.kv_heads + head) * D + lane * 8, x);
+    }
+}
+
+// One row a CTA while that leaves SMs free: a short call is the latency of one row.  Eight (four appended) rows share the search
+// and fill the CTA's threads where there are many.
+template <int MANY>
+bool kv_many_rows(int64_t rows) { return rows >= static_cast<int64_t>(MANY) * 2 * sm_count(); }
+
+template <typename T, int BITS, int D>
+cudaError_t launch_append(const KvArgs& p, const KvAppendArgs& a, cudaStream_t stream) {
+    if (kv_many_rows<4>(p.rows))
+        return launch_dependent(kv_append_kernel<T, BITS, D, 4>, dim3(static_cast<unsigned>((p.rows + 3) / 4)), dim3(kKvThreads), 0, stream, p, a);
+    return launch_dependent(kv_append_kernel<T, BITS, D, 1>, dim3(static_cast<unsigned>(p.rows)), dim3(kKvThreads), 0, stream, p, a);
+}
+
+template <typename T, int BITS, int D, typename O>
+cudaError_t launch_read(const KvArgs& p, void* k, void* v, cudaStream_t stream) {
+    O* ko = static_cast<O*>(k);
+    O* vo = static_cast<O*>(v);
+    if (kv_many_rows<8>(p.rows))
+        return launch_dependent(kv_read_kernel<T, BITS, D, O, 8>, dim3(static_cast<unsigned>((p.rows + 7) / 8)), dim3(kKvThreads), 0, stream, p, ko, vo);
+    return launch_dependent(kv_read_kernel<T, BITS, D, O, 1>, dim3(static_cast<unsigned>(p.rows)), dim3(kKvThreads), 0, stream, p, ko, vo);
+}
+
+template <typename T, int BITS, int D>
+cudaError_t launch_read_out(const KvArgs& p, int out_dtype, void* k, void* v, cudaStream_t stream) {
+    if (out_dtype == kF32) return launch_read<T, BITS, D, float>(p, k, v, stream);
+    if (out_dtype == kF16) return launch_read<T, BITS, D, __half>(p, k, v, stream);
+    return launch_read<T, BITS, D, __nv_bfloat16>(p, k, v, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_append(const KvArgs& p, const KvAppendArgs& a, cudaStream_t stream) {
+#define B200_KV_CASE(T, BITS, D) \
+    if (p.bits == BITS && p.head_dim == D) return launch_append<T, BITS, D>(p, a, stream);
+#define B200_KV_CASES(T)                                                      \
+    B200_KV_CASE(T, 16, 128) B200_KV_CASE(T, 16, 64) B200_KV_CASE(T, 8, 128) \
+    B200_KV_CASE(T, 8, 64) B200_KV_CASE(T, 4, 128) B200_KV_CASE(T, 4, 64)
+    if (p.dtype == kF16) { B200_KV_CASES(__half) }
+    else { B200_KV_CASES(__nv_bfloat16) }
+#undef B200_KV_CASES
+#undef B200_KV_CASE
+    return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_kv_read(const KvArgs& p, int out_dtype, void* k, void* v, cudaStream_t stream) {
+    if (p.bits == 16) {
+        if (p.dtype == kF16) return p.head_dim == 128 ? launch_read_out<__half, 16, 128>(p, out_dtype, k, v, stream) : launch_read_out<__half, 16, 64>(p, out_dtype, k, v, stream);
+        return p.head_dim == 128 ? launch_read_out<__nv_bfloat16, 16, 128>(p, out_dtype, k, v, stream) : launch_read_out<__nv_bfloat16, 16, 64>(p, out_dtype, k, v, stream);
+    }
+    if (p.bits == 8) return p.head_dim == 128 ? launch_read_out<__half, 8, 128>(p, out_dtype, k, v, stream) : launch_read_out<__half, 8, 64>(p, out_dtype, k, v, stream);
+    return p.head_dim == 128 ? launch_read_out<__half, 4, 128>(p, out_dtype, k, v, stream) : launch_read_out<__half, 4, 64>(p, out_dtype, k, v, stream);
+}
+
+}  // namespace b200exl3
