@@ -164,9 +164,10 @@ int b200exl3_init(int device) {
     B200_TRY(cudaGetDeviceCount(&count), "cudaGetDeviceCount");
     if (device < 0 || device >= count) return fail("device %d out of range (%d visible)", device, count);
     B200_TRY(cudaSetDevice(device), "cudaSetDevice");
-    cudaDeviceProp prop{};
-    B200_TRY(cudaGetDeviceProperties(&prop, device), "cudaGetDeviceProperties");
-    if (prop.major != 10) return fail("device %d is sm_%d%d; this library contains sm_100a code only", device, prop.major, prop.minor);
+    int major = 0, minor = 0;                                    // two attributes: all properties take a millisecond
+    B200_TRY(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device), "cudaDeviceGetAttribute");
+    B200_TRY(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device), "cudaDeviceGetAttribute");
+    if (major != 10) return fail("device %d is sm_%d%d; this library contains sm_100a code only", device, major, minor);
     return 0;
 }
 
@@ -1999,7 +2000,7 @@ int b200exl3_kv_attention(const b200exl3_kv_cache* cache, const b200exl3_kv_batc
     if (kv_args(cache, batch, p)) return -1;
     if (max_new == 0 || max_new > batch->rows) max_new = batch->rows;
     if (kv_attention_heads(cache, heads, max_new)) return -1;
-    if (!std::isfinite(scale)) return fail("invalid attention scale");
+    if (!std::isfinite(scale) || !(scale > 0.0f)) return fail("invalid attention scale");
     if (window < 0) return fail("invalid attention window");
     if (!d_q || !d_out) return fail("NULL buffer");
     const int64_t width = static_cast<int64_t>(heads) * p.head_dim;
@@ -2017,6 +2018,7 @@ int b200exl3_kv_attention(const b200exl3_kv_cache* cache, const b200exl3_kv_batc
     a.max_new = static_cast<int>(max_new);
     a.scale_log2e = scale * 1.4426950408889634f;
     a.arrived = static_cast<unsigned int*>(ws);
+    a.error = a.arrived + kCounterBytes / sizeof(unsigned int) - 1;
     a.parts = reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes);
     return check(launch_kv_attention(p, a, as_stream(s)), "cache attention kernel");
 }

@@ -450,12 +450,17 @@ struct KvAttentionArgs {
     void* out;
     int64_t q_stride, out_stride;
     int heads, window, max_new;
+    int least_rows, most_rows; // sequences that a launch takes, by their new tokens * (heads / kv_heads)
     float scale_log2e;
-    unsigned int* arrived;     // [CTAs] arrival counters at the head of the workspace, zero on entry and on exit
+    unsigned int* arrived;     // arrival counters at the head of the workspace, zero on entry and on exit
+    unsigned int* error;       // status word of the workspace
     float* parts;              // two places per CTA for its part of a segment that CTAs share
 };
 size_t kv_attention_workspace_bytes(int bits, int head_dim, int group, int64_t max_new);
 cudaError_t launch_kv_attention(const KvArgs& args, const KvAttentionArgs& attention, cudaStream_t stream);
+// sequences of many rows on the tcgen05 tensor cores (kernels_kv_prefill.cu)
+size_t kv_many_workspace_bytes(int head_dim);
+cudaError_t launch_kv_many(const KvArgs& args, const KvAttentionArgs& attention, cudaStream_t stream);
 
 // ---- weight layout (kernels_codec.cu) -----------------------------------------------------------------
 // checkpoint layout [tiles_k, tiles_n, 8K] words -> quad layout [tiles_n/8, tiles_k, 2, 8K, 4]: the stream words of four

@@ -1,11 +1,7 @@
 // Attention of new tokens over a paged key/value cache: o_i = sum_j softmax_j(scale q_i . k_j) v_j over the tokens j up to its own
 // (with a window w: the last w of them).
 //
-// Work.  The query heads that share a key head are rows of one product: a segment is 16 * WM rows (token-major, then head) of one
-// sequence and key head, and its keys come in blocks of 64.  The blocks of all segments, one after the other, are dealt out to the
-// CTAs of one wave in equal runs, so that ragged lengths, few sequences and few heads all keep every SM busy; the lengths are read
-// on the device, so a recorded call serves growing sequences.  A CTA that holds a whole segment stores it; CTAs that share one
-// leave (maximum, sum, unnormalised rows) and the last to arrive joins the parts in order of the keys.
+// Work is shared out as kv_work.cuh says, in segments of 16 * WM rows and blocks of 64 keys.
 //
 // A block: 128 threads copy the keys and values (cp.async, 16 bytes each, several blocks in flight; what lies outside the
 // visible range is filled with zeros, so nothing behind a length is ever multiplied), WK = 4 / WM warps take 64 / WK keys each
@@ -16,7 +12,7 @@
 // scale multiplies its scores, the value's its probability.  Those probabilities are taken relative to the largest value scale met so
 // far (`unit`), so that rounding them to fp16 costs 2^-11 of what they weigh whatever the scales' magnitude.  bf16 queries enter fp16
 // multiplied by a power of two of their own (exact but for what lies 2^-24 below the row's largest).
-#include "kv.cuh"
+#include "kv_work.cuh"
 
 #include <algorithm>
 
@@ -27,12 +23,14 @@ namespace {
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps;
 constexpr int kFewKeys = 64;                       // keys of a block
 constexpr int kFewCtasPerSm = 2;
+constexpr int kFewTable = 128;
 
 template <int BITS, int D, int WM>
 struct FewShape {
     static constexpr int kWk = kFewWarps / WM;     // warps that share the rows and take different keys
     static constexpr int kWarpKeys = kFewKeys / kWk;
     static constexpr int kRows = 16 * WM;
+    static constexpr int kLanes = WM == 1 ? 1 : 32;    // a sequence has one row tile, or many
     static constexpr int kRowBytes = D * BITS / 8, kChunks = kRowBytes / 16;
     static constexpr int kTileBytes = kFewKeys * kRowBytes;
     static constexpr int kStageBytes = 2 * kTileBytes + (BITS == 16 ? 0 : 2 * kFewKeys * 4);
@@ -44,15 +42,6 @@ struct FewShape {
     static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + kOwnMergeBytes;
     static constexpr int kPartFloats = kRows * (D + 2);
 };
-
-__device__ __forceinline__ void copy16_fill(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy4_fill(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -91,68 +80,6 @@ template <int I> __device__ __forceinline__ uint32_t codes4(uint32_t w) {
     return less(d, 0x64086408u);
 }
 
-// ---- the blocks of a call -------------------------------------------------------------------------------------------
-
-struct FewSegment {
-    int first, last;       // tokens of the segment
-    int low, blocks;       // first key of the first block; blocks (one at least: rows that see nothing are stored too)
-    int key0, key1;        // visible keys
-};
-
-template <int ROWS>
-struct KvWork {
-    const KvArgs& p;
-    const KvAttentionArgs& a;
-    const int group, capacity;
-    __device__ KvWork(const KvArgs& p_, const KvAttentionArgs& a_) : p(p_), a(a_), group(a_.heads / p_.kv_heads), capacity(min(p_.table_width * static_cast<int64_t>(p_.page_size), static_cast<int64_t>(kKvMaxTokens))) {}
-
-    __device__ __forceinline__ int rows_of(const KvSeq& s) const { return min(s.n, a.max_new) * group; }
-    __device__ __forceinline__ int tiles_of(const KvSeq& s) const { return (rows_of(s) + ROWS - 1) / ROWS; }
-    __device__ __forceinline__ FewSegment segment(const KvSeq& s, int tile) const {
-        FewSegment g;
-        const int rows = rows_of(s);
-        g.first = tile * ROWS / group;
-        g.last = (min(rows, (tile + 1) * ROWS) - 1) / group;
-        g.key1 = max(0, min(s.first_pos + g.last + 1, capacity));
-        g.key0 = a.window > 0 ? max(0, s.first_pos + g.first + 1 - a.window) : 0;
-        g.low = g.key0 / kFewKeys * kFewKeys;
-        g.blocks = max(1, (g.key1 - g.low + kFewKeys - 1) / kFewKeys);
-        return g;
-    }
-    // blocks of all row tiles of a sequence, for one key head
-    __device__ __forceinline__ int64_t blocks_of(const KvSeq& s) const {
-        int64_t sum = 0;
-        const int tiles = tiles_of(s);
-        for (int t = 0; t < tiles; ++t) sum += segment(s, t).blocks;
-        return sum;
-    }
-};
-
-// A place in the list of blocks: [sequence][key head][row tile][block].
-template <int ROWS>
-struct KvCursor {
-    int b, head, tile, block;
-    KvSeq seq;
-    FewSegment seg;
-
-    __device__ __forceinline__ void enter(const KvWork<ROWS>& w) { seg = w.segment(seq, tile); }
-    // the next segment, of the next sequence that has rows
-    __device__ __forceinline__ void next_segment(const KvWork<ROWS>& w) {
-        block = 0;
-        if (++tile == w.tiles_of(seq)) {
-            tile = 0;
-            if (++head == w.p.kv_heads) {
-                head = 0;
-                do {
-                    if (++b >= w.p.batch) return;
-                    seq = kv_seq(w.p, b);
-                } while (w.rows_of(seq) == 0);
-            }
-        }
-        enter(w);
-    }
-};
-
 template <typename T, int BITS, int D, int WM>
 __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
 kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
@@ -163,61 +90,19 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
     pdl_launch_dependents();
     pdl_wait();
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ long long s_scan[kFewWarps];
-    __shared__ KvCursor<S::kRows> s_cursor;
+    using Work = KvWork<S::kRows, kFewKeys>;
+    __shared__ int64_t s_sum[kFewThreads / S::kLanes + 1];
+    __shared__ KvTable<kFewTable> s_table;
+    __shared__ KvCursor<S::kRows, kFewKeys> s_cursor;
     __shared__ float2 s_ml[kFewWarps / 2][16];
     __shared__ bool s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int wm = warp % WM, wk = warp / WM;
-    const KvWork<S::kRows> work(p, a);
-
-    // ---- this CTA's run of blocks: every thread adds up a slice of the sequences -------------------------------------
-    const int slice = (p.batch + kFewThreads - 1) / kFewThreads;
-    const int b0 = min(p.batch, tid * slice), b1 = min(p.batch, b0 + slice);
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += work.blocks_of(kv_seq(p, b)) * p.kv_heads;
-    long long upto = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += o;
-    }
-    if (lane == 31) s_scan[warp] = upto;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) {
-        if (w < warp) upto += s_scan[w];
-        total += s_scan[w];
-    }
-    const long long ctas = min(static_cast<long long>(gridDim.x), total);
-    if (blockIdx.x >= ctas) return;
-    const long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
-    if (upto - mine <= u0 && u0 < upto) {                         // one thread: the run begins in its slice
-        long long left = u0 - (upto - mine);
-        KvCursor<S::kRows> c;
-        for (int b = b0; b < b1; ++b) {
-            c.seq = kv_seq(p, b);
-            const long long per_head = work.blocks_of(c.seq);
-            if (left < per_head * p.kv_heads) {
-                c.b = b;
-                c.head = static_cast<int>(left / per_head);
-                left -= c.head * per_head;
-                for (c.tile = 0;; ++c.tile) {
-                    c.enter(work);
-                    if (left < c.seg.blocks) break;
-                    left -= c.seg.blocks;
-                }
-                c.block = static_cast<int>(left);
-                break;
-            }
-            left -= per_head * p.kv_heads;
-        }
-        s_cursor = c;
-    }
-    __syncthreads();
-    KvCursor<S::kRows> put = s_cursor, get = s_cursor;           // copies run ahead of the products
-    const int count = static_cast<int>(u1 - u0);
+    const Work work(p, a, s_table);
+    KvRun run;
+    if (!kv_find_run<kFewThreads, S::kLanes>(work, s_sum, s_cursor, run)) return;
+    KvCursor<S::kRows, kFewKeys> put = s_cursor, get = s_cursor;  // copies run ahead of the products
+    const int count = static_cast<int>(run.u1 - run.u0);
 
     // ---- copies ------------------------------------------------------------------------------------------------------
     constexpr int kPerThread = kFewKeys * S::kChunks / kFewThreads, kRowStep = kFewThreads / S::kChunks;
@@ -409,7 +294,7 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const float safe = top == -INFINITY ? 0.0f : top;     // a row that saw nothing yet
-            const float correction = exp2f(m[h] - safe);
+            const float correction = exp2_fast(m[h] - safe);
             m[h] = top;
             float sum = 0.0f;
 #pragma unroll
@@ -417,7 +302,7 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     float& x = s[i][2 * h + e];
-                    x = exp2f(x - safe);
+                    x = exp2_fast(x - safe);
                     sum += x;
                     if constexpr (BITS != 16) x *= e ? vs[i].y : vs[i].x;
                 }
@@ -473,7 +358,7 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
         if (pair) *reinterpret_cast<uint32_t*>(dst) = w;
         else *dst = reinterpret_cast<const T*>(&w)[0];
     };
-    auto finish = [&](int stage, long long seg_begin, long long seg_end) {
+    auto finish = [&](int stage, int64_t seg_begin, int64_t seg_end) {
         float* merge = reinterpret_cast<float*>(smem + (S::kMergeInStage ? stage : S::kStages) * S::kStageBytes);
         if constexpr (S::kMergeInStage && S::kWk > 1) __syncthreads();     // every warp is through with the block
 #pragma unroll
@@ -508,7 +393,7 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
                 for (int h = 0; h < 2; ++h) {
                     const float2 o = s_ml[wk * WM + wm][g + 8 * h];
                     const float top = fmaxf(m[h], o.x), safe = top == -INFINITY ? 0.0f : top;
-                    const float c0 = exp2f(m[h] - safe), c1 = exp2f(o.x - safe);
+                    const float c0 = exp2_fast(m[h] - safe), c1 = exp2_fast(o.x - safe);
                     m[h] = top;
                     l[h] = l[h] * c0 + o.y * c1;
 #pragma unroll
@@ -521,14 +406,14 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
             __syncthreads();
         }
         const int rows = work.rows_of(get.seq), tile0 = get.tile * S::kRows;
-        const long long c0 = ((seg_begin + 1) * ctas - 1) / total, c1 = (seg_end * ctas - 1) / total;     // CTAs that hold its first and last block
+        const int c0 = run.cta_of(seg_begin), c1 = run.cta_of(seg_end - 1);                 // CTAs that hold its first and last block
         if (c0 == c1) {
             if (wk == 0) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int r = tile0 + wm * 16 + g + 8 * h;
                     if (r >= rows) continue;
-                    const float inverse = l[h] > 0.0f ? 1.0f / l[h] : (l[h] == 0.0f ? 0.0f : l[h]);      // a row that sees nothing is zero
+                    const float inverse = kv_inverse(l[h]);
 #pragma unroll
                     for (int i = 0; i < kTiles; ++i) {
                         if constexpr (BITS == 16) {
@@ -543,7 +428,7 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
             return;
         }
         // this CTA's part: its first place for a segment that began before its run, else the second
-        auto part_of = [&](long long c) { return a.parts + (2 * c + (c == c0 ? 1 : 0)) * static_cast<int64_t>(S::kPartFloats); };
+        auto part_of = [&](int c) { return a.parts + (2 * c + (c == c0 ? 1 : 0)) * static_cast<int64_t>(S::kPartFloats); };
         float* part = part_of(blockIdx.x);
         if (wk == 0) {
 #pragma unroll
@@ -568,7 +453,7 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
         if (!s_last) return;
         __threadfence();
         // a warp joins a row: its lanes weigh the parts, then every lane adds its dimensions over the parts in order
-        const int parts = static_cast<int>(c1 - c0) + 1, rows_here = min(S::kRows, rows - tile0);
+        const int parts = c1 - c0 + 1, rows_here = min(S::kRows, rows - tile0);
         for (int r = warp; r < rows_here; r += kFewWarps) {
             auto weight_of = [&](int q_) { return __ldcg(reinterpret_cast<const float2*>(part_of(c0 + q_) + S::kRows * D) + r); };
             float top = -INFINITY;
@@ -582,7 +467,7 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
             for (int q0 = 0; q0 < parts; q0 += 32) {
                 float2 ml = make_float2(-INFINITY, 0.0f);
                 if (q0 + lane < parts) ml = weight_of(q0 + lane);
-                const float c = exp2f(ml.x - safe);
+                const float c = exp2_fast(ml.x - safe);
                 sum += c * ml.y;
                 const int n = min(32, parts - q0);
 #pragma unroll 8
@@ -595,14 +480,14 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
             }
 #pragma unroll
             for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            const float inverse = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+            const float inverse = kv_inverse(sum);
 #pragma unroll
             for (int e = 0; e < D / 32; e += 2) store_row(tile0 + r, lane * (D / 32) + e, o[e] * inverse, o[e + 1] * inverse, true);
         }
     };
 
     // ---- the run ------------------------------------------------------------------------------------------------------
-    long long seg_begin = u0 - get.block;
+    int64_t seg_begin = run.u0 - get.block;
     begin();
 #pragma unroll 1
     for (int it = 0; it < count; ++it) {
@@ -640,17 +525,34 @@ cudaError_t launch_few(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t s
     return launch_dependent(kv_few_kernel<T, BITS, D, WM>, dim3(static_cast<unsigned>(kFewCtasPerSm * sm_count())), dim3(kFewThreads), S::kSmem, stream, p, a);
 }
 
+// Up to this many rows per key head the few-row kernel takes a sequence.
+constexpr int kFewRows = 16;
+
 template <typename T, int BITS, int D>
-cudaError_t launch_attention(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t stream) {
+cudaError_t launch_attention(const KvArgs& p, KvAttentionArgs a, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(a.max_new) * (a.heads / p.kv_heads);
-    return rows <= 16 ? launch_few<T, BITS, D, 1>(p, a, stream) : launch_few<T, BITS, D, 4>(p, a, stream);
+    a.least_rows = 1;
+    a.most_rows = INT32_MAX;
+    if (rows <= kFewRows) return launch_few<T, BITS, D, 1>(p, a, stream);
+    if constexpr (BITS != 16) {
+        return launch_few<T, BITS, D, 4>(p, a, stream);
+    } else {
+        if (p.batch > 1) {                                        // sequences of few rows among the others
+            a.most_rows = kFewRows;
+            const cudaError_t e = launch_few<T, BITS, D, 1>(p, a, stream);
+            if (e != cudaSuccess) return e;
+            a.least_rows = kFewRows + 1;
+            a.most_rows = INT32_MAX;
+        }
+        return launch_kv_many(p, a, stream);
+    }
 }
 
 }  // namespace
 
-size_t kv_attention_workspace_bytes(int, int head_dim, int group, int64_t max_new) {
-    const size_t rows = max_new * group <= 16 ? 16 : 64;
-    return 2 * static_cast<size_t>(kFewCtasPerSm * sm_count()) * rows * (head_dim + 2) * sizeof(float);
+size_t kv_attention_workspace_bytes(int bits, int head_dim, int group, int64_t max_new) {
+    const size_t few = 2 * static_cast<size_t>(kFewCtasPerSm * sm_count()) * (bits == 16 ? 16 : 64) * (head_dim + 2) * sizeof(float);
+    return max_new * group <= kFewRows ? few : std::max(few, kv_many_workspace_bytes(head_dim));
 }
 
 cudaError_t launch_kv_attention(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t stream) {

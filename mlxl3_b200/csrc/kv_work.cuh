@@ -1,0 +1,217 @@
+// How the attention kernels over the paged cache share out their work.  A segment is up to ROWS rows (token-major, then head) of one
+// sequence and key head -- the query heads that share a key head are rows of one product -- and its keys come in blocks of KEYS.  The
+// blocks of all segments, one after the other, are dealt out to the CTAs of one wave in equal runs: ragged lengths, few sequences
+// and few heads all keep every SM busy, and since the lengths are read on the device a recorded call serves growing sequences.
+// A CTA that holds a whole segment stores it; CTAs that share one leave (maximum, sum, unnormalised rows) and the last to arrive joins
+// the parts in the order of the keys.
+#pragma once
+
+#include "kv.cuh"
+
+namespace b200exl3 {
+
+struct KvSegment {
+    int first, last;       // tokens of the segment
+    int low, blocks;       // first key of the first block; blocks (one at least: rows that see nothing are stored too)
+    int key0, key1;        // visible keys
+};
+
+// Sequences whose first rows and lengths a CTA keeps in shared memory; more are read where they are.
+template <int CAP>
+struct KvTable {
+    int start[CAP + 1], length[CAP];
+};
+
+template <int ROWS, int KEYS>
+struct KvWork {
+    const KvArgs& p;
+    const KvAttentionArgs& a;
+    const int* start;      // [batch + 1], [batch]
+    const int* length;
+    int group, capacity;
+
+    template <int CAP>
+    __device__ __forceinline__ KvWork(const KvArgs& p_, const KvAttentionArgs& a_, KvTable<CAP>& table) : p(p_), a(a_) {
+        group = a.heads / p.kv_heads;
+        capacity = static_cast<int>(min(p.table_width * static_cast<int64_t>(p.page_size), static_cast<int64_t>(kKvMaxTokens)));
+        start = p.row_start;
+        length = p.length;
+        if (p.batch <= CAP) {
+            for (int i = threadIdx.x; i <= p.batch; i += blockDim.x) {
+                table.start[i] = __ldg(p.row_start + i);
+                if (i < p.batch) table.length[i] = __ldg(p.length + i);
+            }
+            __syncthreads();
+            start = table.start;
+            length = table.length;
+        }
+    }
+    __device__ __forceinline__ KvSeq seq(int b) const {
+        KvSeq s;
+        s.first_row = kv_clamp_row(p, start[b]);
+        s.n = max(0, kv_clamp_row(p, start[b + 1]) - s.first_row);
+        s.first_pos = kv_clamp_length(length[b]) - s.n;
+        return s;
+    }
+    // rows of a sequence that this kernel takes: all or none
+    __device__ __forceinline__ int rows_of(const KvSeq& s) const {
+        const int rows = min(s.n, a.max_new) * group;
+        return rows >= a.least_rows && rows <= a.most_rows ? rows : 0;
+    }
+    __device__ __forceinline__ int tiles_of(const KvSeq& s) const { return (rows_of(s) + ROWS - 1) / ROWS; }
+    __device__ __forceinline__ KvSegment segment(const KvSeq& s, int tile) const {
+        KvSegment g;
+        const int rows = min(s.n, a.max_new) * group;
+        g.first = tile * ROWS / group;
+        g.last = (min(rows, (tile + 1) * ROWS) - 1) / group;
+        g.key1 = max(0, min(s.first_pos + g.last + 1, capacity));
+        g.key0 = a.window > 0 ? max(0, s.first_pos + g.first + 1 - a.window) : 0;
+        g.low = g.key0 / KEYS * KEYS;
+        g.blocks = max(1, (g.key1 - g.low + KEYS - 1) / KEYS);
+        return g;
+    }
+    // blocks of all row tiles of a sequence, for one key head; LANES neighbouring lanes count together
+    template <int LANES>
+    __device__ __forceinline__ int64_t blocks_of(const KvSeq& s) const {
+        int64_t sum = 0;
+        const int tiles = tiles_of(s);
+        for (int t = LANES > 1 ? static_cast<int>(threadIdx.x) % LANES : 0; t < tiles; t += LANES) sum += segment(s, t).blocks;
+#pragma unroll
+        for (int d = LANES / 2; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        return sum;
+    }
+};
+
+// A place in the list of blocks: [sequence][key head][row tile][block].
+template <int ROWS, int KEYS>
+struct KvCursor {
+    int b, head, tile, block;
+    KvSeq seq;
+    KvSegment seg;
+
+    // the next segment, of the next sequence that has rows
+    __device__ __forceinline__ void next_segment(const KvWork<ROWS, KEYS>& w) {
+        block = 0;
+        if (++tile == w.tiles_of(seq)) {
+            tile = 0;
+            if (++head == w.p.kv_heads) {
+                head = 0;
+                do {
+                    if (++b >= w.p.batch) return;
+                    seq = w.seq(b);
+                } while (w.rows_of(seq) == 0);
+            }
+        }
+        seg = w.segment(seq, tile);
+    }
+};
+
+// A CTA's run of blocks u0 .. u1 - 1 of `total`, dealt out to `ctas` CTAs.
+struct KvRun {
+    int64_t total, u0, u1;
+    int ctas;
+
+    // the CTA that holds block u
+    __device__ __forceinline__ int cta_of(int64_t u) const { return static_cast<int>(((u + 1) * ctas - 1) / total); }
+};
+
+// Finds this CTA's run; every thread of the block calls it.  Workers of LANES threads (1, or 32: sequences of many row tiles) count a
+// slice of the sequences each; the one whose slice holds the first block writes the place.  Returns false where there is nothing to do.
+template <int THREADS, int LANES, int ROWS, int KEYS>
+__device__ __forceinline__ bool kv_find_run(const KvWork<ROWS, KEYS>& w, int64_t (&s_sum)[THREADS / LANES + 1], KvCursor<ROWS, KEYS>& s_cursor, KvRun& run) {
+    constexpr int kWorkers = THREADS / LANES;
+    static_assert(LANES == 1 || LANES == 32, "threads or warps");
+    const int worker = threadIdx.x / LANES, sub = threadIdx.x % LANES;
+    const int slice = (w.p.batch + kWorkers - 1) / kWorkers;
+    const int b0 = min(w.p.batch, worker * slice), b1 = min(w.p.batch, b0 + slice);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += w.template blocks_of<LANES>(w.seq(b)) * w.p.kv_heads;
+    if (sub == 0) s_sum[worker] = mine;
+    __syncthreads();
+    if (threadIdx.x < 32) {                                       // exclusive sums
+        int64_t carry = 0;
+        for (int i0 = 0; i0 < kWorkers; i0 += 32) {
+            const int i = i0 + static_cast<int>(threadIdx.x);
+            const int64_t own = i < kWorkers ? s_sum[i] : 0;
+            int64_t upto = own;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t o = __shfl_up_sync(0xffffffffu, upto, d);
+                if (static_cast<int>(threadIdx.x) >= d) upto += o;
+            }
+            if (i < kWorkers) s_sum[i] = carry + upto - own;
+            carry += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (threadIdx.x == 0) s_sum[kWorkers] = carry;
+    }
+    __syncthreads();
+    run.total = s_sum[kWorkers];
+    run.ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), run.total));
+    if (static_cast<int>(blockIdx.x) >= run.ctas) return false;
+    run.u0 = run.total * blockIdx.x / run.ctas;
+    run.u1 = run.total * (blockIdx.x + 1) / run.ctas;
+    const int64_t before = s_sum[worker];
+    if (before <= run.u0 && run.u0 < before + mine) {
+        int64_t left = run.u0 - before;
+        KvCursor<ROWS, KEYS> c;
+        for (int b = b0; b < b1; ++b) {
+            c.seq = w.seq(b);
+            const int64_t per_head = w.template blocks_of<LANES>(c.seq);
+            if (left >= per_head * w.p.kv_heads) {
+                left -= per_head * w.p.kv_heads;
+                continue;
+            }
+            c.b = b;
+            c.head = static_cast<int>(left / per_head);
+            left -= c.head * per_head;
+            for (c.tile = 0;; c.tile += LANES) {
+                const int tile = c.tile + sub, tiles = w.tiles_of(c.seq);
+                const int n = tile < tiles ? w.segment(c.seq, tile).blocks : 0;
+                if constexpr (LANES == 1) {
+                    if (left < n) break;
+                    left -= n;
+                } else {
+                    int upto = n;
+#pragma unroll
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const int o = __shfl_up_sync(0xffffffffu, upto, d);
+                        if (sub >= d) upto += o;
+                    }
+                    const unsigned int past = __ballot_sync(0xffffffffu, left < upto);
+                    if (past != 0) {
+                        const int lane = __ffs(past) - 1;
+                        left -= __shfl_sync(0xffffffffu, upto - n, lane);
+                        c.tile += lane;
+                        break;
+                    }
+                    left -= __shfl_sync(0xffffffffu, upto, 31);
+                }
+            }
+            c.seg = w.segment(c.seq, c.tile);
+            c.block = static_cast<int>(left);
+            break;
+        }
+        if (sub == 0) s_cursor = c;
+    }
+    __syncthreads();
+    return true;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {             // 2 ulp; exp2(-inf) = 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 1 / sum of a row; a row that sees nothing is zero
+__device__ __forceinline__ float kv_inverse(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
+
+__device__ __forceinline__ void copy16_fill(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4_fill(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+}  // namespace b200exl3

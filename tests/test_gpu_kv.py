@@ -365,6 +365,31 @@ def test_attention_long(gpu, bits):
     attend(s, 4, max_new=1)
 
 
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("dtype,d,heads,kv_heads,page,window,seqs", [
+    (F16, 128, 4, 1, 16, 0, [(700, 700), (1, 90), (130, 900), (0, 4), (33, 40)]), (BF16, 128, 2, 2, 64, 0, [(257, 1500)]),
+    (BF16, 64, 14, 2, 24, 200, [(300, 300), (20, 777)]), (F16, 64, 2, 2, 128, 0, [(128, 128), (129, 129), (256, 511)]),
+    (F16, 128, 5, 1, 32, 64, [(16, 1200), (26, 26), (200, 150)]), (BF16, 128, 8, 8, 16, 0, [(300, 2000)])])
+def test_attention_prompts(gpu, bits, dtype, d, heads, kv_heads, page, window, seqs):
+    s = Setup(seqs, dtype, bits, kv_heads, d, page, seed=heads + bits + 200, window=window, gap=3)
+    attend(s, heads, window, wide=8)
+
+
+def test_attention_maximum_that_climbs(gpu):
+    # every key scores higher than the ones before, by far more than a row's maximum is left behind
+    s = Setup([(140, 1000)], F16, 16, 1, 128, 16, seed=30)
+    one = np.ones(128) / 8
+    for t in range(1000):
+        s.pool["k"][s.table[0, t // 16], 0, t % 16] = raw(one * (t / 40.0), F16)
+    s.upload()
+    width, heads = 2 * 128, 2
+    q = raw(np.ones((s.rows, width)) * 2.0, F16)
+    d_q, d_out = s.Buffer.from_numpy(q), s.Buffer.from_numpy(q)
+    ws = s.kv.new_attention_workspace(s.cache, s.batch, heads)
+    s.kv.attention(s.cache, s.batch, d_q.ptr, heads, 128 ** -0.5, d_out.ptr, ws)
+    check_attention(s, heads, q, d_out.download(q.shape, np.uint16), q)
+
+
 def test_attention_rows_beyond_max_new(gpu):
     s = Setup([(6, 90), (2, 40)], F16, 16, 2, 128, 16, seed=8)
     attend(s, 4, max_new=3)
