@@ -11,11 +11,14 @@
 // 256, which 16 bits hold as well as 1, and O_x and the sum stay in the same unit.  When it moves, the row's thread rescales O_x in
 // tensor memory; S_x of a block being complete implies that the product before it is, so nothing else has to be waited for.
 //
-// Four warps bring the data: cp.async, 16 bytes each, zeros for what lies outside the visible range, into the 128-byte swizzle that the
-// products read.  One thread issues the products.  Every wait is bounded; one that gives up sets the status word, all roles run on
+// Four warps bring the data, a tile (a block's keys or values) each in turn, into the 128-byte swizzle that the products read: tensor
+// copies of whole pages or parts of pages where every key of the block is visible, else 16 bytes at a time with zeros for what lies
+// outside the visible range.  One thread issues the products.  Every wait is bounded; one that gives up sets the status word, all roles run on
 // to the end, and the kernel frees its tensor memory.
 #include "kv_work.cuh"
 #include "tcgen05.cuh"
+
+#include <cuda.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -26,7 +29,6 @@ namespace {
 
 constexpr int kManyKeys = 128, kManyTile = 128, kManyRows = 2 * kManyTile;
 constexpr int kSoftmaxWarps = 8, kLoadWarps = 4;
-constexpr int kLoadThreads = 32 * kLoadWarps;
 constexpr int kManyThreads = 32 * (kSoftmaxWarps + kLoadWarps + 1);
 constexpr int kManyTable = 512;
 constexpr uint32_t kScoreCols = 128;               // tensor-memory columns of S_x; P_x lies in their second half
@@ -36,7 +38,9 @@ struct ManyShape {
     static constexpr int kTileBytes = kManyKeys * D * 2;           // a block's keys or values, as the products read them
     static constexpr int kSlots = D == 128 ? 4 : 6;                // keys and values in flight, alternately
     static constexpr int kQueryBytes = kManyRows * D * 2;
-    static constexpr size_t kSmem = 1024 + kQueryBytes + static_cast<size_t>(kSlots) * kTileBytes;
+    static constexpr int kStageRow = 80;                           // a row of 32 results on its way out, 64 bytes without bank conflicts
+    static constexpr int kStageBytes = kSoftmaxWarps * 32 * kStageRow;
+    static constexpr size_t kSmem = 1024 + kQueryBytes + static_cast<size_t>(kSlots) * kTileBytes + kStageBytes;
     static constexpr int kPartFloats = kManyRows * (D + 2);
     static constexpr uint32_t kOutCols = 2 * kScoreCols;           // first column of O_0; O_1 lies D further
 };
@@ -83,9 +87,26 @@ __device__ __forceinline__ uint32_t many_at(int rows, int r, int c) {
     return static_cast<uint32_t>((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(c0), "r"(c1) : "memory");
+}
+
+// Two fp32 numbers in one instruction
+struct Pair {
+    uint64_t v;
+    __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Pair fma2(Pair a, const Pair& b, const Pair& c) { asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(a.v) : "l"(b.v), "l"(c.v)); return a; }
+__device__ __forceinline__ Pair add2(Pair a, const Pair& b) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v)); return a; }
+
+// box_rows: rows of a tensor copy, a power of two that divides the page size, or 0: no tensor copies
 template <typename T, int BITS, int D>
 __global__ void __launch_bounds__(kManyThreads, 1)
-kv_many_kernel(const KvArgs p, const KvAttentionArgs a) {
+kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const KvArgs p, const KvAttentionArgs a,
+               const int box_rows) {
     using S = ManyShape<BITS, D>;
     using Work = KvWork<kManyRows, kManyKeys>;
     using Cursor = KvCursor<kManyRows, kManyKeys>;
@@ -96,7 +117,7 @@ kv_many_kernel(const KvArgs p, const KvAttentionArgs a) {
     __shared__ KvTable<kManyTable> s_table;
     __shared__ int64_t s_sum[kManyThreads / 32 + 1];
     __shared__ Cursor s_cursor;
-    __shared__ __align__(8) uint64_t kv_full[S::kSlots], kv_free[S::kSlots], s_full[2], p_full[2], o_full[2], q_free, drained;
+    __shared__ __align__(8) uint64_t kv_full[S::kSlots], kv_free[S::kSlots], s_full[2], p_full[2], o_full[2], q_full[2], drained;
     __shared__ uint32_t tmem_base_slot;
     __shared__ int s_last[2];
     __shared__ volatile int s_failed;
@@ -110,9 +131,8 @@ kv_many_kernel(const KvArgs p, const KvAttentionArgs a) {
     unsigned char* const tiles = queries + S::kQueryBytes;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kSlots; ++s) { mbar_init(&kv_full[s], kLoadThreads); mbar_init(&kv_free[s], 1); }
-        for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 1); mbar_init(&p_full[x], kManyTile); mbar_init(&o_full[x], 1); }
-        mbar_init(&q_free, 1);
+        for (int s = 0; s < S::kSlots; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], 1); }
+        for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 1); mbar_init(&p_full[x], kManyTile); mbar_init(&o_full[x], 1); mbar_init(&q_full[x], kManyTile); }
         mbar_init(&drained, 1);
         s_failed = 0;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -133,13 +153,41 @@ kv_many_kernel(const KvArgs p, const KvAttentionArgs a) {
         uint32_t s_par = 0, o_par = 0;
         int done = 0;
         int64_t seg_begin = run.u0 - at.block;
+        // the cursor at the next segment that has rows of this tile, from where it is
+        auto settle = [&]() {
+            while (done < count && x == 1 && work.rows_of(at.seq) - at.tile * kManyRows <= kManyTile) {
+                done += min(count - done, at.seg.blocks - at.block);
+                seg_begin += at.seg.blocks;
+                if (done < count) at.next_segment(work);
+            }
+        };
+        // this thread's row of queries; rows past the last are zeros
+        auto ask_queries = [&]() {
+            const int row = at.tile * kManyRows + x * kManyTile + r, token = row / work.group;
+            const bool live = row < work.rows_of(at.seq);
+            const T* src = static_cast<const T*>(a.q) + (live ? (at.seq.first_row + token) * a.q_stride +
+                                                                   static_cast<int64_t>(at.head * work.group + row - token * work.group) * D
+                                                              : 0);
+            const uint32_t dst = smem_addr(queries) + x * (S::kQueryBytes / 2);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) copy16_fill(dst + many_at(kManyTile, r, c), src + (live ? c * 8 : 0), live);
+            copy_commit();
+        };
+        auto tell_queries = [&]() {
+            copy_wait<0>();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(&q_full[x]);
+        };
+        settle();
+        if (done < count) {
+            ask_queries();
+            tell_queries();
+        }
         while (done < count) {
-            const int rows = work.rows_of(at.seq), row = at.tile * kManyRows + x * kManyTile + r;
-            const int n = min(count - done, at.seg.blocks - at.block);
-            const bool two = rows - at.tile * kManyRows > kManyTile;
-            if (x == 0 || two) {
+            {
+                const int row = at.tile * kManyRows + x * kManyTile + r, n = min(count - done, at.seg.blocks - at.block);
                 const int token = row / work.group;
-                const bool live = row < rows;
+                const bool live = row < work.rows_of(at.seq);
                 const int position = live ? at.seq.first_pos + token : -1;
                 const int end = min(position + 1, work.capacity), start = a.window > 0 ? position + 1 - a.window : 0;
                 float m = -INFINITY, l = 0.0f;
@@ -151,33 +199,34 @@ kv_many_kernel(const KvArgs p, const KvAttentionArgs a) {
                     s_par ^= 1u;
                     __syncwarp();
                     fence_after();
+                    // columns of a pair of loads that the row does not see
                     const bool masked = __any_sync(0xffffffffu, e < kManyKeys || b > 0);
                     uint32_t v0[32], v1[32];
-                    auto largest = [&](uint32_t (&v)[32], int col, float top) {
+                    auto load = [&](int col) {
+                        __syncwarp();
+                        tmem_ld32(scores + col, v0);
+                        tmem_ld32(scores + col + 32, v1);
+                        tmem_wait_ld();
                         if (masked) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = col + i < e && col + i >= b ? v[i] : 0xff800000u;
+                            for (int i = 0; i < 32; ++i) {
+                                v0[i] = col + i < e && col + i >= b ? v0[i] : 0xff800000u;
+                                v1[i] = col + 32 + i < e && col + 32 + i >= b ? v1[i] : 0xff800000u;
+                            }
                         }
-                        float t0 = top, t1 = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            t0 = fmaxf(t0, __uint_as_float(v[i]));
-                            t1 = fmaxf(t1, __uint_as_float(v[i + 1]));
-                        }
-                        return fmaxf(t0, t1);
                     };
                     float top = -INFINITY;
-                    tmem_ld32(scores, v0);
-                    tmem_ld32(scores + 32, v1);
-                    tmem_wait_ld();
-                    top = largest(v0, 0, top);
-                    top = largest(v1, 32, top);
-                    __syncwarp();
-                    tmem_ld32(scores + 64, v0);
-                    tmem_ld32(scores + 96, v1);
-                    tmem_wait_ld();
-                    top = largest(v0, 64, top);
-                    top = largest(v1, 96, top);
+#pragma unroll 1
+                    for (int col = 0; col < kManyKeys; col += 64) {
+                        load(col);
+                        float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            t0 = fmaxf(t0, fmaxf(__uint_as_float(v0[i]), __uint_as_float(v0[i + 1])));
+                            t1 = fmaxf(t1, fmaxf(__uint_as_float(v1[i]), __uint_as_float(v1[i + 1])));
+                        }
+                        top = fmaxf(top, fmaxf(t0, t1));
+                    }
                     top *= a.scale_log2e;
                     const bool moves = top > m + 8.0f;                           // also from -inf
                     if (__any_sync(0xffffffffu, moves)) {
@@ -187,93 +236,121 @@ kv_many_kernel(const KvArgs p, const KvAttentionArgs a) {
                         l *= factor;
                         if (j > 0) {
 #pragma unroll 1
-                            for (int c = 0; c < D; c += 16) {
-                                uint32_t o[16];
+                            for (int c = 0; c < D; c += 32) {
                                 __syncwarp();
-                                asm volatile(
-                                    "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                                    : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]), "=r"(o[8]),
-                                      "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
-                                    : "r"(outs + c) : "memory");
+                                uint32_t o[32];
+                                tmem_ld32(outs + c, o);
                                 tmem_wait_ld();
+                                uint32_t o0[16], o1[16];
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-                                tmem_st16(outs + c, o);
+                                for (int i = 0; i < 16; ++i) {
+                                    o0[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                                    o1[i] = __float_as_uint(__uint_as_float(o[16 + i]) * factor);
+                                }
+                                tmem_st16(outs + c, o0);
+                                tmem_st16(outs + c + 16, o1);
                             }
+                            load(kManyKeys - 64);
                         }
                     }
-                    const float shift = m == -INFINITY ? 0.0f : -m;
-                    // columns 64 .. 127 are in registers; their probabilities go where those scores lay, then columns 0 .. 63
-                    float l0 = 0.0f, l1 = 0.0f;
-                    auto put = [&](uint32_t (&v)[32], int col) {
+                    // the upper columns are in registers; their probabilities go where those scores lay, then the lower ones'
+                    const Pair scale2(a.scale_log2e, a.scale_log2e), shift2(m == -INFINITY ? 0.0f : -m, m == -INFINITY ? 0.0f : -m);
+                    Pair l2(0.0f, 0.0f);
+                    auto put = [&](const uint32_t (&v)[32], int col) {
                         uint32_t w[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const float p0 = exp2_fast(fmaf(__uint_as_float(v[2 * i]), a.scale_log2e, shift));
-                            const float p1 = exp2_fast(fmaf(__uint_as_float(v[2 * i + 1]), a.scale_log2e, shift));
-                            l0 += p0;
-                            l1 += p1;
-                            w[i] = KvType<T>::pack(p0, p1);
+                            float x0, x1;
+                            fma2(Pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, shift2).get(x0, x1);
+                            x0 = exp2_fast(x0);
+                            x1 = exp2_fast(x1);
+                            l2 = add2(l2, Pair(x0, x1));
+                            w[i] = KvType<T>::pack(x0, x1);
                         }
                         __syncwarp();
                         tmem_st16(probs + col / 2, w);
                     };
-                    put(v0, 64);
-                    put(v1, 96);
-                    tmem_ld32(scores, v0);
-                    tmem_ld32(scores + 32, v1);
-                    tmem_wait_ld();
-                    if (masked) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            v0[i] = i < e && i >= b ? v0[i] : 0xff800000u;
-                            v1[i] = 32 + i < e && 32 + i >= b ? v1[i] : 0xff800000u;
-                        }
+#pragma unroll 1
+                    for (int col = kManyKeys - 64;; col -= 64) {
+                        put(v1, col + 32);
+                        put(v0, col);
+                        if (col == 0) break;
+                        load(col - 64);
                     }
-                    put(v0, 0);
-                    put(v1, 32);
+                    float l0, l1;
+                    l2.get(l0, l1);
                     l += l0 + l1;
                     tmem_wait_st();
                     fence_before();
                     mbar_arrive(&p_full[x]);
                 }
+                // the products that read the queries are done: those of the next segment may come
+                const Cursor here = at;
+                const int64_t here_begin = seg_begin;
+                done += n;
+                seg_begin += at.seg.blocks;
+                if (done < count) at.next_segment(work);
+                settle();
+                if (done < count) ask_queries();
                 // ---- the segment's rows, or this CTA's part of them
                 qmm_wait(&o_full[x], o_par, &s_failed);
                 o_par ^= 1u;
                 __syncwarp();
                 fence_after();
-                const int c0 = run.cta_of(seg_begin), c1 = run.cta_of(seg_begin + at.seg.blocks - 1);
-                T* const dst = static_cast<T*>(a.out) + (at.seq.first_row + token) * a.out_stride +
-                               static_cast<int64_t>(at.head * work.group + row - token * work.group) * D;
+                const int c0 = run.cta_of(here_begin), c1 = run.cta_of(here_begin + here.seg.blocks - 1);
                 auto part_of = [&](int c) { return a.parts + (2 * c + (c == c0 ? 1 : 0)) * static_cast<int64_t>(S::kPartFloats); };
                 const int pr = x * kManyTile + r;
                 const bool whole = c0 == c1;
+                // 32 results of the warp's 32 rows at a time go through shared memory, so that four lanes store 64 bytes of a row
+                unsigned char* const stage = tiles + S::kSlots * S::kTileBytes + warp * 32 * S::kStageRow;
+                T* dst[4];                                        // of the rows that this lane stores a quarter of
+                {
+                    const int rows_here = work.rows_of(here.seq), lane = threadIdx.x & 31;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int q_row = here.tile * kManyRows + x * kManyTile + (warp & 3) * 32 + i * 8 + lane / 4, q_token = q_row / work.group;
+                        dst[i] = q_row < rows_here ? static_cast<T*>(a.out) + (here.seq.first_row + q_token) * a.out_stride +
+                                                         static_cast<int64_t>(here.head * work.group + q_row - q_token * work.group) * D + (lane & 3) * 8
+                                                   : nullptr;
+                    }
+                }
+                auto store = [&](const float (&v)[32], int c) {   // results c .. c + 31 of this thread's row
+                    __syncwarp();
+                    const int lane = threadIdx.x & 31;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<uint4*>(stage + lane * S::kStageRow + i * 16) =
+                            make_uint4(KvType<T>::pack(v[8 * i], v[8 * i + 1]), KvType<T>::pack(v[8 * i + 2], v[8 * i + 3]),
+                                       KvType<T>::pack(v[8 * i + 4], v[8 * i + 5]), KvType<T>::pack(v[8 * i + 6], v[8 * i + 7]));
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (dst[i] != nullptr)
+                            *reinterpret_cast<uint4*>(dst[i] + c) = *reinterpret_cast<const uint4*>(stage + (i * 8 + lane / 4) * S::kStageRow + (lane & 3) * 16);
+                };
                 const float inverse = kv_inverse(l);
-                float* const mine = whole ? nullptr : part_of(blockIdx.x) + pr * D;
+                float4* const mine = whole ? nullptr : reinterpret_cast<float4*>(part_of(blockIdx.x)) + pr;      // [four results][row]
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     uint32_t v[32];
                     __syncwarp();
                     tmem_ld32(outs + c, v);
                     tmem_wait_ld();
-                    if (!live) continue;
+                    float f[32];
                     if (whole) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                w[k] = KvType<T>::pack(__uint_as_float(v[i + 2 * k]) * inverse, __uint_as_float(v[i + 2 * k + 1]) * inverse);
-                            *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]) * inverse;
+                        store(f, c);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(mine + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        for (int i = 0; i < 8; ++i)
+                            __stcg(mine + (c / 4 + i) * kManyRows, make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                                                              __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])));
                     }
                 }
                 fence_before();
                 if (!whole) {
-                    if (live) reinterpret_cast<float2*>(part_of(blockIdx.x) + kManyRows * D)[pr] = make_float2(m, l);
+                    reinterpret_cast<float2*>(part_of(blockIdx.x) + kManyRows * D)[pr] = make_float2(m, l);
                     __threadfence();
                     group_sync(1 + x, kManyTile);
                     if (r == 0) {
@@ -282,112 +359,106 @@ kv_many_kernel(const KvArgs p, const KvAttentionArgs a) {
                         if (s_last[x]) *counter = 0;                              // the next call starts from zero
                     }
                     group_sync(1 + x, kManyTile);
-                    if (s_last[x] && live) {
+                    if (s_last[x]) {
                         __threadfence();
                         auto weight_of = [&](int c) { return __ldcg(reinterpret_cast<const float2*>(part_of(c) + kManyRows * D) + pr); };
                         float top = -INFINITY, sum = 0.0f;
-                        for (int c = c0; c <= c1; ++c) top = fmaxf(top, weight_of(c).x);
-                        const float safe = top == -INFINITY ? 0.0f : top;
                         for (int c = c0; c <= c1; ++c) {
                             const float2 ml = weight_of(c);
-                            sum = fmaf(exp2_fast(ml.x - safe), ml.y, sum);
+                            const float to = fmaxf(top, ml.x), safe = to == -INFINITY ? 0.0f : to;
+                            sum = sum * exp2_fast(top - safe) + ml.y * exp2_fast(ml.x - safe);
+                            top = to;
                         }
-                        const float inv = kv_inverse(sum);
+                        const float safe = top == -INFINITY ? 0.0f : top, inv = kv_inverse(sum);
 #pragma unroll 1
                         for (int d = 0; d < D; d += 32) {
-                            float4 o[8];
+                            float o[32];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+#pragma unroll 1
                             for (int c = c0; c <= c1; ++c) {
-                                const float w = exp2_fast(weight_of(c).x - safe);
-                                const float4* src = reinterpret_cast<const float4*>(part_of(c) + pr * D + d);
+                                const float w = exp2_fast(weight_of(c).x - safe) * inv;
+                                const float4* src = reinterpret_cast<const float4*>(part_of(c)) + (d / 4) * kManyRows + pr;
+                                float4 f[8];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) f[i] = __ldcg(src + i * kManyRows);
 #pragma unroll
                                 for (int i = 0; i < 8; ++i) {
-                                    const float4 f = __ldcg(src + i);
-                                    o[i].x = fmaf(f.x, w, o[i].x); o[i].y = fmaf(f.y, w, o[i].y); o[i].z = fmaf(f.z, w, o[i].z); o[i].w = fmaf(f.w, w, o[i].w);
+                                    o[4 * i] = fmaf(f[i].x, w, o[4 * i]);
+                                    o[4 * i + 1] = fmaf(f[i].y, w, o[4 * i + 1]);
+                                    o[4 * i + 2] = fmaf(f[i].z, w, o[4 * i + 2]);
+                                    o[4 * i + 3] = fmaf(f[i].w, w, o[4 * i + 3]);
                                 }
                             }
-#pragma unroll
-                            for (int i = 0; i < 8; i += 2)
-                                *reinterpret_cast<uint4*>(dst + d + 4 * i) =
-                                    make_uint4(KvType<T>::pack(o[i].x * inv, o[i].y * inv), KvType<T>::pack(o[i].z * inv, o[i].w * inv),
-                                               KvType<T>::pack(o[i + 1].x * inv, o[i + 1].y * inv), KvType<T>::pack(o[i + 1].z * inv, o[i + 1].w * inv));
+                            store(o, d);
                         }
                     }
                     __syncwarp();
                 }
+                if (done < count) tell_queries();
             }
-            done += n;
-            seg_begin += at.seg.blocks;
-            if (done < count) at.next_segment(work);
         }
     } else if (warp < kSoftmaxWarps + kLoadWarps) {
-        // ================= copies =================
-        const int tid = threadIdx.x - 32 * kSoftmaxWarps;
-        constexpr int kRowStep = kLoadThreads / kChunks, kPer = kManyKeys / kRowStep;
-        const int chunk = tid % kChunks, row0 = tid / kChunks;
-        const uint32_t q_base = smem_addr(queries), tile_base = smem_addr(tiles);
+        // ================= copies: every warp a tile of its own (even blocks' keys, their values, odd blocks' keys, their values) =================
+        const int w = warp - kSoftmaxWarps, lane = threadIdx.x & 31;
+        constexpr int kRowStep = 32 / kChunks, kPer = kManyKeys / kRowStep;
+        const int chunk = lane % kChunks, row0 = lane / kChunks;
+        const uint32_t tile_base = smem_addr(tiles);
+        const char* const pool = static_cast<const char*>(w & 1 ? p.v : p.k) + chunk * 16;
         Cursor at = s_cursor;
-        int issued = 0, told = 0;                                 // tiles asked for; tiles whose arrival was announced
-        auto announce = [&](int upto) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            for (; told < upto; ++told) mbar_arrive(&kv_full[told % S::kSlots]);
+        int left = count;                                         // blocks from the cursor on
+        auto step = [&]() {
+            if (--left > 0 && ++at.block == at.seg.blocks) at.next_segment(work);
         };
-        uint32_t segments = 0;
-        int done = 0;
-        while (done < count) {
-            const int rows = work.rows_of(at.seq), tile0 = at.tile * kManyRows;
-            const int n = min(count - done, at.seg.blocks - at.block);
-            if (segments > 0) {
-                copy_wait<0>();
-                announce(issued);                                 // the products that free the queries wait for these
-                qmm_wait(&q_free, (segments - 1) & 1u, &s_failed);
-                __syncwarp();
-            }
-            ++segments;
-            // queries of both tiles; rows past the last are zeros
-#pragma unroll 4
-            for (int r = row0; r < kManyRows; r += kRowStep) {
-                const int row = tile0 + r, token = row / work.group;
-                const bool live = row < rows;
-                const T* src = static_cast<const T*>(a.q) + (live ? (at.seq.first_row + token) * a.q_stride +
-                                                                       static_cast<int64_t>(at.head * work.group + row - token * work.group) * D + chunk * 8
-                                                                  : 0);
-                copy16_fill(q_base + (r >> 7) * (S::kQueryBytes / 2) + many_at(kManyTile, r & 127, chunk), src, live);
-            }
-#pragma unroll 1
-            for (int j = 0; j < n; ++j) {
-                const int first = at.seg.low + (at.block + j) * kManyKeys;
-                int64_t place[kPer];
+        if (w >= 2) step();
+        for (int tile = w; left > 0; tile += kLoadWarps) {
+            const int slot = tile % S::kSlots, first = at.seg.low + at.block * kManyKeys;
+            // tensor copies: lane i looks up the i-th part of the block
+            const bool inside = box_rows > 0 && first >= at.seg.key0 && first + kManyKeys <= at.seg.key1;
+            const int parts = inside ? kManyKeys / box_rows : 0;
+            int64_t from = 0;
+            if (lane < parts) from = kv_place(p, at.b, first + lane * box_rows);
+            const bool whole = inside && __all_sync(0xffffffffu, from >= 0);
+            int64_t place[kManyKeys / 32];                        // else of keys first + lane, + 32 ...
+            if (!whole) {
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                    const int key = first + row0 + i * kRowStep;
+                for (int i = 0; i < kManyKeys / 32; ++i) {
+                    const int key = first + lane + 32 * i;
                     place[i] = key >= at.seg.key0 && key < at.seg.key1 ? kv_place(p, at.b, key) : -1;
                     if (place[i] >= 0) place[i] += static_cast<int64_t>(at.head) * p.page_size;
                 }
-#pragma unroll
-                for (int kind = 0; kind < 2; ++kind) {            // keys, values
-                    const int slot = issued % S::kSlots;
-                    if (issued >= S::kSlots) {
-                        qmm_wait(&kv_free[slot], (issued / S::kSlots - 1) & 1u, &s_failed);
-                        __syncwarp();
-                    }
-                    const char* pool = static_cast<const char*>(kind ? p.v : p.k) + chunk * 16;
-                    const uint32_t dst = tile_base + slot * S::kTileBytes;
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i)
-                        copy16_fill(dst + many_at(kManyKeys, row0 + i * kRowStep, chunk), pool + (place[i] < 0 ? 0 : place[i] * (D * 2)), place[i] >= 0);
-                    copy_commit();
-                    ++issued;
-                    copy_wait<2>();
-                    announce(issued - 2);
-                }
             }
-            done += n;
-            if (done < count) at.next_segment(work);
+            if (tile >= S::kSlots) {
+                qmm_wait(&kv_free[slot], (tile / S::kSlots - 1) & 1u, &s_failed);
+                __syncwarp();
+            }
+            const uint32_t dst = tile_base + slot * S::kTileBytes;
+            if (whole) {
+                if (lane == 0) mbar_expect_tx(&kv_full[slot], S::kTileBytes);
+                __syncwarp();
+                if (lane < parts) {
+                    const int row = static_cast<int>(from) + at.head * p.page_size;
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h)
+                        tma_rows(dst + h * kManyKeys * 128 + lane * box_rows * 128, w & 1 ? &v_map : &k_map, h * 64, row, &kv_full[slot]);
+                }
+            } else {
+#pragma unroll 4
+                for (int i = 0; i < kPer; ++i) {
+                    const int r = row0 + i * kRowStep, at_key = r / 32;
+                    const int64_t own = at_key == 0 ? place[0] : at_key == 1 ? place[1] : at_key == 2 ? place[2] : place[3];
+                    const int64_t row = __shfl_sync(0xffffffffu, own, r % 32);
+                    copy16_fill(dst + many_at(kManyKeys, r, chunk), pool + (row < 0 ? 0 : row * (D * 2)), row >= 0);
+                }
+                copy_commit();
+                copy_wait<0>();
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&kv_full[slot]);
+            }
+            step();
+            if (left > 0) step();
         }
-        copy_wait<0>();
-        announce(issued);
     } else if (elect_one()) {
         // ================= products =================
         constexpr uint32_t kFormat = std::is_same_v<T, __half> ? 0u : 1u;
@@ -398,7 +469,7 @@ kv_many_kernel(const KvArgs p, const KvAttentionArgs a) {
         const uint64_t v_desc = umma_desc_values(smem_addr(tiles), kManyKeys * 128);
         Cursor at = s_cursor;
         int tile = 0, done = 0;                                   // tiles consumed
-        uint32_t p_par[2] = {0, 0};
+        uint32_t p_par[2] = {0, 0}, q_par[2] = {0, 0};
         auto wait_tile = [&](int i) {
             qmm_wait(&kv_full[i % S::kSlots], (i / S::kSlots) & 1u, &s_failed);
             fence_after();
@@ -427,10 +498,13 @@ kv_many_kernel(const KvArgs p, const KvAttentionArgs a) {
             const int n = min(count - done, at.seg.blocks - at.block);
             const bool two = rows - at.tile * kManyRows > kManyTile;
             wait_tile(tile);
-            score(0, tile % S::kSlots);
-            if (two) score(1, tile % S::kSlots);
+            for (int x = 0; x < (two ? 2 : 1); ++x) {
+                qmm_wait(&q_full[x], q_par[x], &s_failed);
+                q_par[x] ^= 1u;
+                fence_after();
+                score(x, tile % S::kSlots);
+            }
             umma_commit(&kv_free[tile % S::kSlots]);
-            if (n == 1) umma_commit(&q_free);
             for (int j = 0; j < n; ++j) {
                 const int vt = tile + 1, kt = tile + 2;
                 const bool more = j + 1 < n;
@@ -450,10 +524,7 @@ kv_many_kernel(const KvArgs p, const KvAttentionArgs a) {
                 } else {
                     umma_commit(&kv_free[vt % S::kSlots]);
                 }
-                if (more) {
-                    umma_commit(&kv_free[kt % S::kSlots]);
-                    if (j + 2 == n) umma_commit(&q_free);
-                }
+                if (more) umma_commit(&kv_free[kt % S::kSlots]);
                 tile += 2;
             }
             done += n;
@@ -473,6 +544,29 @@ kv_many_kernel(const KvArgs p, const KvAttentionArgs a) {
     if (threadIdx.x == 0 && s_failed) atomicExch(a.error, 8u);
 }
 
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+    static EncodeFn fn = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult qres;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) != cudaSuccess || qres != cudaDriverEntryPointSuccess)
+            return static_cast<EncodeFn>(nullptr);
+        return reinterpret_cast<EncodeFn>(ptr);
+    }();
+    return fn;
+}
+// the pool's vectors as rows of a 2-D tensor: boxes of 64 dimensions x box_rows, 128-byte swizzle
+bool encode_pool(CUtensorMap* map, const KvArgs& p, void* pool, int box_rows) {
+    EncodeFn encode = encode_fn();
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.head_dim), static_cast<cuuint64_t>(p.pages) * p.kv_heads * p.page_size};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.head_dim) * 2};
+    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)}, elem[2] = {1, 1};
+    return encode && encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, pool, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int BITS, int D>
 cudaError_t launch_many(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t stream) {
     using S = ManyShape<BITS, D>;
@@ -482,7 +576,13 @@ cudaError_t launch_many(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t 
         if (e != cudaSuccess) return e;
         attribute.mark();
     }
-    return launch_dependent(kv_many_kernel<T, BITS, D>, dim3(static_cast<unsigned>(sm_count())), dim3(kManyThreads), S::kSmem, stream, p, a);
+    // tensor copies of the largest power of two that divides the page size, from eight rows (a swizzle atom) on
+    CUtensorMap k_map{}, v_map{};
+    int box_rows = std::min(kManyKeys, p.page_size & -p.page_size);
+    if (box_rows < 8 || p.pages * p.kv_heads * p.page_size > INT32_MAX || !encode_pool(&k_map, p, p.k, box_rows) || !encode_pool(&v_map, p, p.v, box_rows))
+        box_rows = 0;
+    return launch_dependent(kv_many_kernel<T, BITS, D>, dim3(static_cast<unsigned>(sm_count())), dim3(kManyThreads), S::kSmem, stream, k_map, v_map, p, a,
+                            box_rows);
 }
 
 }  // namespace
