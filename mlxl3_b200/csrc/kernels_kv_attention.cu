@@ -24,6 +24,7 @@ constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps;
 constexpr int kFewKeys = 64;                       // keys of a block
 constexpr int kFewCtasPerSm = 2;
 constexpr int kFewTable = 128;
+constexpr int kFewOver = 1;
 
 template <int BITS, int D, int WM>
 struct FewShape {
@@ -90,10 +91,11 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
     pdl_launch_dependents();
     pdl_wait();
     extern __shared__ __align__(128) unsigned char smem[];
-    using Work = KvWork<S::kRows, kFewKeys>;
+    using Work = KvWork<S::kRows, kFewKeys, kFewOver>;
+    using Cursor = KvCursor<S::kRows, kFewKeys, kFewOver>;
     __shared__ int64_t s_sum[kFewThreads / S::kLanes + 1];
     __shared__ KvTable<kFewTable> s_table;
-    __shared__ KvCursor<S::kRows, kFewKeys> s_cursor;
+    __shared__ Cursor s_cursor;
     __shared__ float2 s_ml[kFewWarps / 2][16];
     __shared__ bool s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -101,8 +103,10 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
     const Work work(p, a, s_table);
     KvRun run;
     if (!kv_find_run<kFewThreads, S::kLanes>(work, s_sum, s_cursor, run)) return;
-    KvCursor<S::kRows, kFewKeys> put = s_cursor, get = s_cursor;  // copies run ahead of the products
-    const int count = static_cast<int>(run.u1 - run.u0);
+    Cursor get = s_cursor;                                        // copies (put) run ahead of the products (get)
+    if (get.block == get.end && !get.next_segment(work)) return;
+    Cursor put = get;
+    bool more = true;                                             // put stands at a block
 
     // ---- copies ------------------------------------------------------------------------------------------------------
     constexpr int kPerThread = kFewKeys * S::kChunks / kFewThreads, kRowStep = kFewThreads / S::kChunks;
@@ -138,20 +142,19 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
         if constexpr (BITS != 16)
             copy4_fill(dst + 2 * S::kTileBytes + tid * 4, (tid < kFewKeys ? p.k_scale : p.v_scale) + (scale_place < 0 ? 0 : scale_place), scale_place >= 0);
     };
-    auto step_put = [&]() {
-        if (++put.block == put.seg.blocks) put.next_segment(work);
-    };
     int asked = 0;
-    look_up();
-#pragma unroll 1
-    for (; asked < S::kStages - 1; ++asked) {
-        if (asked < count) {
+    auto ask = [&]() {
+        if (more) {
             copy_block(asked);
-            step_put();
-            if (asked + 1 < count) look_up();
+            if (++asked == S::kStages) asked = 0;
+            more = put.step(work);
+            if (more) look_up();
         }
         copy_commit();
-    }
+    };
+    look_up();
+#pragma unroll 1
+    for (int i = 0; i < S::kStages - 1; ++i) ask();
 
     // ---- state of a segment ---------------------------------------------------------------------------------------------
     uint32_t q[kSteps][4];
@@ -358,7 +361,7 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
         if (pair) *reinterpret_cast<uint32_t*>(dst) = w;
         else *dst = reinterpret_cast<const T*>(&w)[0];
     };
-    auto finish = [&](int stage, int64_t seg_begin, int64_t seg_end) {
+    auto finish = [&](int stage) {
         float* merge = reinterpret_cast<float*>(smem + (S::kMergeInStage ? stage : S::kStages) * S::kStageBytes);
         if constexpr (S::kMergeInStage && S::kWk > 1) __syncthreads();     // every warp is through with the block
 #pragma unroll
@@ -406,7 +409,8 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
             __syncthreads();
         }
         const int rows = work.rows_of(get.seq), tile0 = get.tile * S::kRows;
-        const int c0 = run.cta_of(seg_begin), c1 = run.cta_of(seg_end - 1);                 // CTAs that hold its first and last block
+        const int64_t first_unit = get.base + kFewOver;
+        const int c0 = run.cta_of(first_unit), c1 = run.cta_of(first_unit + get.seg.blocks - 1);     // CTAs that hold its first and last block
         if (c0 == c1) {
             if (wk == 0) {
 #pragma unroll
@@ -487,28 +491,16 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
     };
 
     // ---- the run ------------------------------------------------------------------------------------------------------
-    int64_t seg_begin = run.u0 - get.block;
     begin();
-#pragma unroll 1
-    for (int it = 0; it < count; ++it) {
+    for (int stage = 0;; stage = stage + 1 == S::kStages ? 0 : stage + 1) {
         copy_wait<S::kStages - 2>();
         __syncthreads();                                          // the block has landed, and the one before was used by all
-        if (asked < count) {
-            copy_block(asked % S::kStages);
-            step_put();
-        }
-        copy_commit();
-        ++asked;
-        if (asked < count) look_up();
-        multiply(it % S::kStages);
-        const bool end = ++get.block == get.seg.blocks;
-        if (end || it + 1 == count) {
-            finish(it % S::kStages, seg_begin, seg_begin + get.seg.blocks);
-            seg_begin += get.seg.blocks;
-            if (it + 1 < count) {
-                get.next_segment(work);
-                begin();
-            }
+        ask();
+        multiply(stage);
+        if (++get.block == get.end) {
+            finish(stage);
+            if (!get.next_segment(work)) break;
+            begin();
         }
     }
 }

@@ -31,6 +31,7 @@ constexpr int kManyKeys = 128, kManyTile = 128, kManyRows = 2 * kManyTile;
 constexpr int kSoftmaxWarps = 8, kLoadWarps = 4;
 constexpr int kManyThreads = 32 * (kSoftmaxWarps + kLoadWarps + 1);
 constexpr int kManyTable = 512;
+constexpr int kManyOver = 3;
 constexpr uint32_t kScoreCols = 128;               // tensor-memory columns of S_x; P_x lies in their second half
 
 template <int BITS, int D>
@@ -102,14 +103,35 @@ struct Pair {
 __device__ __forceinline__ Pair fma2(Pair a, const Pair& b, const Pair& c) { asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(a.v) : "l"(b.v), "l"(c.v)); return a; }
 __device__ __forceinline__ Pair add2(Pair a, const Pair& b) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v)); return a; }
 
+// 2^x of two numbers <= 2^7 on the multiply-add pipe: the nearest whole number goes into the exponent, the rest, |f| <= 1/2, through a
+// polynomial (least squares of the relative error, reweighted to equal ripples: 1.6e-7).  Below 2^-126 the result stays there.
+__device__ __forceinline__ void exp2_by_fma(Pair x, float& y0, float& y1) {
+    float x0, x1;
+    x.get(x0, x1);
+    x = Pair(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
+    const Pair magic(12582912.0f, 12582912.0f), unmagic(-12582912.0f, -12582912.0f), minus(-1.0f, -1.0f);
+    const Pair t = add2(x, magic), f = fma2(add2(t, unmagic), minus, x);
+    Pair y(0.00132764940f, 0.00132764940f);
+    y = fma2(y, f, Pair(0.00967553636f, 0.00967553636f));
+    y = fma2(y, f, Pair(0.0555071309f, 0.0555071309f));
+    y = fma2(y, f, Pair(0.240221202f, 0.240221202f));
+    y = fma2(y, f, Pair(0.693146944f, 0.693146944f));
+    y = fma2(y, f, Pair(1.00000012f, 1.00000012f));
+    float t0, t1;
+    t.get(t0, t1);
+    y.get(y0, y1);
+    y0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
+    y1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
+}
+
 // box_rows: rows of a tensor copy, a power of two that divides the page size, or 0: no tensor copies
 template <typename T, int BITS, int D>
 __global__ void __launch_bounds__(kManyThreads, 1)
 kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const KvArgs p, const KvAttentionArgs a,
                const int box_rows) {
     using S = ManyShape<BITS, D>;
-    using Work = KvWork<kManyRows, kManyKeys>;
-    using Cursor = KvCursor<kManyRows, kManyKeys>;
+    using Work = KvWork<kManyRows, kManyKeys, kManyOver>;
+    using Cursor = KvCursor<kManyRows, kManyKeys, kManyOver>;
     constexpr int kChunks = D / 8;
     pdl_launch_dependents();
     pdl_wait();
@@ -117,7 +139,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     __shared__ KvTable<kManyTable> s_table;
     __shared__ int64_t s_sum[kManyThreads / 32 + 1];
     __shared__ Cursor s_cursor;
-    __shared__ __align__(8) uint64_t kv_full[S::kSlots], kv_free[S::kSlots], s_full[2], p_full[2], o_full[2], q_full[2], drained;
+    __shared__ __align__(8) uint64_t kv_full[S::kSlots], kv_free[S::kSlots], s_full[2], p_half[2], p_full[2], o_full[2], q_full[2], drained;
     __shared__ uint32_t tmem_base_slot;
     __shared__ int s_last[2];
     __shared__ volatile int s_failed;
@@ -126,13 +148,22 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     const Work work(p, a, s_table);
     KvRun run;
     if (!kv_find_run<kManyThreads, 32>(work, s_sum, s_cursor, run)) return;
-    const int count = static_cast<int>(run.u1 - run.u0);
+    if (s_cursor.block == s_cursor.end) {                         // the run begins in a segment that is another CTA's
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            Cursor c = s_cursor;
+            if (!c.next_segment(work)) c.end = c.block;
+            s_cursor = c;
+        }
+        __syncthreads();
+        if (s_cursor.block == s_cursor.end) return;
+    }
     unsigned char* const queries = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     unsigned char* const tiles = queries + S::kQueryBytes;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kSlots; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], 1); }
-        for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 1); mbar_init(&p_full[x], kManyTile); mbar_init(&o_full[x], 1); mbar_init(&q_full[x], kManyTile); }
+        for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 1); mbar_init(&p_half[x], kManyTile); mbar_init(&p_full[x], kManyTile); mbar_init(&o_full[x], 1); mbar_init(&q_full[x], kManyTile); }
         mbar_init(&drained, 1);
         s_failed = 0;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -151,26 +182,30 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         const uint32_t scores = tmem + lanes + x * kScoreCols, probs = scores + kScoreCols / 2, outs = tmem + lanes + S::kOutCols + x * D;
         Cursor at = s_cursor;
         uint32_t s_par = 0, o_par = 0;
-        int done = 0;
-        int64_t seg_begin = run.u0 - at.block;
+        bool more = true;                                         // `at` is a segment of this CTA's
         // the cursor at the next segment that has rows of this tile, from where it is
         auto settle = [&]() {
-            while (done < count && x == 1 && work.rows_of(at.seq) - at.tile * kManyRows <= kManyTile) {
-                done += min(count - done, at.seg.blocks - at.block);
-                seg_begin += at.seg.blocks;
-                if (done < count) at.next_segment(work);
-            }
+            while (more && x == 1 && work.rows_of(at.seq) - at.tile * kManyRows <= kManyTile) more = at.next_segment(work);
         };
-        // this thread's row of queries; rows past the last are zeros
+        // the warp's 32 rows of queries, neighbouring lanes a row; rows past the last are zeros
         auto ask_queries = [&]() {
-            const int row = at.tile * kManyRows + x * kManyTile + r, token = row / work.group;
-            const bool live = row < work.rows_of(at.seq);
-            const T* src = static_cast<const T*>(a.q) + (live ? (at.seq.first_row + token) * a.q_stride +
-                                                                   static_cast<int64_t>(at.head * work.group + row - token * work.group) * D
-                                                              : 0);
+            constexpr int kStep = 32 / kChunks;
+            const int lane = threadIdx.x & 31, chunk = lane % kChunks, rows = work.rows_of(at.seq);
+            int q = (warp & 3) * 32 + lane / kChunks;
+            int row = at.tile * kManyRows + x * kManyTile + q, token = row / work.group, head = row - token * work.group;
             const uint32_t dst = smem_addr(queries) + x * (S::kQueryBytes / 2);
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c) copy16_fill(dst + many_at(kManyTile, r, c), src + (live ? c * 8 : 0), live);
+#pragma unroll 1
+            for (int i = 0; i < 32 / kStep; ++i) {
+                const bool live = row < rows;
+                const T* src = static_cast<const T*>(a.q) + (live ? (at.seq.first_row + token) * a.q_stride +
+                                                                       static_cast<int64_t>(at.head * work.group + head) * D + chunk * 8
+                                                                  : 0);
+                copy16_fill(dst + many_at(kManyTile, q, chunk), src, live);
+                q += kStep;
+                row += kStep;
+                head += kStep;
+                while (head >= work.group) { head -= work.group; ++token; }
+            }
             copy_commit();
         };
         auto tell_queries = [&]() {
@@ -179,26 +214,30 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             mbar_arrive(&q_full[x]);
         };
         settle();
-        if (done < count) {
+        if (more) {
             ask_queries();
             tell_queries();
         }
-        while (done < count) {
+        while (more) {
             {
-                const int row = at.tile * kManyRows + x * kManyTile + r, n = min(count - done, at.seg.blocks - at.block);
-                const int token = row / work.group;
-                const bool live = row < work.rows_of(at.seq);
-                const int position = live ? at.seq.first_pos + token : -1;
+                const Cursor here = at;
+                const int row = here.tile * kManyRows + x * kManyTile + r, n = here.end - here.block;
+                const int position = row < work.rows_of(here.seq) ? here.seq.first_pos + row / work.group : -1;
                 const int end = min(position + 1, work.capacity), start = a.window > 0 ? position + 1 - a.window : 0;
                 float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
                 for (int j = 0; j < n; ++j) {
-                    const int first = at.seg.low + (at.block + j) * kManyKeys;
+                    const int first = here.seg.low + (here.block + j) * kManyKeys;
                     const int e = end - first, b = start - first;              // visible: columns b .. e - 1
                     qmm_wait(&s_full[x], s_par, &s_failed);
                     s_par ^= 1u;
                     __syncwarp();
                     fence_after();
+                    if (j + 1 == n) {                             // the products that read the queries are done: the next segment's may come
+                        more = at.next_segment(work);
+                        settle();
+                        if (more) ask_queries();
+                    }
                     // columns of a pair of loads that the row does not see
                     const bool masked = __any_sync(0xffffffffu, e < kManyKeys || b > 0);
                     uint32_t v0[32], v1[32];
@@ -208,10 +247,15 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                         tmem_ld32(scores + col + 32, v1);
                         tmem_wait_ld();
                         if (masked) {
+                            auto seen = [&](int from) {           // bit i: column from + i is visible
+                                const int hi = min(max(e - from, 0), 32), lo = min(max(b - from, 0), 32);
+                                return (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & (lo == 32 ? 0u : 0xffffffffu << lo);
+                            };
+                            const uint32_t m0 = seen(col), m1 = seen(col + 32);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
-                                v0[i] = col + i < e && col + i >= b ? v0[i] : 0xff800000u;
-                                v1[i] = col + 32 + i < e && col + 32 + i >= b ? v1[i] : 0xff800000u;
+                                v0[i] = m0 & (1u << i) ? v0[i] : 0xff800000u;
+                                v1[i] = m1 & (1u << i) ? v1[i] : 0xff800000u;
                             }
                         }
                     };
@@ -256,48 +300,51 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                     // the upper columns are in registers; their probabilities go where those scores lay, then the lower ones'
                     const Pair scale2(a.scale_log2e, a.scale_log2e), shift2(m == -INFINITY ? 0.0f : -m, m == -INFINITY ? 0.0f : -m);
                     Pair l2(0.0f, 0.0f);
-                    auto put = [&](const uint32_t (&v)[32], int col) {
+                    // every fourth pair of exponentials runs on the multiply-add pipe, which the other pipe would wait for
+                    auto put = [&](auto mixed, const uint32_t (&v)[32], int col) {
                         uint32_t w[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             float x0, x1;
-                            fma2(Pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, shift2).get(x0, x1);
-                            x0 = exp2_fast(x0);
-                            x1 = exp2_fast(x1);
+                            const Pair x = fma2(Pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, shift2);
+                            if (decltype(mixed)::value && i % 4 == 3) {
+                                exp2_by_fma(x, x0, x1);
+                            } else {
+                                x.get(x0, x1);
+                                x0 = exp2_fast(x0);
+                                x1 = exp2_fast(x1);
+                            }
                             l2 = add2(l2, Pair(x0, x1));
                             w[i] = KvType<T>::pack(x0, x1);
                         }
                         __syncwarp();
                         tmem_st16(probs + col / 2, w);
                     };
+                    auto put_all = [&](auto mixed) {
 #pragma unroll 1
-                    for (int col = kManyKeys - 64;; col -= 64) {
-                        put(v1, col + 32);
-                        put(v0, col);
-                        if (col == 0) break;
-                        load(col - 64);
-                    }
+                        for (int col = kManyKeys - 64;; col -= 64) {
+                            put(mixed, v1, col + 32);
+                            put(mixed, v0, col);
+                            tmem_wait_st();
+                            fence_before();
+                            mbar_arrive(col == 0 ? &p_full[x] : &p_half[x]);
+                            if (col == 0) break;
+                            load(col - 64);
+                        }
+                    };
+                    if (masked) put_all(std::false_type{}); else put_all(std::true_type{});
                     float l0, l1;
                     l2.get(l0, l1);
                     l += l0 + l1;
-                    tmem_wait_st();
-                    fence_before();
-                    mbar_arrive(&p_full[x]);
                 }
-                // the products that read the queries are done: those of the next segment may come
-                const Cursor here = at;
-                const int64_t here_begin = seg_begin;
-                done += n;
-                seg_begin += at.seg.blocks;
-                if (done < count) at.next_segment(work);
-                settle();
-                if (done < count) ask_queries();
+                if (more) tell_queries();
                 // ---- the segment's rows, or this CTA's part of them
                 qmm_wait(&o_full[x], o_par, &s_failed);
                 o_par ^= 1u;
                 __syncwarp();
                 fence_after();
-                const int c0 = run.cta_of(here_begin), c1 = run.cta_of(here_begin + here.seg.blocks - 1);
+                const int64_t first_unit = here.base + kManyOver;
+                const int c0 = run.cta_of(first_unit), c1 = run.cta_of(first_unit + here.seg.blocks - 1);
                 auto part_of = [&](int c) { return a.parts + (2 * c + (c == c0 ? 1 : 0)) * static_cast<int64_t>(S::kPartFloats); };
                 const int pr = x * kManyTile + r;
                 const bool whole = c0 == c1;
@@ -395,69 +442,66 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                     }
                     __syncwarp();
                 }
-                if (done < count) tell_queries();
             }
         }
     } else if (warp < kSoftmaxWarps + kLoadWarps) {
         // ================= copies: every warp a tile of its own (even blocks' keys, their values, odd blocks' keys, their values) =================
         const int w = warp - kSoftmaxWarps, lane = threadIdx.x & 31;
-        constexpr int kRowStep = 32 / kChunks, kPer = kManyKeys / kRowStep;
+        constexpr int kRowStep = 32 / kChunks;
         const int chunk = lane % kChunks, row0 = lane / kChunks;
+        const int parts = box_rows > 0 ? kManyKeys / box_rows : 0;
         const uint32_t tile_base = smem_addr(tiles);
         const char* const pool = static_cast<const char*>(w & 1 ? p.v : p.k) + chunk * 16;
         Cursor at = s_cursor;
-        int left = count;                                         // blocks from the cursor on
-        auto step = [&]() {
-            if (--left > 0 && ++at.block == at.seg.blocks) at.next_segment(work);
-        };
-        if (w >= 2) step();
-        for (int tile = w; left > 0; tile += kLoadWarps) {
+        bool more = w < 2 || at.step(work);
+        for (int tile = w; more; tile += kLoadWarps) {
             const int slot = tile % S::kSlots, first = at.seg.low + at.block * kManyKeys;
-            // tensor copies: lane i looks up the i-th part of the block
-            const bool inside = box_rows > 0 && first >= at.seg.key0 && first + kManyKeys <= at.seg.key1;
-            const int parts = inside ? kManyKeys / box_rows : 0;
-            int64_t from = 0;
-            if (lane < parts) from = kv_place(p, at.b, first + lane * box_rows);
-            const bool whole = inside && __all_sync(0xffffffffu, from >= 0);
-            int64_t place[kManyKeys / 32];                        // else of keys first + lane, + 32 ...
-            if (!whole) {
-#pragma unroll
-                for (int i = 0; i < kManyKeys / 32; ++i) {
-                    const int key = first + lane + 32 * i;
-                    place[i] = key >= at.seg.key0 && key < at.seg.key1 ? kv_place(p, at.b, key) : -1;
-                    if (place[i] >= 0) place[i] += static_cast<int64_t>(at.head) * p.page_size;
-                }
+            // Lane i looks up the i-th part of the block: a tensor copy where every key of it is a token that some row of the sequence
+            // sees (and so holds numbers), row by row with zeros where not.
+            const int low = a.window > 0 ? max(0, at.seq.first_pos + 1 - a.window) : 0;
+            const int high = min(at.seq.first_pos + min(at.seq.n, a.max_new), work.capacity);
+            int64_t from = -1;
+            if (lane < parts) {
+                const int key = first + lane * box_rows;
+                if (key >= low && key + box_rows <= high) from = kv_place(p, at.b, key);
             }
+            const uint32_t whole = __ballot_sync(0xffffffffu, from >= 0);
             if (tile >= S::kSlots) {
                 qmm_wait(&kv_free[slot], (tile / S::kSlots - 1) & 1u, &s_failed);
                 __syncwarp();
             }
             const uint32_t dst = tile_base + slot * S::kTileBytes;
-            if (whole) {
-                if (lane == 0) mbar_expect_tx(&kv_full[slot], S::kTileBytes);
-                __syncwarp();
-                if (lane < parts) {
-                    const int row = static_cast<int>(from) + at.head * p.page_size;
+            if (from >= 0) {
+                const int row = static_cast<int>(from) + at.head * p.page_size;
 #pragma unroll
-                    for (int h = 0; h < D / 64; ++h)
-                        tma_rows(dst + h * kManyKeys * 128 + lane * box_rows * 128, w & 1 ? &v_map : &k_map, h * 64, row, &kv_full[slot]);
-                }
-            } else {
-#pragma unroll 4
-                for (int i = 0; i < kPer; ++i) {
-                    const int r = row0 + i * kRowStep, at_key = r / 32;
-                    const int64_t own = at_key == 0 ? place[0] : at_key == 1 ? place[1] : at_key == 2 ? place[2] : place[3];
-                    const int64_t row = __shfl_sync(0xffffffffu, own, r % 32);
-                    copy16_fill(dst + many_at(kManyKeys, r, chunk), pool + (row < 0 ? 0 : row * (D * 2)), row >= 0);
+                for (int h = 0; h < D / 64; ++h)
+                    tma_rows(dst + h * kManyKeys * 128 + lane * box_rows * 128, w & 1 ? &v_map : &k_map, h * 64, row, &kv_full[slot]);
+            }
+            __syncwarp();
+            if (__popc(whole) < parts || parts == 0) {
+#pragma unroll 1
+                for (int k0 = 0; k0 < kManyKeys; k0 += 32) {      // 32 keys: lane i finds key k0 + i
+                    const int key = first + k0 + lane;
+                    int64_t place = -1;
+                    if (key >= at.seg.key0 && key < at.seg.key1) place = kv_place(p, at.b, key);
+                    if (place >= 0) place += static_cast<int64_t>(at.head) * p.page_size;
+#pragma unroll
+                    for (int i = 0; i < 32 / kRowStep; ++i) {
+                        const int r = row0 + i * kRowStep;
+                        const int64_t row = __shfl_sync(0xffffffffu, place, r);
+                        if (parts == 0 || !(whole >> ((k0 + r) / box_rows) & 1u))
+                            copy16_fill(dst + many_at(kManyKeys, k0 + r, chunk), pool + (row < 0 ? 0 : row * (D * 2)), row >= 0);
+                    }
                 }
                 copy_commit();
                 copy_wait<0>();
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&kv_full[slot]);
             }
-            step();
-            if (left > 0) step();
+            // the copies' bytes may arrive before they are announced: the phase ends with this arrival at the earliest
+            if (lane == 0) mbar_expect_tx(&kv_full[slot], static_cast<uint32_t>(__popc(whole) * box_rows * D * 2));
+            __syncwarp();
+            more = at.step(work) && at.step(work);
         }
     } else if (elect_one()) {
         // ================= products =================
@@ -468,7 +512,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         const uint64_t q_desc = umma_desc(smem_addr(queries)), k_desc = umma_desc(smem_addr(tiles));
         const uint64_t v_desc = umma_desc_values(smem_addr(tiles), kManyKeys * 128);
         Cursor at = s_cursor;
-        int tile = 0, done = 0;                                   // tiles consumed
+        int tile = 0;                                             // tiles consumed
         uint32_t p_par[2] = {0, 0}, q_par[2] = {0, 0};
         auto wait_tile = [&](int i) {
             qmm_wait(&kv_full[i % S::kSlots], (i / S::kSlots) & 1u, &s_failed);
@@ -484,18 +528,21 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             umma_commit(&s_full[x]);
         };
         auto weigh = [&](int x, int slot, bool accumulate) {
-            qmm_wait(&p_full[x], p_par[x], &s_failed);
-            p_par[x] ^= 1u;
-            fence_after();
+            // the probabilities of the upper keys come first
             const uint64_t vd = v_desc + slot * (S::kTileBytes >> 4);
 #pragma unroll
-            for (int k = 0; k < kManyKeys / 16; ++k)
-                umma_f16_ts(tmem + S::kOutCols + x * D, tmem + x * kScoreCols + kScoreCols / 2 + k * 8, vd + k * (16 * 128 >> 4), kValueDesc,
-                            accumulate || k > 0);
+            for (int h = 1; h >= 0; --h) {
+                qmm_wait(h ? &p_half[x] : &p_full[x], p_par[x], &s_failed);
+                fence_after();
+#pragma unroll
+                for (int k = h * (kManyKeys / 32); k < (h + 1) * (kManyKeys / 32); ++k)
+                    umma_f16_ts(tmem + S::kOutCols + x * D, tmem + x * kScoreCols + kScoreCols / 2 + k * 8, vd + k * (16 * 128 >> 4), kValueDesc,
+                                accumulate || h == 0 || k > kManyKeys / 32);
+            }
+            p_par[x] ^= 1u;
         };
-        while (done < count) {
-            const int rows = work.rows_of(at.seq);
-            const int n = min(count - done, at.seg.blocks - at.block);
+        do {
+            const int rows = work.rows_of(at.seq), n = at.end - at.block;
             const bool two = rows - at.tile * kManyRows > kManyTile;
             wait_tile(tile);
             for (int x = 0; x < (two ? 2 : 1); ++x) {
@@ -527,9 +574,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 if (more) umma_commit(&kv_free[kt % S::kSlots]);
                 tile += 2;
             }
-            done += n;
-            if (done < count) at.next_segment(work);
-        }
+        } while (at.next_segment(work));
         umma_commit(&drained);
         qmm_wait(&drained, 0, &s_failed);
     }

@@ -1,7 +1,8 @@
 // How the attention kernels over the paged cache share out their work.  A segment is up to ROWS rows (token-major, then head) of one
 // sequence and key head -- the query heads that share a key head are rows of one product -- and its keys come in blocks of KEYS.  The
 // blocks of all segments, one after the other, are dealt out to the CTAs of one wave in equal runs: ragged lengths, few sequences
-// and few heads all keep every SM busy, and since the lengths are read on the device a recorded call serves growing sequences.
+// and few heads all keep every SM busy, and since the lengths are read on the device a recorded call serves growing sequences.  A
+// segment counts OVER units before its first block, for what its beginning and its end cost.
 // A CTA that holds a whole segment stores it; CTAs that share one leave (maximum, sum, unnormalised rows) and the last to arrive joins
 // the parts in the order of the keys.
 #pragma once
@@ -22,8 +23,9 @@ struct KvTable {
     int start[CAP + 1], length[CAP];
 };
 
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, int OVER>
 struct KvWork {
+    static constexpr int kOver = OVER;
     const KvArgs& p;
     const KvAttentionArgs& a;
     const int* start;      // [batch + 1], [batch]
@@ -70,62 +72,78 @@ struct KvWork {
         g.blocks = max(1, (g.key1 - g.low + KEYS - 1) / KEYS);
         return g;
     }
-    // blocks of all row tiles of a sequence, for one key head; LANES neighbouring lanes count together
+    // units of all row tiles of a sequence, for one key head; LANES neighbouring lanes count together
     template <int LANES>
-    __device__ __forceinline__ int64_t blocks_of(const KvSeq& s) const {
+    __device__ __forceinline__ int64_t units_of(const KvSeq& s) const {
         int64_t sum = 0;
         const int tiles = tiles_of(s);
-        for (int t = LANES > 1 ? static_cast<int>(threadIdx.x) % LANES : 0; t < tiles; t += LANES) sum += segment(s, t).blocks;
+        for (int t = LANES > 1 ? static_cast<int>(threadIdx.x) % LANES : 0; t < tiles; t += LANES) sum += OVER + segment(s, t).blocks;
 #pragma unroll
         for (int d = LANES / 2; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         return sum;
     }
 };
 
-// A place in the list of blocks: [sequence][key head][row tile][block].
-template <int ROWS, int KEYS>
+// Walks the blocks of a run: [sequence][key head][row tile][block].  The blocks of the segment at hand are block .. end - 1.
+template <int ROWS, int KEYS, int OVER>
 struct KvCursor {
-    int b, head, tile, block;
+    using Work = KvWork<ROWS, KEYS, OVER>;
+    int b, head, tile, block, end;
+    int64_t base, left;    // unit at which the segment begins; units of the run behind this segment
     KvSeq seq;
     KvSegment seg;
 
-    // the next segment, of the next sequence that has rows
-    __device__ __forceinline__ void next_segment(const KvWork<ROWS, KEYS>& w) {
-        block = 0;
-        if (++tile == w.tiles_of(seq)) {
-            tile = 0;
-            if (++head == w.p.kv_heads) {
-                head = 0;
-                do {
-                    if (++b >= w.p.batch) return;
-                    seq = w.seq(b);
-                } while (w.rows_of(seq) == 0);
-            }
-        }
-        seg = w.segment(seq, tile);
+    // the segment at hand, entered at its unit `at`
+    __device__ __forceinline__ void enter(int64_t at) {
+        const int64_t units = min(seg.blocks + OVER - at, left);
+        left -= units;
+        block = static_cast<int>(max(at - OVER, static_cast<int64_t>(0)));
+        end = static_cast<int>(max(at + units - OVER, static_cast<int64_t>(0)));
     }
+    // the next segment of the run that has blocks in it; false: the run is at its end
+    __device__ __forceinline__ bool next_segment(const Work& w) {
+        while (left > 0) {
+            base += seg.blocks + OVER;
+            if (++tile == w.tiles_of(seq)) {
+                tile = 0;
+                if (++head == w.p.kv_heads) {
+                    head = 0;
+                    do {
+                        if (++b >= w.p.batch) return false;
+                        seq = w.seq(b);
+                    } while (w.rows_of(seq) == 0);
+                }
+            }
+            seg = w.segment(seq, tile);
+            enter(0);
+            if (block < end) return true;
+        }
+        return false;
+    }
+    __device__ __forceinline__ bool step(const Work& w) { return ++block < end || next_segment(w); }
 };
 
-// A CTA's run of blocks u0 .. u1 - 1 of `total`, dealt out to `ctas` CTAs.
+// A CTA's run of units u0 .. u1 - 1 of `total`, dealt out to `ctas` CTAs.
 struct KvRun {
     int64_t total, u0, u1;
     int ctas;
 
-    // the CTA that holds block u
+    // the CTA that holds unit u
     __device__ __forceinline__ int cta_of(int64_t u) const { return static_cast<int>(((u + 1) * ctas - 1) / total); }
 };
 
 // Finds this CTA's run; every thread of the block calls it.  Workers of LANES threads (1, or 32: sequences of many row tiles) count a
-// slice of the sequences each; the one whose slice holds the first block writes the place.  Returns false where there is nothing to do.
-template <int THREADS, int LANES, int ROWS, int KEYS>
-__device__ __forceinline__ bool kv_find_run(const KvWork<ROWS, KEYS>& w, int64_t (&s_sum)[THREADS / LANES + 1], KvCursor<ROWS, KEYS>& s_cursor, KvRun& run) {
+// slice of the sequences each; the one whose slice holds the first unit writes the place.  Returns false where there is nothing to do.
+template <int THREADS, int LANES, int ROWS, int KEYS, int OVER>
+__device__ __forceinline__ bool kv_find_run(const KvWork<ROWS, KEYS, OVER>& w, int64_t (&s_sum)[THREADS / LANES + 1],
+                                            KvCursor<ROWS, KEYS, OVER>& s_cursor, KvRun& run) {
     constexpr int kWorkers = THREADS / LANES;
     static_assert(LANES == 1 || LANES == 32, "threads or warps");
     const int worker = threadIdx.x / LANES, sub = threadIdx.x % LANES;
     const int slice = (w.p.batch + kWorkers - 1) / kWorkers;
     const int b0 = min(w.p.batch, worker * slice), b1 = min(w.p.batch, b0 + slice);
     int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += w.template blocks_of<LANES>(w.seq(b)) * w.p.kv_heads;
+    for (int b = b0; b < b1; ++b) mine += w.template units_of<LANES>(w.seq(b)) * w.p.kv_heads;
     if (sub == 0) s_sum[worker] = mine;
     __syncthreads();
     if (threadIdx.x < 32) {                                       // exclusive sums
@@ -153,10 +171,10 @@ __device__ __forceinline__ bool kv_find_run(const KvWork<ROWS, KEYS>& w, int64_t
     const int64_t before = s_sum[worker];
     if (before <= run.u0 && run.u0 < before + mine) {
         int64_t left = run.u0 - before;
-        KvCursor<ROWS, KEYS> c;
+        KvCursor<ROWS, KEYS, OVER> c;
         for (int b = b0; b < b1; ++b) {
             c.seq = w.seq(b);
-            const int64_t per_head = w.template blocks_of<LANES>(c.seq);
+            const int64_t per_head = w.template units_of<LANES>(c.seq);
             if (left >= per_head * w.p.kv_heads) {
                 left -= per_head * w.p.kv_heads;
                 continue;
@@ -166,7 +184,7 @@ __device__ __forceinline__ bool kv_find_run(const KvWork<ROWS, KEYS>& w, int64_t
             left -= c.head * per_head;
             for (c.tile = 0;; c.tile += LANES) {
                 const int tile = c.tile + sub, tiles = w.tiles_of(c.seq);
-                const int n = tile < tiles ? w.segment(c.seq, tile).blocks : 0;
+                const int n = tile < tiles ? OVER + w.segment(c.seq, tile).blocks : 0;
                 if constexpr (LANES == 1) {
                     if (left < n) break;
                     left -= n;
@@ -188,13 +206,15 @@ __device__ __forceinline__ bool kv_find_run(const KvWork<ROWS, KEYS>& w, int64_t
                 }
             }
             c.seg = w.segment(c.seq, c.tile);
-            c.block = static_cast<int>(left);
+            c.base = run.u0 - left;
+            c.left = run.u1 - run.u0;
+            c.enter(left);
             break;
         }
         if (sub == 0) s_cursor = c;
     }
     __syncthreads();
-    return true;
+    return s_cursor.block < s_cursor.end || s_cursor.left > 0;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {             // 2 ulp; exp2(-inf) = 0
