@@ -14,7 +14,9 @@
 //
 // Both kernels are bound by memory (and short calls by the chain row_start -> length -> page table -> data): 16 or 8 lanes hold a
 // vector, 8 dimensions each, so that every access is 16 bytes (8 or 4 for codes) and a vector one coalesced piece.
-#include "kv.cuh"
+#include <algorithm>
+
+#include "kv_work.cuh"
 
 namespace b200exl3 {
 
@@ -317,6 +319,31 @@ cudaError_t launch_read_out(const KvArgs& p, int out_dtype, void* k, void* v, cu
 }
 
 }  // namespace
+
+bool kv_tensor_maps(const KvArgs& p, int most, CUtensorMap* k_map, CUtensorMap* v_map, int* box_rows) {
+    using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const EncodeFn encode = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+            ptr = nullptr;
+        return reinterpret_cast<EncodeFn>(ptr);
+    }();
+    const int64_t vectors = p.pages * p.kv_heads * p.page_size;
+    const int rows = std::min(most, p.page_size & -p.page_size);
+    if (!encode || rows < 8 || vectors > INT32_MAX) return false;       // eight rows are an atom of the swizzle
+    const cuuint32_t width = static_cast<cuuint32_t>(p.head_dim * p.bits / 8), box_width = std::min(width, 128u);
+    const cuuint64_t dims[2] = {width, static_cast<cuuint64_t>(vectors)}, strides[1] = {width};
+    const cuuint32_t box[2] = {box_width, static_cast<cuuint32_t>(rows)}, elem[2] = {1, 1};
+    const CUtensorMapSwizzle swizzle = box_width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : box_width == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+    for (int kind = 0; kind < 2; ++kind)
+        if (encode(kind ? v_map : k_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, kind ? p.v : p.k, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return false;
+    *box_rows = rows;
+    return true;
+}
 
 cudaError_t launch_kv_append(const KvArgs& p, const KvAppendArgs& a, cudaStream_t stream) {
 #define B200_KV_CASE(T, BITS, D) \

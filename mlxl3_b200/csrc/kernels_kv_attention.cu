@@ -1,12 +1,14 @@
 // Attention of new tokens over a paged key/value cache: o_i = sum_j softmax_j(scale q_i . k_j) v_j over the tokens j up to its own
 // (with a window w: the last w of them).
 //
-// Work is shared out as kv_work.cuh says, in segments of 16 * WM rows and blocks of 64 keys.
+// Work is shared out as kv_work.cuh says, in segments of 16 * WM rows and blocks of 64 keys (128 of codes).
 //
-// A block: 128 threads copy the keys and values (cp.async, 16 bytes each, several blocks in flight; what lies outside the
-// visible range is filled with zeros, so nothing behind a length is ever multiplied), WK = 4 / WM warps take 64 / WK keys each
-// against 16 rows: scores by mma.sync, online softmax in fp32 registers, probabilities rounded to 16 bits for the second product.
-// Loads bound it: what a step of single tokens moves is the cache, once.
+// A block: the warps take turns to ask for its keys and values (tensor copies of whole pages or parts of pages, several blocks in flight; row by
+// row with zeros at the ends of the visible range and where pages are too small, so that nothing behind a length is ever
+// multiplied); WK = 4 / WM warps take a share of the keys each against 16 rows: scores by mma.sync, online softmax in fp32 registers,
+// probabilities rounded to 16 bits for the second product.  Loads bound it: what a step of single tokens moves is the cache, once.
+// A row's maximum moves only when a score exceeds it by 2^8, so that the outputs are seldom rescaled; until then probabilities
+// reach 256, which 16 bits hold as well as 1.
 //
 // Codes are multiplied as they are: 8- and 4-bit codes are exact in fp16, and so is what the tensor cores add up in fp32; the key's
 // scale multiplies its scores, the value's its probability.  Those probabilities are taken relative to the largest value scale met so
@@ -21,29 +23,35 @@ namespace b200exl3 {
 namespace {
 
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps;
-constexpr int kFewKeys = 64;                       // keys of a block
 constexpr int kFewCtasPerSm = 2;
 constexpr int kFewTable = 128;
 constexpr int kFewOver = 1;
 
 template <int BITS, int D, int WM>
 struct FewShape {
+    static constexpr int kKeys = BITS == 16 ? 64 : 128;            // of a block
     static constexpr int kWk = kFewWarps / WM;     // warps that share the rows and take different keys
-    static constexpr int kWarpKeys = kFewKeys / kWk;
+    static constexpr int kWarpKeys = kKeys / kWk;
+    static constexpr int kStepKeys = 16;                            // of a warp's step
     static constexpr int kRows = 16 * WM;
     static constexpr int kLanes = WM == 1 ? 1 : 32;    // a sequence has one row tile, or many
     static constexpr int kRowBytes = D * BITS / 8, kChunks = kRowBytes / 16;
-    static constexpr int kTileBytes = kFewKeys * kRowBytes;
-    static constexpr int kStageBytes = 2 * kTileBytes + (BITS == 16 ? 0 : 2 * kFewKeys * 4);
-    static constexpr int kMergeStride = D + 4;
-    static constexpr int kMergeBytes = kWk > 1 ? (kFewWarps / 2) * 16 * kMergeStride * 4 : 0;
-    static constexpr bool kMergeInStage = kMergeBytes <= kStageBytes;      // the warps join in the block's own place where they fit
+    static constexpr int kTileBytes = kKeys * kRowBytes;
+    static constexpr int kScaleBytes = BITS == 16 ? 0 : 2 * kKeys * 4;
+    static constexpr int kStageBytes = (2 * kTileBytes + kScaleBytes + 1023) / 1024 * 1024;
+    static constexpr int kMergeBytes = kFewWarps * 16 * D * 4;     // outputs of the warps, joined in the block's own place where they fit
+    static constexpr bool kMergeInStage = kMergeBytes <= kStageBytes;
     static constexpr int kOwnMergeBytes = kMergeInStage ? 0 : kMergeBytes;
-    static constexpr int kStages = std::min(6, (111 * 1024 - kOwnMergeBytes) / kStageBytes);      // two CTAs per SM
-    static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + kOwnMergeBytes;
+    static constexpr int kStages = std::min(6, (109 * 1024 - kOwnMergeBytes) / kStageBytes);      // two CTAs per SM
+    static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStageBytes + kOwnMergeBytes;
     static constexpr int kPartFloats = kRows * (D + 2);
+    static_assert(kStages >= 3, "copies in flight");
 };
 
+// announces that this thread's copies so far have landed
+__device__ __forceinline__ void copy_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -60,12 +68,13 @@ __device__ __forceinline__ void mma_rows(float (&d)[4], const uint32_t (&a)[4], 
     }
 }
 
-// Where a 16-byte chunk of a tile's row lies: rows of 128 bytes and more swap their chunks by the row's number, shorter ones by the
-// number of the 128 bytes they are in, so that eight rows' same chunk uses all banks.
-template <int CHUNKS>
+// Where a 16-byte chunk of a tile's row lies, as the tensor copies put it: pieces of up to 128 bytes of all rows, one after the other; in
+// a piece rows of 128 bytes swap their chunks by the row's number, shorter ones by the number of the 128 bytes they are in, so that eight
+// rows' same chunk uses all banks.
+template <int CHUNKS, int KEYS>
 __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
-    constexpr int kShift = CHUNKS >= 8 ? 0 : (CHUNKS == 4 ? 1 : 2), kMask = CHUNKS >= 8 ? 7 : CHUNKS - 1;
-    return static_cast<uint32_t>(row * CHUNKS + (chunk ^ ((row >> kShift) & kMask))) * 16;
+    constexpr int kPiece = CHUNKS >= 8 ? 8 : CHUNKS, kShift = CHUNKS >= 8 ? 0 : (CHUNKS == 4 ? 1 : 2);
+    return static_cast<uint32_t>((chunk / kPiece * KEYS + row) * kPiece + ((chunk % kPiece) ^ ((row >> kShift) & (kPiece - 1)))) * 16;
 }
 
 // Two codes as fp16.  8 bits: bytes i and j of a word whose sign bits were flipped become 1024 + (code + 128); 4 bits: the low nibbles
@@ -81,84 +90,114 @@ template <int I> __device__ __forceinline__ uint32_t codes4(uint32_t w) {
     return less(d, 0x64086408u);
 }
 
+// box_rows: rows of a tensor copy, a power of two that divides the page size, or 0: no tensor copies
 template <typename T, int BITS, int D, int WM>
 __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
-kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
+kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const KvArgs p, const KvAttentionArgs a,
+              const int box_rows) {
     using S = FewShape<BITS, D, WM>;
     using M = std::conditional_t<BITS == 16, T, __half>;          // type of the products
+    using Work = KvWork<S::kRows, S::kKeys, kFewOver>;
+    using Cursor = KvCursor<S::kRows, S::kKeys, kFewOver>;
     constexpr int kTiles = D / 8, kSteps = D / 16;                // column tiles of the output, steps of the first product
-    constexpr int kNt = S::kWarpKeys / 8;                         // key tiles of a warp's block
+    constexpr int kNt = S::kStepKeys / 8;                         // key tiles of a warp's step
     pdl_launch_dependents();
     pdl_wait();
-    extern __shared__ __align__(128) unsigned char smem[];
-    using Work = KvWork<S::kRows, kFewKeys, kFewOver>;
-    using Cursor = KvCursor<S::kRows, kFewKeys, kFewOver>;
+    extern __shared__ __align__(128) unsigned char smem_raw[];
     __shared__ int64_t s_sum[kFewThreads / S::kLanes + 1];
     __shared__ KvTable<kFewTable> s_table;
     __shared__ Cursor s_cursor;
-    __shared__ float2 s_ml[kFewWarps / 2][16];
+    __shared__ float2 s_ml[S::kWk][S::kRows];
+    __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages];
     __shared__ bool s_last;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    __shared__ volatile int s_failed;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int wm = warp % WM, wk = warp / WM;
+    unsigned char* const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    if (threadIdx.x == 0) {
+        // a block is there when its tensor copies are (lane 0 says how many bytes) and every lane's own copies
+        for (int i = 0; i < S::kStages; ++i) { mbar_init(&full[i], 33); mbar_init(&empty[i], kFewWarps); }
+        s_failed = 0;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
     const Work work(p, a, s_table);
     KvRun run;
     if (!kv_find_run<kFewThreads, S::kLanes>(work, s_sum, s_cursor, run)) return;
-    Cursor get = s_cursor;                                        // copies (put) run ahead of the products (get)
-    if (get.block == get.end && !get.next_segment(work)) return;
-    Cursor put = get;
-    bool more = true;                                             // put stands at a block
+    const uint32_t base = smem_addr(smem);
 
     // ---- copies ------------------------------------------------------------------------------------------------------
-    constexpr int kPerThread = kFewKeys * S::kChunks / kFewThreads, kRowStep = kFewThreads / S::kChunks;
-    const int chunk = tid % S::kChunks, row0 = tid / S::kChunks;
-    const uint32_t base = smem_addr(smem);
-    int64_t place[kPerThread];                                    // of the next block to copy: its keys' vectors, or -1
-    int64_t scale_place = -1;
-    auto key_place = [&](int key) -> int64_t {
-        return key >= put.seg.key0 && key < put.seg.key1 ? kv_place(p, put.b, key) : -1;
-    };
-    auto look_up = [&]() {
-        const int first = put.seg.low + put.block * kFewKeys;
-        const int64_t head = static_cast<int64_t>(put.head) * p.page_size;
-#pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-            place[i] = key_place(first + row0 + i * kRowStep);
-            if (place[i] >= 0) place[i] += head;
+    const int parts = box_rows > 0 ? S::kKeys / box_rows : 0;
+    // a warp asks for the block at `at`; where the place was used before, once all warps are through with it
+    auto copy_block = [&](const Cursor& at, int stage, bool wait, uint32_t parity) {
+        const int chunk = lane % S::kChunks, row0 = lane / S::kChunks;
+        constexpr int kRowStep = 32 / S::kChunks;
+        const int first = at.seg.low + at.block * S::kKeys;
+        // Lane i looks up the i-th part of the block: a tensor copy where every key of it is a token that some row of the sequence
+        // sees (and so holds numbers), row by row with zeros where not.
+        const int low = a.window > 0 ? max(0, at.seq.first_pos + 1 - a.window) : 0;
+        const int high = min(at.seq.first_pos + min(at.seq.n, a.max_new), work.capacity);
+        int64_t from = -1;
+        if (lane < parts) {
+            const int key = first + lane * box_rows;
+            if (key >= low && key + box_rows <= high) from = kv_place(p, at.b, key);
         }
-        if constexpr (BITS != 16) {
-            scale_place = key_place(first + (tid & 63));
-            if (scale_place >= 0) scale_place += head;
-        }
-    };
-    auto copy_block = [&](int stage) {
+        const uint32_t whole = __ballot_sync(0xffffffffu, from >= 0);
+        if (wait) qmm_wait(&empty[stage], parity, &s_failed);
+        __syncwarp();
         const uint32_t dst = base + stage * S::kStageBytes;
+        if (from >= 0) {
+            const int row = static_cast<int>(from) + at.head * p.page_size;
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-            const uint32_t at = dst + tile_at<S::kChunks>(row0 + i * kRowStep, chunk);
-            const int64_t from = (place[i] < 0 ? 0 : place[i]) * S::kRowBytes + chunk * 16;
-            copy16_fill(at, static_cast<const char*>(p.k) + from, place[i] >= 0);
-            copy16_fill(at + S::kTileBytes, static_cast<const char*>(p.v) + from, place[i] >= 0);
+            for (int c = 0; c < S::kRowBytes; c += 128) {
+                constexpr int kWidth = S::kRowBytes < 128 ? S::kRowBytes : 128;
+                const uint32_t to = dst + c * S::kKeys + lane * box_rows * kWidth;
+                tma_rows(to, &k_map, c, row, &full[stage]);
+                tma_rows(to + S::kTileBytes, &v_map, c, row, &full[stage]);
+            }
         }
-        if constexpr (BITS != 16)
-            copy4_fill(dst + 2 * S::kTileBytes + tid * 4, (tid < kFewKeys ? p.k_scale : p.v_scale) + (scale_place < 0 ? 0 : scale_place), scale_place >= 0);
-    };
-    int asked = 0;
-    auto ask = [&]() {
-        if (more) {
-            copy_block(asked);
-            if (++asked == S::kStages) asked = 0;
-            more = put.step(work);
-            if (more) look_up();
-        }
-        copy_commit();
-    };
-    look_up();
+        __syncwarp();
+        if (parts == 0 || __popc(whole) < parts || BITS != 16) {
+            const int64_t head = static_cast<int64_t>(at.head) * p.page_size;
 #pragma unroll 1
-    for (int i = 0; i < S::kStages - 1; ++i) ask();
+            for (int k0 = 0; k0 < S::kKeys; k0 += 32) {       // 32 keys: lane i finds key k0 + i
+                const int key = first + k0 + lane;
+                int64_t place = -1;
+                if (key >= at.seg.key0 && key < at.seg.key1) place = kv_place(p, at.b, key);
+                if (place >= 0) place += head;
+                if constexpr (BITS != 16) {
+                    const uint32_t to = dst + 2 * S::kTileBytes + (k0 + lane) * 4;
+                    copy4_fill(to, p.k_scale + (place < 0 ? 0 : place), place >= 0);
+                    copy4_fill(to + S::kKeys * 4, p.v_scale + (place < 0 ? 0 : place), place >= 0);
+                }
+                if (parts > 0 && __popc(whole) == parts) continue;
+#pragma unroll
+                for (int i = 0; i < 32 / kRowStep; ++i) {
+                    const int r = row0 + i * kRowStep;
+                    const int64_t row = __shfl_sync(0xffffffffu, place, r);
+                    if (parts == 0 || !(whole >> ((k0 + r) / box_rows) & 1u)) {
+                        const uint32_t to = dst + tile_at<S::kChunks, S::kKeys>(k0 + r, chunk);
+                        const int64_t src = (row < 0 ? 0 : row) * S::kRowBytes + chunk * 16;
+                        copy16_fill(to, static_cast<const char*>(p.k) + src, row >= 0);
+                        copy16_fill(to + S::kTileBytes, static_cast<const char*>(p.v) + src, row >= 0);
+                    }
+                }
+            }
+        }
+        copy_arrive(&full[stage]);
+        if (lane == 0) mbar_expect_tx(&full[stage], static_cast<uint32_t>(__popc(whole) * box_rows * 2 * S::kRowBytes));
+        __syncwarp();
+    };
+    Cursor put = s_cursor;                                        // copies (put) run ahead of the products (get)
+    bool more = true;                                             // put stands at a block
+    for (int i = 0; i < S::kStages - 1 && more; ++i) {
+        if (i % kFewWarps == warp) copy_block(put, i, false, 0);
+        more = put.step(work);
+    }
+    Cursor get = s_cursor;
 
     // ---- state of a segment ---------------------------------------------------------------------------------------------
     uint32_t q[kSteps][4];
-    float out[kTiles][4], m[2], l[2], unit = 0.0f, row_scale[2];
+    float out[kTiles][4], m[2], l[2], unit = 0.0f, unit_inverse = 0.0f, row_scale[2];
     int position[2];                                              // of this lane's two rows; -1: no row
     auto begin = [&]() {
         const int rows = work.rows_of(get.seq);
@@ -175,7 +214,7 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
             l[h] = 0.0f;
             row_scale[h] = a.scale_log2e;
         }
-        unit = 0.0f;
+        unit = unit_inverse = 0.0f;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) out[i][0] = out[i][1] = out[i][2] = out[i][3] = 0.0f;
         // the order of the dimensions within a step is the one the keys come in
@@ -226,9 +265,8 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
     };
 
     // ---- a block of a warp's keys ---------------------------------------------------------------------------------------
-    auto multiply = [&](int stage) {
+    auto multiply = [&](int stage, int wrow) {
         const uint32_t keys = base + stage * S::kStageBytes, values = keys + S::kTileBytes;
-        const int wrow = wk * S::kWarpKeys;
         const int mrow = (lane & 7) + ((lane >> 4) << 3), mchunk = (lane >> 3) & 1;     // matrices of keys: (octet, chunk) = (0, 0) (0, 1) (1, 0) (1, 1)
         float s[kNt][4];
 #pragma unroll
@@ -238,7 +276,7 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
 #pragma unroll
             for (int i = 0; i < kNt; i += 2) {
                 uint32_t r[4];
-                ldmatrix4(keys + tile_at<S::kChunks>(wrow + i * 8 + mrow, c + mchunk), r);
+                ldmatrix4(keys + tile_at<S::kChunks, S::kKeys>(wrow + i * 8 + mrow, c + mchunk), r);
                 if constexpr (BITS == 16) {
                     mma_rows<M>(s[i], q[c / 2], r[0], r[1]);
                     mma_rows<M>(s[i + 1], q[c / 2], r[2], r[3]);
@@ -258,61 +296,74 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
             }
         const float* scales = reinterpret_cast<const float*>(smem + stage * S::kStageBytes + 2 * S::kTileBytes) + wrow + 2 * t;
         float2 vs[kNt];
-        float unit_ratio = 1.0f;
+        bool rescale = false;
+        float factor[2] = {1.0f, 1.0f};                           // of the outputs so far
         if constexpr (BITS != 16) {
             float top = 0.0f;
 #pragma unroll
             for (int i = 0; i < kNt; ++i) {
                 const float2 ks = *reinterpret_cast<const float2*>(scales + i * 8);
-                vs[i] = *reinterpret_cast<const float2*>(scales + kFewKeys + i * 8);
+                vs[i] = *reinterpret_cast<const float2*>(scales + S::kKeys + i * 8);
                 top = fmaxf(top, fmaxf(vs[i].x, vs[i].y));
                 s[i][0] *= ks.x; s[i][1] *= ks.y; s[i][2] *= ks.x; s[i][3] *= ks.y;
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            if (top > unit) {
-                unit_ratio = unit / top;
-                unit = top;
+            if (top > unit) {                                     // the same for all lanes
+                // a quarter more, so that the unit seldom moves; its inverse need not be exact, only the same at the end
+                factor[0] = factor[1] = unit / (1.25f * top);
+                unit = 1.25f * top;
+                unit_inverse = 1.0f / unit;
+                rescale = true;
             }
-            const float inverse = unit > 0.0f ? 1.0f / unit : 0.0f;
 #pragma unroll
-            for (int i = 0; i < kNt; ++i) { vs[i].x *= inverse; vs[i].y *= inverse; }
+            for (int i = 0; i < kNt; ++i) { vs[i].x *= unit_inverse; vs[i].y *= unit_inverse; }
         }
         // masks, maximum, probabilities
-        const int first = get.seg.low + get.block * kFewKeys + wrow + 2 * t;
+        const int first = get.seg.low + get.block * S::kKeys + wrow + 2 * t;
+        float shift[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int end = min(position[h] + 1, work.capacity);
-            const int start = a.window > 0 ? position[h] + 1 - a.window : 0;
-            float top = m[h];
+            const int end = min(position[h] + 1, work.capacity) - first, start = (a.window > 0 ? position[h] + 1 - a.window : 0) - first;
+            float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < kNt; ++i)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int key = first + i * 8 + e;
                     float& x = s[i][2 * h + e];
-                    x = key < end && key >= start ? x * row_scale[h] : -INFINITY;
+                    x = i * 8 + e < end && i * 8 + e >= start ? x * row_scale[h] : -INFINITY;
                     top = fmaxf(top, x);
                 }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float safe = top == -INFINITY ? 0.0f : top;     // a row that saw nothing yet
-            const float correction = exp2_fast(m[h] - safe);
-            m[h] = top;
+            if (top > m[h] + 8.0f) {                              // also from -inf; the same for a row's four lanes
+                const float c = exp2_fast(m[h] - top);
+                m[h] = top;
+                l[h] *= c;
+                factor[h] *= c;
+                rescale = true;
+            }
+            shift[h] = m[h] == -INFINITY ? 0.0f : m[h];           // a row that saw nothing yet
+        }
+        if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                out[i][0] *= factor[0]; out[i][1] *= factor[0]; out[i][2] *= factor[1]; out[i][3] *= factor[1];
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < kNt; ++i)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     float& x = s[i][2 * h + e];
-                    x = exp2_fast(x - safe);
+                    x = exp2_fast(x - shift[h]);
                     sum += x;
                     if constexpr (BITS != 16) x *= e ? vs[i].y : vs[i].x;
                 }
-            l[h] = fmaf(l[h], correction, sum);
-            const float factor = BITS == 16 ? correction : correction * unit_ratio;
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i) { out[i][2 * h] *= factor; out[i][2 * h + 1] *= factor; }
+            l[h] += sum;
         }
         // probabilities times values
         const int vrow = (lane & 7) + ((lane >> 3) & 1) * 8, vchunk = lane >> 4;         // matrices of values: (octet, chunk) = (0, 0) (1, 0) (0, 1) (1, 1)
@@ -323,7 +374,7 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
 #pragma unroll
             for (int c = 0; c < S::kChunks; c += 2) {
                 uint32_t r[4];
-                ldmatrix4_trans(values + tile_at<S::kChunks>(wrow + k * 16 + vrow, c + vchunk), r);
+                ldmatrix4_trans(values + tile_at<S::kChunks, S::kKeys>(wrow + k * 16 + vrow, c + vchunk), r);
                 if constexpr (BITS == 16) {
                     mma_rows<M>(out[c], pr, r[0], r[1]);
                     mma_rows<M>(out[c + 1], pr, r[2], r[3]);
@@ -354,155 +405,166 @@ kv_few_kernel(const KvArgs p, const KvAttentionArgs a) {
     };
 
     // ---- end of a segment, or of this CTA's part of it ----------------------------------------------------------------
-    auto store_row = [&](int r, int d, float v0, float v1, bool pair) {     // row r of the segment's sequence
+    // The warps' outputs of the rows that there are go through shared memory; then a warp at a time holds a row, joins what the WK warps
+    // made of their keys and stores it, or this CTA's part of it.
+    constexpr int kLaneDims = D / 32;
+    auto store_row = [&](int r, const float (&v)[kLaneDims]) {            // row r of the segment's sequence; this lane's dimensions
         const int token = r / work.group;
-        T* dst = static_cast<T*>(a.out) + (get.seq.first_row + token) * a.out_stride + static_cast<int64_t>(get.head * work.group + r - token * work.group) * D + d;
-        const uint32_t w = KvType<T>::pack(v0, v1);
-        if (pair) *reinterpret_cast<uint32_t*>(dst) = w;
-        else *dst = reinterpret_cast<const T*>(&w)[0];
+        T* dst = static_cast<T*>(a.out) + (get.seq.first_row + token) * a.out_stride +
+                 static_cast<int64_t>(get.head * work.group + r - token * work.group) * D + lane * kLaneDims;
+#pragma unroll
+        for (int e = 0; e < kLaneDims; e += 2) reinterpret_cast<uint32_t*>(dst)[e / 2] = KvType<T>::pack(v[e], v[e + 1]);
+    };
+    auto load_row = [&](const float* src, float (&v)[kLaneDims]) {
+        if constexpr (kLaneDims == 4) {
+            const float4 f = __ldcg(reinterpret_cast<const float4*>(src) + lane);
+            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+        } else {
+            const float2 f = __ldcg(reinterpret_cast<const float2*>(src) + lane);
+            v[0] = f.x; v[1] = f.y;
+        }
     };
     auto finish = [&](int stage) {
-        float* merge = reinterpret_cast<float*>(smem + (S::kMergeInStage ? stage : S::kStages) * S::kStageBytes);
-        if constexpr (S::kMergeInStage && S::kWk > 1) __syncthreads();     // every warp is through with the block
+        float* const merge = reinterpret_cast<float*>(smem + (S::kMergeInStage ? stage : S::kStages) * S::kStageBytes);      // [row][warp of its keys][dimension]
+        const int tile0 = get.tile * S::kRows, rows_here = min(S::kRows, work.rows_of(get.seq) - tile0);
+        group_sync(1, 32 * kFewWarps);                            // every warp is through with the block
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        }
-        if constexpr (BITS != 16) {
+            const int r = wm * 16 + g + 8 * h;
+            if (r < rows_here) {
+                if (t == 0) s_ml[wk][r] = make_float2(m[h], l[h]);
+                float* dst = merge + (r * S::kWk + wk) * D;
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) out[i][e] *= unit;
-        }
-        // the warps that took other keys of the same rows, the upper half into the lower
-#pragma unroll
-        for (int half = S::kWk / 2; half >= 1; half >>= 1) {
-            if (wk >= half && wk < 2 * half) {
-                float* dst = merge + ((wk - half) * WM + wm) * 16 * S::kMergeStride;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (t == 0) s_ml[(wk - half) * WM + wm][g + 8 * h] = make_float2(m[h], l[h]);
-#pragma unroll
-                    for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) dst[(g + 8 * h) * S::kMergeStride + i * 8 + 2 * t + e] = out[i][2 * h + e];
-                }
-            }
-            __syncthreads();
-            if (wk < half) {
-                const float* src = merge + (wk * WM + wm) * 16 * S::kMergeStride;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float2 o = s_ml[wk * WM + wm][g + 8 * h];
-                    const float top = fmaxf(m[h], o.x), safe = top == -INFINITY ? 0.0f : top;
-                    const float c0 = exp2_fast(m[h] - safe), c1 = exp2_fast(o.x - safe);
-                    m[h] = top;
-                    l[h] = l[h] * c0 + o.y * c1;
-#pragma unroll
-                    for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            out[i][2 * h + e] = out[i][2 * h + e] * c0 + src[(g + 8 * h) * S::kMergeStride + i * 8 + 2 * t + e] * c1;
-                }
-            }
-            __syncthreads();
-        }
-        const int rows = work.rows_of(get.seq), tile0 = get.tile * S::kRows;
-        const int64_t first_unit = get.base + kFewOver;
-        const int c0 = run.cta_of(first_unit), c1 = run.cta_of(first_unit + get.seg.blocks - 1);     // CTAs that hold its first and last block
-        if (c0 == c1) {
-            if (wk == 0) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int r = tile0 + wm * 16 + g + 8 * h;
-                    if (r >= rows) continue;
-                    const float inverse = kv_inverse(l[h]);
-#pragma unroll
-                    for (int i = 0; i < kTiles; ++i) {
-                        if constexpr (BITS == 16) {
-                            store_row(r, dim_of(i, 0), out[i][2 * h] * inverse, out[i][2 * h + 1] * inverse, true);
-                        } else {
-                            store_row(r, dim_of(i, 0), out[i][2 * h] * inverse, 0.0f, false);
-                            store_row(r, dim_of(i, 1), out[i][2 * h + 1] * inverse, 0.0f, false);
-                        }
+                for (int i = 0; i < kTiles; ++i) {
+                    const float scale = BITS == 16 ? 1.0f : unit;
+                    if constexpr (BITS == 16) {
+                        *reinterpret_cast<float2*>(dst + dim_of(i, 0)) = make_float2(out[i][2 * h], out[i][2 * h + 1]);
+                    } else {
+                        dst[dim_of(i, 0)] = out[i][2 * h] * scale;
+                        dst[dim_of(i, 1)] = out[i][2 * h + 1] * scale;
                     }
                 }
             }
-            return;
         }
-        // this CTA's part: its first place for a segment that began before its run, else the second
+        group_sync(1, 32 * kFewWarps);
+        const int64_t first_unit = get.base + kFewOver;
+        const int c0 = run.cta_of(first_unit), c1 = run.cta_of(first_unit + get.seg.blocks - 1);      // CTAs that hold its first and last block
+        // a CTA's part: its first place for a segment that began before its run, else the second
         auto part_of = [&](int c) { return a.parts + (2 * c + (c == c0 ? 1 : 0)) * static_cast<int64_t>(S::kPartFloats); };
-        float* part = part_of(blockIdx.x);
-        if (wk == 0) {
+#pragma unroll 1
+        for (int r = warp; r < rows_here; r += kFewWarps) {
+            float top = -INFINITY, sum = 0.0f, o[kLaneDims];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = wm * 16 + g + 8 * h;
-                if (tile0 + r >= rows) continue;
-                if (t == 0) reinterpret_cast<float2*>(part + S::kRows * D)[r] = make_float2(m[h], l[h]);
+            for (int w = 0; w < S::kWk; ++w) top = fmaxf(top, s_ml[w][r].x);
+            const float safe = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-                for (int i = 0; i < kTiles; ++i)
+            for (int e = 0; e < kLaneDims; ++e) o[e] = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) part[r * D + dim_of(i, e)] = out[i][2 * h + e];
+            for (int w = 0; w < S::kWk; ++w) {
+                const float2 ml = s_ml[w][r];
+                const float c = exp2_fast(ml.x - safe);
+                sum = fmaf(ml.y, c, sum);
+                const float* src = merge + (r * S::kWk + w) * D + lane * kLaneDims;
+#pragma unroll
+                for (int e = 0; e < kLaneDims; ++e) o[e] = fmaf(src[e], c, o[e]);
+            }
+            if (c0 == c1) {
+                const float inverse = kv_inverse(sum);
+#pragma unroll
+                for (int e = 0; e < kLaneDims; ++e) o[e] *= inverse;
+                store_row(tile0 + r, o);
+            } else {
+                float* part = part_of(blockIdx.x);
+                if (lane == 0) reinterpret_cast<float2*>(part + S::kRows * D)[r] = make_float2(top, sum);
+#pragma unroll
+                for (int e = 0; e < kLaneDims; ++e) part[r * D + lane * kLaneDims + e] = o[e];
             }
         }
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-            const unsigned int before = atomicAdd(a.arrived + c0, 1u);
-            s_last = before == static_cast<unsigned int>(c1 - c0);
-            if (s_last) a.arrived[c0] = 0;                        // the next call starts from zero
-        }
-        __syncthreads();
-        if (!s_last) return;
-        __threadfence();
-        // a warp joins a row: its lanes weigh the parts, then every lane adds its dimensions over the parts in order
-        const int parts = c1 - c0 + 1, rows_here = min(S::kRows, rows - tile0);
-        for (int r = warp; r < rows_here; r += kFewWarps) {
-            auto weight_of = [&](int q_) { return __ldcg(reinterpret_cast<const float2*>(part_of(c0 + q_) + S::kRows * D) + r); };
-            float top = -INFINITY;
-            for (int q_ = lane; q_ < parts; q_ += 32) top = fmaxf(top, weight_of(q_).x);
+        if (c0 != c1) {
+            __threadfence();
+            group_sync(1, 32 * kFewWarps);
+            if (threadIdx.x == 0) {
+                const unsigned int before = atomicAdd(a.arrived + c0, 1u);
+                s_last = before == static_cast<unsigned int>(c1 - c0);
+                if (s_last) a.arrived[c0] = 0;                    // the next call starts from zero
+            }
+            group_sync(1, 32 * kFewWarps);
+            if (s_last) {
+                __threadfence();
+                // a warp's lanes weigh the parts, then every lane adds its dimensions over the parts in order
+                const int parts = c1 - c0 + 1;
+#pragma unroll 1
+                for (int r = warp; r < rows_here; r += kFewWarps) {
+                    auto weight_of = [&](int i) { return __ldcg(reinterpret_cast<const float2*>(part_of(c0 + i) + S::kRows * D) + r); };
+                    float top = -INFINITY;
+                    for (int i = lane; i < parts; i += 32) top = fmaxf(top, weight_of(i).x);
 #pragma unroll
-            for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float safe = top == -INFINITY ? 0.0f : top;
-            float sum = 0.0f, o[D / 32];
+                    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    const float safe = top == -INFINITY ? 0.0f : top;
+                    float sum = 0.0f, o[kLaneDims];
 #pragma unroll
-            for (int e = 0; e < D / 32; ++e) o[e] = 0.0f;
-            for (int q0 = 0; q0 < parts; q0 += 32) {
-                float2 ml = make_float2(-INFINITY, 0.0f);
-                if (q0 + lane < parts) ml = weight_of(q0 + lane);
-                const float c = exp2_fast(ml.x - safe);
-                sum += c * ml.y;
-                const int n = min(32, parts - q0);
-#pragma unroll 8
-                for (int i = 0; i < n; ++i) {
-                    const float w = __shfl_sync(0xffffffffu, c, i);
-                    const float* src = part_of(c0 + q0 + i) + r * D;
+                    for (int e = 0; e < kLaneDims; ++e) o[e] = 0.0f;
+                    for (int i0 = 0; i0 < parts; i0 += 32) {
+                        float2 ml = make_float2(-INFINITY, 0.0f);
+                        if (i0 + lane < parts) ml = weight_of(i0 + lane);
+                        const float c = exp2_fast(ml.x - safe);
+                        sum += c * ml.y;
+                        // sixteen parts on their way at a time; what is none counts for nothing
+                        for (int j = i0; j < min(i0 + 32, parts); j += 16) {
+                            float v[16][kLaneDims];
 #pragma unroll
-                    for (int e = 0; e < D / 32; ++e) o[e] = fmaf(__ldcg(src + lane * (D / 32) + e), w, o[e]);
+                            for (int i = 0; i < 16; ++i) load_row(part_of(c0 + min(j + i, parts - 1)) + r * D, v[i]);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float w = __shfl_sync(0xffffffffu, c, (j - i0 + i) & 31);
+#pragma unroll
+                                for (int e = 0; e < kLaneDims; ++e) o[e] = fmaf(v[i][e], j + i < parts ? w : 0.0f, o[e]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                    const float inverse = kv_inverse(sum);
+#pragma unroll
+                    for (int e = 0; e < kLaneDims; ++e) o[e] *= inverse;
+                    store_row(tile0 + r, o);
                 }
             }
-#pragma unroll
-            for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            const float inverse = kv_inverse(sum);
-#pragma unroll
-            for (int e = 0; e < D / 32; e += 2) store_row(tile0 + r, lane * (D / 32) + e, o[e] * inverse, o[e + 1] * inverse, true);
         }
+        // the block's place goes back to the tensor copies
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        group_sync(1, 32 * kFewWarps);
     };
 
     // ---- the run ------------------------------------------------------------------------------------------------------
     begin();
-    for (int stage = 0;; stage = stage + 1 == S::kStages ? 0 : stage + 1) {
-        copy_wait<S::kStages - 2>();
-        __syncthreads();                                          // the block has landed, and the one before was used by all
-        ask();
-        multiply(stage);
-        if (++get.block == get.end) {
-            finish(stage);
+    uint32_t parity = 0;
+    for (int stage = 0, turn = S::kStages - 1;; ++turn) {
+        if (more) {
+            // into the place of the block before: used by it in the round before this one where stage is 0
+            const bool used = turn >= S::kStages;
+            const int to = stage == 0 ? S::kStages - 1 : stage - 1;
+            if (turn % kFewWarps == warp) copy_block(put, to, used, stage == 0 ? parity ^ 1u : parity);
+            more = put.step(work);
+        }
+        qmm_wait(&full[stage], parity, &s_failed);
+        __syncwarp();
+#pragma unroll 1
+        for (int k = 0; k < S::kWarpKeys; k += S::kStepKeys) multiply(stage, wk * S::kWarpKeys + k);
+        const bool end = ++get.block == get.end;
+        if (end) finish(stage);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
+        if (end) {
             if (!get.next_segment(work)) break;
             begin();
         }
+        if (++stage == S::kStages) { stage = 0; parity ^= 1u; }
     }
+    __syncthreads();
+    if (threadIdx.x == 0 && s_failed) atomicExch(a.error, 8u);
 }
 
 template <typename T, int BITS, int D, int WM>
@@ -514,7 +576,11 @@ cudaError_t launch_few(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t s
         if (e != cudaSuccess) return e;
         attribute.mark();
     }
-    return launch_dependent(kv_few_kernel<T, BITS, D, WM>, dim3(static_cast<unsigned>(kFewCtasPerSm * sm_count())), dim3(kFewThreads), S::kSmem, stream, p, a);
+    CUtensorMap k_map{}, v_map{};
+    int box_rows = 0;
+    if (!kv_tensor_maps(p, S::kKeys, &k_map, &v_map, &box_rows)) box_rows = 0;
+    return launch_dependent(kv_few_kernel<T, BITS, D, WM>, dim3(static_cast<unsigned>(kFewCtasPerSm * sm_count())), dim3(kFewThreads), S::kSmem, stream,
+                            k_map, v_map, p, a, box_rows);
 }
 
 // Up to this many rows per key head the few-row kernel takes a sequence.

@@ -16,9 +16,6 @@
 // outside the visible range.  One thread issues the products.  Every wait is bounded; one that gives up sets the status word, all roles run on
 // to the end, and the kernel frees its tensor memory.
 #include "kv_work.cuh"
-#include "tcgen05.cuh"
-
-#include <cuda.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -88,12 +85,6 @@ __device__ __forceinline__ uint32_t many_at(int rows, int r, int c) {
     return static_cast<uint32_t>((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(c0), "r"(c1) : "memory");
-}
-
 // Two fp32 numbers in one instruction
 struct Pair {
     uint64_t v;
@@ -148,16 +139,6 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     const Work work(p, a, s_table);
     KvRun run;
     if (!kv_find_run<kManyThreads, 32>(work, s_sum, s_cursor, run)) return;
-    if (s_cursor.block == s_cursor.end) {                         // the run begins in a segment that is another CTA's
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            Cursor c = s_cursor;
-            if (!c.next_segment(work)) c.end = c.block;
-            s_cursor = c;
-        }
-        __syncthreads();
-        if (s_cursor.block == s_cursor.end) return;
-    }
     unsigned char* const queries = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     unsigned char* const tiles = queries + S::kQueryBytes;
 
@@ -475,7 +456,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 const int row = static_cast<int>(from) + at.head * p.page_size;
 #pragma unroll
                 for (int h = 0; h < D / 64; ++h)
-                    tma_rows(dst + h * kManyKeys * 128 + lane * box_rows * 128, w & 1 ? &v_map : &k_map, h * 64, row, &kv_full[slot]);
+                    tma_rows(dst + h * kManyKeys * 128 + lane * box_rows * 128, w & 1 ? &v_map : &k_map, h * 128, row, &kv_full[slot]);
             }
             __syncwarp();
             if (__popc(whole) < parts || parts == 0) {
@@ -589,29 +570,6 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     if (threadIdx.x == 0 && s_failed) atomicExch(a.error, 8u);
 }
 
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encode_fn() {
-    static EncodeFn fn = [] {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult qres;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) != cudaSuccess || qres != cudaDriverEntryPointSuccess)
-            return static_cast<EncodeFn>(nullptr);
-        return reinterpret_cast<EncodeFn>(ptr);
-    }();
-    return fn;
-}
-// the pool's vectors as rows of a 2-D tensor: boxes of 64 dimensions x box_rows, 128-byte swizzle
-bool encode_pool(CUtensorMap* map, const KvArgs& p, void* pool, int box_rows) {
-    EncodeFn encode = encode_fn();
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.head_dim), static_cast<cuuint64_t>(p.pages) * p.kv_heads * p.page_size};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.head_dim) * 2};
-    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)}, elem[2] = {1, 1};
-    return encode && encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, pool, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int BITS, int D>
 cudaError_t launch_many(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t stream) {
     using S = ManyShape<BITS, D>;
@@ -621,11 +579,9 @@ cudaError_t launch_many(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t 
         if (e != cudaSuccess) return e;
         attribute.mark();
     }
-    // tensor copies of the largest power of two that divides the page size, from eight rows (a swizzle atom) on
     CUtensorMap k_map{}, v_map{};
-    int box_rows = std::min(kManyKeys, p.page_size & -p.page_size);
-    if (box_rows < 8 || p.pages * p.kv_heads * p.page_size > INT32_MAX || !encode_pool(&k_map, p, p.k, box_rows) || !encode_pool(&v_map, p, p.v, box_rows))
-        box_rows = 0;
+    int box_rows = 0;
+    if (!kv_tensor_maps(p, kManyKeys, &k_map, &v_map, &box_rows)) box_rows = 0;
     return launch_dependent(kv_many_kernel<T, BITS, D>, dim3(static_cast<unsigned>(sm_count())), dim3(kManyThreads), S::kSmem, stream, k_map, v_map, p, a,
                             box_rows);
 }

@@ -7,7 +7,10 @@
 // the parts in the order of the keys.
 #pragma once
 
+#include <cuda.h>
+
 #include "kv.cuh"
+#include "tcgen05.cuh"
 
 namespace b200exl3 {
 
@@ -123,13 +126,28 @@ struct KvCursor {
     __device__ __forceinline__ bool step(const Work& w) { return ++block < end || next_segment(w); }
 };
 
-// A CTA's run of units u0 .. u1 - 1 of `total`, dealt out to `ctas` CTAs.
-struct KvRun {
-    int64_t total, u0, u1;
-    int ctas;
+__device__ __forceinline__ int64_t kv_quotient(int64_t a, int64_t b) {      // of non-negative numbers
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
 
+// `total` units dealt out to `ctas` CTAs: `each` to every one, one more to the first `more`.
+struct KvRun {
+    int64_t total, each;
+    int ctas, more;
+
+    __device__ __forceinline__ void deal(int64_t total_, int grid) {
+        total = total_;
+        ctas = static_cast<int>(min(static_cast<int64_t>(grid), total));
+        each = ctas > 0 ? kv_quotient(total, ctas) : 0;
+        more = static_cast<int>(total - each * ctas);
+    }
+    __device__ __forceinline__ int64_t first(int cta) const { return cta * each + min(cta, more); }
     // the CTA that holds unit u
-    __device__ __forceinline__ int cta_of(int64_t u) const { return static_cast<int>(((u + 1) * ctas - 1) / total); }
+    __device__ __forceinline__ int cta_of(int64_t u) const {
+        const int64_t longer = more * (each + 1);
+        return static_cast<int>(u < longer ? kv_quotient(u, each + 1) : more + kv_quotient(u - longer, each));
+    }
 };
 
 // Finds this CTA's run; every thread of the block calls it.  Workers of LANES threads (1, or 32: sequences of many row tiles) count a
@@ -163,14 +181,11 @@ __device__ __forceinline__ bool kv_find_run(const KvWork<ROWS, KEYS, OVER>& w, i
         if (threadIdx.x == 0) s_sum[kWorkers] = carry;
     }
     __syncthreads();
-    run.total = s_sum[kWorkers];
-    run.ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), run.total));
+    run.deal(s_sum[kWorkers], gridDim.x);
     if (static_cast<int>(blockIdx.x) >= run.ctas) return false;
-    run.u0 = run.total * blockIdx.x / run.ctas;
-    run.u1 = run.total * (blockIdx.x + 1) / run.ctas;
-    const int64_t before = s_sum[worker];
-    if (before <= run.u0 && run.u0 < before + mine) {
-        int64_t left = run.u0 - before;
+    const int64_t before = s_sum[worker], u0 = run.first(blockIdx.x);
+    if (before <= u0 && u0 < before + mine) {
+        int64_t left = u0 - before;
         KvCursor<ROWS, KEYS, OVER> c;
         for (int b = b0; b < b1; ++b) {
             c.seq = w.seq(b);
@@ -180,7 +195,7 @@ __device__ __forceinline__ bool kv_find_run(const KvWork<ROWS, KEYS, OVER>& w, i
                 continue;
             }
             c.b = b;
-            c.head = static_cast<int>(left / per_head);
+            c.head = static_cast<int>(kv_quotient(left, per_head));
             left -= c.head * per_head;
             for (c.tile = 0;; c.tile += LANES) {
                 const int tile = c.tile + sub, tiles = w.tiles_of(c.seq);
@@ -206,15 +221,16 @@ __device__ __forceinline__ bool kv_find_run(const KvWork<ROWS, KEYS, OVER>& w, i
                 }
             }
             c.seg = w.segment(c.seq, c.tile);
-            c.base = run.u0 - left;
-            c.left = run.u1 - run.u0;
+            c.base = u0 - left;
+            c.left = run.first(blockIdx.x + 1) - u0;
             c.enter(left);
+            if (c.block == c.end && !c.next_segment(w)) c.end = c.block;     // the run begins before a segment's first block
             break;
         }
         if (sub == 0) s_cursor = c;
     }
     __syncthreads();
-    return s_cursor.block < s_cursor.end || s_cursor.left > 0;
+    return s_cursor.block < s_cursor.end;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {             // 2 ulp; exp2(-inf) = 0
@@ -233,5 +249,16 @@ __device__ __forceinline__ void copy4_fill(uint32_t dst, const void* src, bool l
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// `rows` rows of the pool, 128 bytes of each at most (column c0 on), into shared memory by the tensor-copy unit
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int c0, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(c0), "r"(row) : "memory");
+}
+
+// Host: the pool's vectors as rows of a 2-D tensor, copied in boxes of box_rows rows of up to 128 bytes, swizzled over the row's width.
+// False where there are no such copies; box_rows is the largest power of two that divides the page size, at most `most`.
+bool kv_tensor_maps(const KvArgs& p, int most, CUtensorMap* k_map, CUtensorMap* v_map, int* box_rows);
 
 }  // namespace b200exl3
