@@ -333,6 +333,7 @@ bool kv_tensor_maps(const KvArgs& p, int most, CUtensorMap* k_map, CUtensorMap* 
     const int64_t vectors = p.pages * p.kv_heads * p.page_size;
     const int rows = std::min(most, p.page_size & -p.page_size);
     if (!encode || rows < 8 || vectors > INT32_MAX) return false;       // eight rows are an atom of the swizzle
+    if (p.bits != 16 && ((reinterpret_cast<uintptr_t>(p.k_scale) | reinterpret_cast<uintptr_t>(p.v_scale)) & 15u)) return false;     // their scales are copied in bulk
     const cuuint32_t width = static_cast<cuuint32_t>(p.head_dim * p.bits / 8), box_width = std::min(width, 128u);
     const cuuint64_t dims[2] = {width, static_cast<cuuint64_t>(vectors)}, strides[1] = {width};
     const cuuint32_t box[2] = {box_width, static_cast<cuuint32_t>(rows)}, elem[2] = {1, 1};

@@ -77,6 +77,13 @@ __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
     return static_cast<uint32_t>((chunk / kPiece * KEYS + row) * kPiece + ((chunk % kPiece) ^ ((row >> kShift) & (kPiece - 1)))) * 16;
 }
 
+// The same for chunk c + of, c even and of 0 or 1, from the place of chunk `of`: the swizzle is an exclusive or.
+template <int CHUNKS, int KEYS>
+__device__ __forceinline__ uint32_t tile_next(uint32_t at, int c) {
+    constexpr int kPiece = CHUNKS >= 8 ? 8 : CHUNKS;
+    return (at ^ static_cast<uint32_t>((c % kPiece) << 4)) + static_cast<uint32_t>(c / kPiece * KEYS * kPiece * 16);
+}
+
 // Two codes as fp16.  8 bits: bytes i and j of a word whose sign bits were flipped become 1024 + (code + 128); 4 bits: the low nibbles
 // of its halves become 1024 + (code + 8).
 __device__ __forceinline__ uint32_t less(uint32_t a, uint32_t bias) {
@@ -154,9 +161,14 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
                 tma_rows(to, &k_map, c, row, &full[stage]);
                 tma_rows(to + S::kTileBytes, &v_map, c, row, &full[stage]);
             }
+            if constexpr (BITS != 16) {
+                unsigned char* const to = smem + stage * S::kStageBytes + 2 * S::kTileBytes + lane * box_rows * 4;
+                bulk_copy_g2s(to, p.k_scale + row, box_rows * 4, &full[stage]);
+                bulk_copy_g2s(to + S::kKeys * 4, p.v_scale + row, box_rows * 4, &full[stage]);
+            }
         }
         __syncwarp();
-        if (parts == 0 || __popc(whole) < parts || BITS != 16) {
+        if (parts == 0 || __popc(whole) < parts) {
             const int64_t head = static_cast<int64_t>(at.head) * p.page_size;
 #pragma unroll 1
             for (int k0 = 0; k0 < S::kKeys; k0 += 32) {       // 32 keys: lane i finds key k0 + i
@@ -164,12 +176,11 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
                 int64_t place = -1;
                 if (key >= at.seg.key0 && key < at.seg.key1) place = kv_place(p, at.b, key);
                 if (place >= 0) place += head;
-                if constexpr (BITS != 16) {
+                if (BITS != 16 && (parts == 0 || !(whole >> ((k0 + lane) / box_rows) & 1u))) {
                     const uint32_t to = dst + 2 * S::kTileBytes + (k0 + lane) * 4;
                     copy4_fill(to, p.k_scale + (place < 0 ? 0 : place), place >= 0);
                     copy4_fill(to + S::kKeys * 4, p.v_scale + (place < 0 ? 0 : place), place >= 0);
                 }
-                if (parts > 0 && __popc(whole) == parts) continue;
 #pragma unroll
                 for (int i = 0; i < 32 / kRowStep; ++i) {
                     const int r = row0 + i * kRowStep;
@@ -184,7 +195,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             }
         }
         copy_arrive(&full[stage]);
-        if (lane == 0) mbar_expect_tx(&full[stage], static_cast<uint32_t>(__popc(whole) * box_rows * 2 * S::kRowBytes));
+        if (lane == 0) mbar_expect_tx(&full[stage], static_cast<uint32_t>(__popc(whole) * box_rows * 2 * (S::kRowBytes + (BITS == 16 ? 0 : 4))));
         __syncwarp();
     };
     Cursor put = s_cursor;                                        // copies (put) run ahead of the products (get)
@@ -268,32 +279,33 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     auto multiply = [&](int stage, int wrow) {
         const uint32_t keys = base + stage * S::kStageBytes, values = keys + S::kTileBytes;
         const int mrow = (lane & 7) + ((lane >> 4) << 3), mchunk = (lane >> 3) & 1;     // matrices of keys: (octet, chunk) = (0, 0) (0, 1) (1, 0) (1, 1)
+        static_assert(kNt == 2, "a step is 16 keys");
+        const uint32_t key_at = keys + tile_at<S::kChunks, S::kKeys>(wrow + mrow, mchunk);
         float s[kNt][4];
 #pragma unroll
         for (int i = 0; i < kNt; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
 #pragma unroll
         for (int c = 0; c < S::kChunks; c += 2)
+        {
+            uint32_t r[4];
+            ldmatrix4(tile_next<S::kChunks, S::kKeys>(key_at, c), r);
+            if constexpr (BITS == 16) {
+                mma_rows<M>(s[0], q[c / 2], r[0], r[1]);
+                mma_rows<M>(s[1], q[c / 2], r[2], r[3]);
+            } else if constexpr (BITS == 8) {
 #pragma unroll
-            for (int i = 0; i < kNt; i += 2) {
-                uint32_t r[4];
-                ldmatrix4(keys + tile_at<S::kChunks, S::kKeys>(wrow + i * 8 + mrow, c + mchunk), r);
-                if constexpr (BITS == 16) {
-                    mma_rows<M>(s[i], q[c / 2], r[0], r[1]);
-                    mma_rows<M>(s[i + 1], q[c / 2], r[2], r[3]);
-                } else if constexpr (BITS == 8) {
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w = r[j] ^ 0x80808080u;
+                    mma_rows<M>(s[j >> 1], q[c + (j & 1)], codes8<0, 1>(w), codes8<2, 3>(w));
+                }
+            } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t w = r[j] ^ 0x80808080u;
-                        mma_rows<M>(s[i + (j >> 1)], q[c + (j & 1)], codes8<0, 1>(w), codes8<2, 3>(w));
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        mma_rows<M>(s[i + (j >> 1)], q[2 * (c + (j & 1))], codes4<0>(r[j]), codes4<1>(r[j]));
-                        mma_rows<M>(s[i + (j >> 1)], q[2 * (c + (j & 1)) + 1], codes4<2>(r[j]), codes4<3>(r[j]));
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    mma_rows<M>(s[j >> 1], q[2 * (c + (j & 1))], codes4<0>(r[j]), codes4<1>(r[j]));
+                    mma_rows<M>(s[j >> 1], q[2 * (c + (j & 1)) + 1], codes4<2>(r[j]), codes4<3>(r[j]));
                 }
             }
+        }
         const float* scales = reinterpret_cast<const float*>(smem + stage * S::kStageBytes + 2 * S::kTileBytes) + wrow + 2 * t;
         float2 vs[kNt];
         bool rescale = false;
@@ -325,15 +337,14 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int end = min(position[h] + 1, work.capacity) - first, start = (a.window > 0 ? position[h] + 1 - a.window : 0) - first;
-            float top = -INFINITY;
+            if (__any_sync(0xffffffffu, end < S::kStepKeys || start > -2 * t)) {
 #pragma unroll
-            for (int i = 0; i < kNt; ++i)
+                for (int i = 0; i < kNt; ++i)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float& x = s[i][2 * h + e];
-                    x = i * 8 + e < end && i * 8 + e >= start ? x * row_scale[h] : -INFINITY;
-                    top = fmaxf(top, x);
-                }
+                    for (int e = 0; e < 2; ++e)
+                        if (i * 8 + e >= end || i * 8 + e < start) s[i][2 * h + e] = -INFINITY;
+            }
+            float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1])) * row_scale[h];
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             if (top > m[h] + 8.0f) {                              // also from -inf; the same for a row's four lanes
@@ -359,7 +370,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     float& x = s[i][2 * h + e];
-                    x = exp2_fast(x - shift[h]);
+                    x = exp2_fast(fmaf(x, row_scale[h], -shift[h]));
                     sum += x;
                     if constexpr (BITS != 16) x *= e ? vs[i].y : vs[i].x;
                 }
@@ -367,14 +378,15 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         }
         // probabilities times values
         const int vrow = (lane & 7) + ((lane >> 3) & 1) * 8, vchunk = lane >> 4;         // matrices of values: (octet, chunk) = (0, 0) (1, 0) (0, 1) (1, 1)
-#pragma unroll
-        for (int k = 0; k < kNt / 2; ++k) {
+        const uint32_t value_at = values + tile_at<S::kChunks, S::kKeys>(wrow + vrow, vchunk);
+        {
+            constexpr int k = 0;
             const uint32_t pr[4] = {KvType<M>::pack(s[2 * k][0], s[2 * k][1]), KvType<M>::pack(s[2 * k][2], s[2 * k][3]),
                                     KvType<M>::pack(s[2 * k + 1][0], s[2 * k + 1][1]), KvType<M>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
 #pragma unroll
             for (int c = 0; c < S::kChunks; c += 2) {
                 uint32_t r[4];
-                ldmatrix4_trans(values + tile_at<S::kChunks, S::kKeys>(wrow + k * 16 + vrow, c + vchunk), r);
+                ldmatrix4_trans(tile_next<S::kChunks, S::kKeys>(value_at, c), r);
                 if constexpr (BITS == 16) {
                     mma_rows<M>(out[c], pr, r[0], r[1]);
                     mma_rows<M>(out[c + 1], pr, r[2], r[3]);
