@@ -32,7 +32,7 @@ struct FewShape {
     static constexpr int kKeys = BITS == 16 ? 64 : 128;            // of a block
     static constexpr int kWk = kFewWarps / WM;     // warps that share the rows and take different keys
     static constexpr int kWarpKeys = kKeys / kWk;
-    static constexpr int kStepKeys = 16;                            // of a warp's step
+    static constexpr int kStepKeys = BITS == 16 ? 16 : 32;         // of a warp's step
     static constexpr int kRows = 16 * WM;
     static constexpr int kLanes = WM == 1 ? 1 : 32;    // a sequence has one row tile, or many
     static constexpr int kRowBytes = D * BITS / 8, kChunks = kRowBytes / 16;
@@ -279,30 +279,32 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     auto multiply = [&](int stage, int wrow) {
         const uint32_t keys = base + stage * S::kStageBytes, values = keys + S::kTileBytes;
         const int mrow = (lane & 7) + ((lane >> 4) << 3), mchunk = (lane >> 3) & 1;     // matrices of keys: (octet, chunk) = (0, 0) (0, 1) (1, 0) (1, 1)
-        static_assert(kNt == 2, "a step is 16 keys");
-        const uint32_t key_at = keys + tile_at<S::kChunks, S::kKeys>(wrow + mrow, mchunk);
+        uint32_t key_at[kNt / 2];
+#pragma unroll
+        for (int i = 0; i < kNt / 2; ++i) key_at[i] = keys + tile_at<S::kChunks, S::kKeys>(wrow + i * 16 + mrow, mchunk);
         float s[kNt][4];
 #pragma unroll
         for (int i = 0; i < kNt; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
 #pragma unroll
         for (int c = 0; c < S::kChunks; c += 2)
-        {
+#pragma unroll
+        for (int i = 0; i < kNt; i += 2) {
             uint32_t r[4];
-            ldmatrix4(tile_next<S::kChunks, S::kKeys>(key_at, c), r);
+            ldmatrix4(tile_next<S::kChunks, S::kKeys>(key_at[i / 2], c), r);
             if constexpr (BITS == 16) {
-                mma_rows<M>(s[0], q[c / 2], r[0], r[1]);
-                mma_rows<M>(s[1], q[c / 2], r[2], r[3]);
+                mma_rows<M>(s[i], q[c / 2], r[0], r[1]);
+                mma_rows<M>(s[i + 1], q[c / 2], r[2], r[3]);
             } else if constexpr (BITS == 8) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t w = r[j] ^ 0x80808080u;
-                    mma_rows<M>(s[j >> 1], q[c + (j & 1)], codes8<0, 1>(w), codes8<2, 3>(w));
+                    mma_rows<M>(s[i + (j >> 1)], q[c + (j & 1)], codes8<0, 1>(w), codes8<2, 3>(w));
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    mma_rows<M>(s[j >> 1], q[2 * (c + (j & 1))], codes4<0>(r[j]), codes4<1>(r[j]));
-                    mma_rows<M>(s[j >> 1], q[2 * (c + (j & 1)) + 1], codes4<2>(r[j]), codes4<3>(r[j]));
+                    mma_rows<M>(s[i + (j >> 1)], q[2 * (c + (j & 1))], codes4<0>(r[j]), codes4<1>(r[j]));
+                    mma_rows<M>(s[i + (j >> 1)], q[2 * (c + (j & 1)) + 1], codes4<2>(r[j]), codes4<3>(r[j]));
                 }
             }
         }
@@ -344,7 +346,10 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
                     for (int e = 0; e < 2; ++e)
                         if (i * 8 + e >= end || i * 8 + e < start) s[i][2 * h + e] = -INFINITY;
             }
-            float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1])) * row_scale[h];
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kNt; ++i) top = fmaxf(top, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
+            top *= row_scale[h];
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             if (top > m[h] + 8.0f) {                              // also from -inf; the same for a row's four lanes
@@ -378,9 +383,9 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         }
         // probabilities times values
         const int vrow = (lane & 7) + ((lane >> 3) & 1) * 8, vchunk = lane >> 4;         // matrices of values: (octet, chunk) = (0, 0) (1, 0) (0, 1) (1, 1)
-        const uint32_t value_at = values + tile_at<S::kChunks, S::kKeys>(wrow + vrow, vchunk);
-        {
-            constexpr int k = 0;
+#pragma unroll
+        for (int k = 0; k < kNt / 2; ++k) {
+            const uint32_t value_at = values + tile_at<S::kChunks, S::kKeys>(wrow + k * 16 + vrow, vchunk);
             const uint32_t pr[4] = {KvType<M>::pack(s[2 * k][0], s[2 * k][1]), KvType<M>::pack(s[2 * k][2], s[2 * k][3]),
                                     KvType<M>::pack(s[2 * k + 1][0], s[2 * k + 1][1]), KvType<M>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
 #pragma unroll
