@@ -1,14 +1,17 @@
 // Attention of new tokens over a paged key/value cache: o_i = sum_j softmax_j(scale q_i . k_j) v_j over the tokens j up to its own
 // (with a window w: the last w of them).
 //
-// Work is shared out as kv_work.cuh says, in segments of 16 * WM rows and blocks of 64 keys (128 of codes).
+// Work is shared out as kv_work.cuh says, in segments of 8 * NB rows and blocks of 64 keys (128 of codes).
 //
 // A block: the warps take turns to ask for its keys and values (tensor copies of whole pages or parts of pages, several blocks in flight; row by
 // row with zeros at the ends of the visible range and where pages are too small, so that nothing behind a length is ever
-// multiplied); WK = 4 / WM warps take a share of the keys each against 16 rows: scores by mma.sync, online softmax in fp32 registers,
-// probabilities rounded to 16 bits for the second product.  Loads bound it: what a step of single tokens moves is the cache, once.
-// A row's maximum moves only when a score exceeds it by 2^8, so that the outputs are seldom rescaled; until then probabilities
-// reach 256, which 16 bits hold as well as 1.
+// multiplied); four warps take a quarter of the keys each: scores by mma.sync, online softmax in fp32 registers, probabilities rounded to
+// 16 bits for the second product.  Loads bound it: what a step of single tokens moves is the cache, once.
+// Both products have the keys and values as their left operand and the rows as their right one, whose tiles are 8 wide: a group of four
+// query heads leaves half of a tile idle where it would leave three quarters of a left one's 16, and scores, outputs and exponentials
+// take half the registers and instructions (long 4-bit contexts 254 -> NNN us).
+// A row's maximum moves only when a score exceeds it by 2^8, so that outputs are seldom rescaled and the lanes that share a row seldom
+// have to agree; until then probabilities reach 256, which 16 bits hold as well as 1.
 //
 // Codes are multiplied as they are: 8- and 4-bit codes are exact in fp16, and so is what the tensor cores add up in fp32; the key's
 // scale multiplies its scores, the value's its probability.  Those probabilities are taken relative to the largest value scale met so
@@ -23,26 +26,24 @@ namespace b200exl3 {
 namespace {
 
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps;
-constexpr int kFewCtasPerSm = 2;
 constexpr int kFewTable = 128;
 constexpr int kFewOver = 1;
 
-template <int BITS, int D, int WM>
+template <int BITS, int D, int NB>
 struct FewShape {
+    static constexpr int kCtas = 2;                                // per SM
     static constexpr int kKeys = BITS == 16 ? 64 : 128;            // of a block
-    static constexpr int kWk = kFewWarps / WM;     // warps that share the rows and take different keys
-    static constexpr int kWarpKeys = kKeys / kWk;
-    static constexpr int kStepKeys = BITS == 16 ? 16 : 32;         // of a warp's step
-    static constexpr int kRows = 16 * WM;
-    static constexpr int kLanes = WM == 1 ? 1 : 32;    // a sequence has one row tile, or many
+    static constexpr int kWarpKeys = kKeys / kFewWarps;            // they share the rows and take different keys
+    static constexpr int kStepKeys = std::min(kWarpKeys, 32);      // of a warp's step
+    static constexpr int kRows = 8 * NB;
     static constexpr int kRowBytes = D * BITS / 8, kChunks = kRowBytes / 16;
     static constexpr int kTileBytes = kKeys * kRowBytes;
     static constexpr int kScaleBytes = BITS == 16 ? 0 : 2 * kKeys * 4;
     static constexpr int kStageBytes = (2 * kTileBytes + kScaleBytes + 1023) / 1024 * 1024;
-    static constexpr int kMergeBytes = kFewWarps * 16 * D * 4;     // outputs of the warps, joined in the block's own place where they fit
+    static constexpr int kMergeBytes = kFewWarps * kRows * D * 4;  // outputs of the warps, joined in the block's own place where they fit
     static constexpr bool kMergeInStage = kMergeBytes <= kStageBytes;
     static constexpr int kOwnMergeBytes = kMergeInStage ? 0 : kMergeBytes;
-    static constexpr int kStages = std::min(6, (109 * 1024 - kOwnMergeBytes) / kStageBytes);      // two CTAs per SM
+    static constexpr int kStages = std::min(6, (222 * 1024 / kCtas - 2 * 1024 - kOwnMergeBytes) / kStageBytes);
     static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStageBytes + kOwnMergeBytes;
     static constexpr int kPartFloats = kRows * (D + 2);
     static_assert(kStages >= 3, "copies in flight");
@@ -97,29 +98,35 @@ template <int I> __device__ __forceinline__ uint32_t codes4(uint32_t w) {
     return less(d, 0x64086408u);
 }
 
+// Matrices of 8 x 8 numbers of 16 bits, held as the products hold them, turned over
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
+}
+
 // box_rows: rows of a tensor copy, a power of two that divides the page size, or 0: no tensor copies
-template <typename T, int BITS, int D, int WM>
-__global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
+template <typename T, int BITS, int D, int NB, int LANES>
+__global__ void __launch_bounds__(kFewThreads, FewShape<BITS, D, NB>::kCtas)
 kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const KvArgs p, const KvAttentionArgs a,
               const int box_rows) {
-    using S = FewShape<BITS, D, WM>;
+    using S = FewShape<BITS, D, NB>;
     using M = std::conditional_t<BITS == 16, T, __half>;          // type of the products
     using Work = KvWork<S::kRows, S::kKeys, kFewOver>;
     using Cursor = KvCursor<S::kRows, S::kKeys, kFewOver>;
-    constexpr int kTiles = D / 8, kSteps = D / 16;                // column tiles of the output, steps of the first product
-    constexpr int kNt = S::kStepKeys / 8;                         // key tiles of a warp's step
+    constexpr int kTiles = D / 16, kSteps = D / 16;               // tiles of the output, steps of the first product
+    constexpr int kSub = S::kStepKeys / 16;                       // tiles of keys of a warp's step
     pdl_launch_dependents();
     pdl_wait();
     extern __shared__ __align__(128) unsigned char smem_raw[];
-    __shared__ int64_t s_sum[kFewThreads / S::kLanes + 1];
+    __shared__ int64_t s_sum[kFewThreads / LANES + 1];
     __shared__ KvTable<kFewTable> s_table;
     __shared__ Cursor s_cursor;
-    __shared__ float2 s_ml[S::kWk][S::kRows];
+    __shared__ float2 s_ml[kFewWarps][S::kRows];
     __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages];
     __shared__ bool s_last;
     __shared__ volatile int s_failed;
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int wm = warp % WM, wk = warp / WM;
     unsigned char* const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     if (threadIdx.x == 0) {
         // a block is there when its tensor copies are (lane 0 says how many bytes) and every lane's own copies
@@ -129,7 +136,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     }
     const Work work(p, a, s_table);
     KvRun run;
-    if (!kv_find_run<kFewThreads, S::kLanes>(work, s_sum, s_cursor, run)) return;
+    if (!kv_find_run<kFewThreads, LANES>(work, s_sum, s_cursor, run)) return;
     const uint32_t base = smem_addr(smem);
 
     // ---- copies ------------------------------------------------------------------------------------------------------
@@ -207,222 +214,237 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     Cursor get = s_cursor;
 
     // ---- state of a segment ---------------------------------------------------------------------------------------------
-    uint32_t q[kSteps][4];
-    float out[kTiles][4], m[2], l[2], unit = 0.0f, unit_inverse = 0.0f, row_scale[2];
-    int position[2];                                              // of this lane's two rows; -1: no row
+    // A lane holds the queries of row 8 b + g; scores, sums and outputs of rows 8 b + 2 t and the next (e = 0, 1).
+    uint32_t q[NB][kSteps][2];
+    float out[NB][kTiles][4], m[NB][2], l[NB][2], row_scale[NB][2], unit = 0.0f, unit_inverse = 0.0f;
+    int position[NB][2];                                          // -1: no row
     auto begin = [&]() {
         const int rows = work.rows_of(get.seq);
-        const T* src[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = get.tile * S::kRows + wm * 16 + g + 8 * h;
-            const int token = r / work.group;
-            position[h] = r < rows ? get.seq.first_pos + token : -1;
-            src[h] = r < rows ? static_cast<const T*>(a.q) + (get.seq.first_row + token) * a.q_stride +
-                                    static_cast<int64_t>(get.head * work.group + r - token * work.group) * D
-                              : nullptr;
-            m[h] = -INFINITY;
-            l[h] = 0.0f;
-            row_scale[h] = a.scale_log2e;
-        }
         unit = unit_inverse = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) out[i][0] = out[i][1] = out[i][2] = out[i][3] = 0.0f;
-        // the order of the dimensions within a step is the one the keys come in
+        for (int b = 0; b < NB; ++b) {
+            const int row0 = get.tile * S::kRows + 8 * b;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s)
+            for (int e = 0; e < 2; ++e) {
+                const int r = row0 + 2 * t + e;
+                position[b][e] = r < rows ? get.seq.first_pos + r / work.group : -1;
+                m[b][e] = -INFINITY;
+                l[b][e] = 0.0f;
+                row_scale[b][e] = a.scale_log2e;
+            }
 #pragma unroll
-            for (int w = 0; w < 2; ++w)                           // columns 2t, 2t + 1 and 2t + 8, 2t + 9 of the step
+            for (int i = 0; i < kTiles; ++i) out[b][i][0] = out[b][i][1] = out[b][i][2] = out[b][i][3] = 0.0f;
+            const int r = row0 + g, token = r / work.group;
+            const T* const src = static_cast<const T*>(a.q) + (get.seq.first_row + token) * a.q_stride +
+                                 static_cast<int64_t>(get.head * work.group + r - token * work.group) * D;
+            // the order of the dimensions within a step is the one the keys come in
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {                     // places 2t, 2t + 1 and 2t + 8, 2t + 9 of the step
                     uint32_t v = 0;
-                    if (src[h] != nullptr) {
-                        if constexpr (BITS == 16) v = *reinterpret_cast<const uint32_t*>(src[h] + s * 16 + 2 * t + 8 * w);
-                        else if constexpr (BITS == 8) v = *reinterpret_cast<const uint32_t*>(src[h] + s * 16 + 4 * t + 2 * w);
+                    if (r < rows) {
+                        if constexpr (BITS == 16) v = *reinterpret_cast<const uint32_t*>(src + s * 16 + 2 * t + 8 * w);
+                        else if constexpr (BITS == 8) v = *reinterpret_cast<const uint32_t*>(src + s * 16 + 4 * t + 2 * w);
                         else {
-                            const uint16_t* e = reinterpret_cast<const uint16_t*>(src[h]) + (s >> 1) * 32 + 8 * t + 2 * (s & 1) + w;
+                            const uint16_t* e = reinterpret_cast<const uint16_t*>(src) + (s >> 1) * 32 + 8 * t + 2 * (s & 1) + w;
                             v = e[0] | static_cast<uint32_t>(e[4]) << 16;
                         }
                     }
-                    q[s][2 * w + h] = v;
+                    q[b][s][w] = v;
                 }
-        if constexpr (!std::is_same_v<T, M>) {
-            // bf16 rows enter fp16 products: scaled by the power of two that brings the row's largest to [1, 2)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            if constexpr (!std::is_same_v<T, M>) {
+                // bf16 rows enter fp16 products: scaled by the power of two that brings the row's largest to [1, 2)
                 float top = 0.0f;
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s)
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
-                        const float2 f = KvType<T>::unpack(q[s][2 * w + h]);
+                        const float2 f = KvType<T>::unpack(q[b][s][w]);
                         top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
                     }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
-                // |e| <= 133: in two factors, each a normal number
-                const float f0 = ldexpf(1.0f, -e / 2), f1 = ldexpf(1.0f, -e - -e / 2);
-                row_scale[h] = ldexpf(row_scale[h], e);
+                const int x = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
+                // |x| <= 133: in two factors, each a normal number
+                const float f0 = ldexpf(1.0f, -x / 2), f1 = ldexpf(1.0f, -x - -x / 2);
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s)
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
-                        const float2 f = KvType<T>::unpack(q[s][2 * w + h]);
-                        q[s][2 * w + h] = KvType<M>::pack(f.x * f0 * f1, f.y * f0 * f1);
+                        const float2 f = KvType<T>::unpack(q[b][s][w]);
+                        q[b][s][w] = KvType<M>::pack(f.x * f0 * f1, f.y * f0 * f1);
                     }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) row_scale[b][e] = ldexpf(row_scale[b][e], __shfl_sync(0xffffffffu, x, (2 * t + e) * 4));
             }
         }
     };
 
-    // ---- a block of a warp's keys ---------------------------------------------------------------------------------------
+    // ---- a step of a warp's keys ----------------------------------------------------------------------------------------
     auto multiply = [&](int stage, int wrow) {
         const uint32_t keys = base + stage * S::kStageBytes, values = keys + S::kTileBytes;
-        const int mrow = (lane & 7) + ((lane >> 4) << 3), mchunk = (lane >> 3) & 1;     // matrices of keys: (octet, chunk) = (0, 0) (0, 1) (1, 0) (1, 1)
-        uint32_t key_at[kNt / 2];
+        // matrices of a load: (octet of keys, chunk) = (0, 0) (1, 0) (0, 1) (1, 1), or (0, 0) (0, 1) (1, 0) (1, 1)
+        const int row_a = (lane & 7) + ((lane >> 3) & 1) * 8, chunk_a = lane >> 4, row_b = (lane & 7) + (lane >> 4) * 8, chunk_b = (lane >> 3) & 1;
+        float s[kSub][NB][4];                                     // keys g and g + 8, rows 2t and 2t + 1
 #pragma unroll
-        for (int i = 0; i < kNt / 2; ++i) key_at[i] = keys + tile_at<S::kChunks, S::kKeys>(wrow + i * 16 + mrow, mchunk);
-        float s[kNt][4];
+        for (int k = 0; k < kSub; ++k)
 #pragma unroll
-        for (int i = 0; i < kNt; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+            for (int b = 0; b < NB; ++b) s[k][b][0] = s[k][b][1] = s[k][b][2] = s[k][b][3] = 0.0f;
 #pragma unroll
         for (int c = 0; c < S::kChunks; c += 2)
 #pragma unroll
-        for (int i = 0; i < kNt; i += 2) {
-            uint32_t r[4];
-            ldmatrix4(tile_next<S::kChunks, S::kKeys>(key_at[i / 2], c), r);
-            if constexpr (BITS == 16) {
-                mma_rows<M>(s[i], q[c / 2], r[0], r[1]);
-                mma_rows<M>(s[i + 1], q[c / 2], r[2], r[3]);
-            } else if constexpr (BITS == 8) {
+            for (int k = 0; k < kSub; ++k) {
+                uint32_t r[4];
+                ldmatrix4(tile_next<S::kChunks, S::kKeys>(keys + tile_at<S::kChunks, S::kKeys>(wrow + k * 16 + row_a, chunk_a), c), r);
+                auto product = [&](int step, const uint32_t (&v)[4]) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t w = r[j] ^ 0x80808080u;
-                    mma_rows<M>(s[i + (j >> 1)], q[c + (j & 1)], codes8<0, 1>(w), codes8<2, 3>(w));
-                }
-            } else {
+                    for (int b = 0; b < NB; ++b) mma_rows<M>(s[k][b], v, q[b][step][0], q[b][step][1]);
+                };
+                if constexpr (BITS == 16) {
+                    product(c / 2, r);
+                } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    mma_rows<M>(s[i + (j >> 1)], q[2 * (c + (j & 1))], codes4<0>(r[j]), codes4<1>(r[j]));
-                    mma_rows<M>(s[i + (j >> 1)], q[2 * (c + (j & 1)) + 1], codes4<2>(r[j]), codes4<3>(r[j]));
+                    for (int j = 0; j < 2; ++j) {
+                        if constexpr (BITS == 8) {
+                            const uint32_t w0 = r[2 * j] ^ 0x80808080u, w1 = r[2 * j + 1] ^ 0x80808080u;
+                            product(c + j, {codes8<0, 1>(w0), codes8<0, 1>(w1), codes8<2, 3>(w0), codes8<2, 3>(w1)});
+                        } else {
+                            const uint32_t w0 = r[2 * j], w1 = r[2 * j + 1];
+                            product(2 * (c + j), {codes4<0>(w0), codes4<0>(w1), codes4<1>(w0), codes4<1>(w1)});
+                            product(2 * (c + j) + 1, {codes4<2>(w0), codes4<2>(w1), codes4<3>(w0), codes4<3>(w1)});
+                        }
+                    }
                 }
             }
-        }
-        const float* scales = reinterpret_cast<const float*>(smem + stage * S::kStageBytes + 2 * S::kTileBytes) + wrow + 2 * t;
-        float2 vs[kNt];
+        const float* scales = reinterpret_cast<const float*>(smem + stage * S::kStageBytes + 2 * S::kTileBytes) + wrow + g;
+        float vs[kSub][2];
         bool rescale = false;
-        float factor[2] = {1.0f, 1.0f};                           // of the outputs so far
+        float factor[NB][2];                                      // of the outputs so far
+#pragma unroll
+        for (int b = 0; b < NB; ++b) factor[b][0] = factor[b][1] = 1.0f;
         if constexpr (BITS != 16) {
             float top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kNt; ++i) {
-                const float2 ks = *reinterpret_cast<const float2*>(scales + i * 8);
-                vs[i] = *reinterpret_cast<const float2*>(scales + S::kKeys + i * 8);
-                top = fmaxf(top, fmaxf(vs[i].x, vs[i].y));
-                s[i][0] *= ks.x; s[i][1] *= ks.y; s[i][2] *= ks.x; s[i][3] *= ks.y;
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            if (top > unit) {                                     // the same for all lanes
+            for (int k = 0; k < kSub; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float ks = scales[k * 16 + 8 * h];
+                    vs[k][h] = scales[S::kKeys + k * 16 + 8 * h];
+                    top = fmaxf(top, vs[k][h]);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) { s[k][b][2 * h] *= ks; s[k][b][2 * h + 1] *= ks; }
+                }
+            if (__any_sync(0xffffffffu, top > unit)) {
+#pragma unroll
+                for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                 // a quarter more, so that the unit seldom moves; its inverse need not be exact, only the same at the end
-                factor[0] = factor[1] = unit / (1.25f * top);
+                const float ratio = unit / (1.25f * top);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) factor[b][0] = factor[b][1] = ratio;
                 unit = 1.25f * top;
                 unit_inverse = 1.0f / unit;
                 rescale = true;
             }
 #pragma unroll
-            for (int i = 0; i < kNt; ++i) { vs[i].x *= unit_inverse; vs[i].y *= unit_inverse; }
+            for (int k = 0; k < kSub; ++k) { vs[k][0] *= unit_inverse; vs[k][1] *= unit_inverse; }
         }
         // masks, maximum, probabilities
-        const int first = get.seg.low + get.block * S::kKeys + wrow + 2 * t;
-        float shift[2];
+        const int first = get.seg.low + get.block * S::kKeys + wrow + g;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int end = min(position[h] + 1, work.capacity) - first, start = (a.window > 0 ? position[h] + 1 - a.window : 0) - first;
-            if (__any_sync(0xffffffffu, end < S::kStepKeys || start > -2 * t)) {
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int i = 0; i < kNt; ++i)
+            for (int e = 0; e < 2; ++e) {
+                const int end = min(position[b][e] + 1, work.capacity) - first, start = (a.window > 0 ? position[b][e] + 1 - a.window : 0) - first;
+                if (__any_sync(0xffffffffu, end < S::kStepKeys - 7 || start > 0)) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        if (i * 8 + e >= end || i * 8 + e < start) s[i][2 * h + e] = -INFINITY;
-            }
-            float top = -INFINITY;
+                    for (int k = 0; k < kSub; ++k)
 #pragma unroll
-            for (int i = 0; i < kNt; ++i) top = fmaxf(top, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
-            top *= row_scale[h];
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            if (top > m[h] + 8.0f) {                              // also from -inf; the same for a row's four lanes
-                const float c = exp2_fast(m[h] - top);
-                m[h] = top;
-                l[h] *= c;
-                factor[h] *= c;
-                rescale = true;
-            }
-            shift[h] = m[h] == -INFINITY ? 0.0f : m[h];           // a row that saw nothing yet
-        }
-        if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i) {
-                out[i][0] *= factor[0]; out[i][1] *= factor[0]; out[i][2] *= factor[1]; out[i][3] *= factor[1];
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kNt; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float& x = s[i][2 * h + e];
-                    x = exp2_fast(fmaf(x, row_scale[h], -shift[h]));
-                    sum += x;
-                    if constexpr (BITS != 16) x *= e ? vs[i].y : vs[i].x;
+                        for (int h = 0; h < 2; ++h)
+                            if (k * 16 + 8 * h >= end || k * 16 + 8 * h < start) s[k][b][2 * h + e] = -INFINITY;
                 }
-            l[h] += sum;
-        }
-        // probabilities times values
-        const int vrow = (lane & 7) + ((lane >> 3) & 1) * 8, vchunk = lane >> 4;         // matrices of values: (octet, chunk) = (0, 0) (1, 0) (0, 1) (1, 1)
+                float top = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < kNt / 2; ++k) {
-            const uint32_t value_at = values + tile_at<S::kChunks, S::kKeys>(wrow + k * 16 + vrow, vchunk);
-            const uint32_t pr[4] = {KvType<M>::pack(s[2 * k][0], s[2 * k][1]), KvType<M>::pack(s[2 * k][2], s[2 * k][3]),
-                                    KvType<M>::pack(s[2 * k + 1][0], s[2 * k + 1][1]), KvType<M>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
+                for (int k = 0; k < kSub; ++k) top = fmaxf(top, fmaxf(s[k][b][e], s[k][b][2 + e]));
+                top *= row_scale[b][e];
+                if (__any_sync(0xffffffffu, top > m[b][e] + 8.0f)) {              // also from -inf
+#pragma unroll
+                    for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    if (top > m[b][e]) {                          // the same for all lanes of the row
+                        const float c = exp2_fast(m[b][e] - top);
+                        m[b][e] = top;
+                        l[b][e] *= c;
+                        factor[b][e] *= c;
+                    }
+                    rescale = true;
+                }
+            }
+        if (rescale) {                                            // the same for all lanes
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) {
+                    out[b][i][0] *= factor[b][0]; out[b][i][1] *= factor[b][1]; out[b][i][2] *= factor[b][0]; out[b][i][3] *= factor[b][1];
+                }
+        }
+        uint32_t pr[kSub][NB][2];                                 // probabilities as the right operand: keys 2t, 2t + 1 (+ 8) of row g
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float shift[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) shift[e] = m[b][e] == -INFINITY ? 0.0f : -m[b][e];        // a row that saw nothing yet
+#pragma unroll
+            for (int k = 0; k < kSub; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float x[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        x[e] = exp2_fast(fmaf(s[k][b][2 * h + e], row_scale[b][e], shift[e]));
+                        l[b][e] += x[e];
+                        if constexpr (BITS != 16) x[e] *= vs[k][h];
+                    }
+                    pr[k][b][h] = transposed(KvType<M>::pack(x[0], x[1]));
+                }
+        }
+        // values times probabilities
+#pragma unroll
+        for (int k = 0; k < kSub; ++k)
 #pragma unroll
             for (int c = 0; c < S::kChunks; c += 2) {
                 uint32_t r[4];
-                ldmatrix4_trans(tile_next<S::kChunks, S::kKeys>(value_at, c), r);
+                auto product = [&](int tile, const uint32_t (&v)[4]) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) mma_rows<M>(out[b][tile], v, pr[k][b][0], pr[k][b][1]);
+                };
                 if constexpr (BITS == 16) {
-                    mma_rows<M>(out[c], pr, r[0], r[1]);
-                    mma_rows<M>(out[c + 1], pr, r[2], r[3]);
-                } else if constexpr (BITS == 8) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const uint32_t w0 = r[2 * j] ^ 0x80808080u, w1 = r[2 * j + 1] ^ 0x80808080u;
-                        mma_rows<M>(out[2 * (c + j)], pr, codes8<0, 2>(w0), codes8<0, 2>(w1));
-                        mma_rows<M>(out[2 * (c + j) + 1], pr, codes8<1, 3>(w0), codes8<1, 3>(w1));
-                    }
+                    ldmatrix4_trans(tile_next<S::kChunks, S::kKeys>(values + tile_at<S::kChunks, S::kKeys>(wrow + k * 16 + row_b, chunk_b), c), r);
+                    product(c / 2, r);
                 } else {
+                    ldmatrix4_trans(tile_next<S::kChunks, S::kKeys>(values + tile_at<S::kChunks, S::kKeys>(wrow + k * 16 + row_a, chunk_a), c), r);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        mma_rows<M>(out[4 * (c + j)], pr, codes4<0>(r[2 * j]), codes4<0>(r[2 * j + 1]));
-                        mma_rows<M>(out[4 * (c + j) + 1], pr, codes4<1>(r[2 * j]), codes4<1>(r[2 * j + 1]));
-                        mma_rows<M>(out[4 * (c + j) + 2], pr, codes4<2>(r[2 * j]), codes4<2>(r[2 * j + 1]));
-                        mma_rows<M>(out[4 * (c + j) + 3], pr, codes4<3>(r[2 * j]), codes4<3>(r[2 * j + 1]));
+                        if constexpr (BITS == 8) {
+                            const uint32_t w0 = r[2 * j] ^ 0x80808080u, w1 = r[2 * j + 1] ^ 0x80808080u;
+                            product(c + j, {codes8<0, 2>(w0), codes8<1, 3>(w0), codes8<0, 2>(w1), codes8<1, 3>(w1)});
+                        } else {
+                            const uint32_t w0 = r[2 * j], w1 = r[2 * j + 1];
+                            product(2 * (c + j), {codes4<0>(w0), codes4<1>(w0), codes4<0>(w1), codes4<1>(w1)});
+                            product(2 * (c + j) + 1, {codes4<2>(w0), codes4<3>(w0), codes4<2>(w1), codes4<3>(w1)});
+                        }
                     }
                 }
             }
-        }
     };
-    // dimension of out[i][e] (e = 0, 1): where the values' chunks put it
-    auto dim_of = [&](int i, int e) {
-        if constexpr (BITS == 16) return i * 8 + 2 * t + e;
-        else if constexpr (BITS == 8) return (i >> 1) * 16 + 2 * (2 * t + e) + (i & 1);
-        else return (i >> 2) * 32 + 4 * (2 * t + e) + (i & 3);
+    // dimension of out[.][i][2 h + e]: where the values' chunks put it
+    auto dim_of = [&](int i, int h) {
+        if constexpr (BITS == 16) return i * 16 + 8 * h + g;
+        else if constexpr (BITS == 8) return i * 16 + 2 * g + h;
+        else return (i >> 1) * 32 + 4 * g + 2 * (i & 1) + h;
     };
 
     // ---- end of a segment, or of this CTA's part of it ----------------------------------------------------------------
-    // The warps' outputs of the rows that there are go through shared memory; then a warp at a time holds a row, joins what the WK warps
+    // The warps' outputs of the rows that there are go through shared memory; then a warp at a time holds a row, joins what the warps
     // made of their keys and stores it, or this CTA's part of it.
     constexpr int kLaneDims = D / 32;
     auto store_row = [&](int r, const float (&v)[kLaneDims]) {            // row r of the segment's sequence; this lane's dimensions
@@ -446,25 +468,21 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         const int tile0 = get.tile * S::kRows, rows_here = min(S::kRows, work.rows_of(get.seq) - tile0);
         group_sync(1, 32 * kFewWarps);                            // every warp is through with the block
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            const int r = wm * 16 + g + 8 * h;
-            if (r < rows_here) {
-                if (t == 0) s_ml[wk][r] = make_float2(m[h], l[h]);
-                float* dst = merge + (r * S::kWk + wk) * D;
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int i = 0; i < kTiles; ++i) {
-                    const float scale = BITS == 16 ? 1.0f : unit;
-                    if constexpr (BITS == 16) {
-                        *reinterpret_cast<float2*>(dst + dim_of(i, 0)) = make_float2(out[i][2 * h], out[i][2 * h + 1]);
-                    } else {
-                        dst[dim_of(i, 0)] = out[i][2 * h] * scale;
-                        dst[dim_of(i, 1)] = out[i][2 * h + 1] * scale;
-                    }
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int d = 4; d <= 16; d <<= 1) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], d);
+                const int r = 8 * b + 2 * t + e;
+                if (r < rows_here) {
+                    if (g == 0) s_ml[warp][r] = make_float2(m[b][e], l[b][e]);
+                    float* dst = merge + (r * kFewWarps + warp) * D;
+#pragma unroll
+                    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) dst[dim_of(i, h)] = BITS == 16 ? out[b][i][2 * h + e] : out[b][i][2 * h + e] * unit;
                 }
             }
-        }
         group_sync(1, 32 * kFewWarps);
         const int64_t first_unit = get.base + kFewOver;
         const int c0 = run.cta_of(first_unit), c1 = run.cta_of(first_unit + get.seg.blocks - 1);      // CTAs that hold its first and last block
@@ -474,16 +492,16 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         for (int r = warp; r < rows_here; r += kFewWarps) {
             float top = -INFINITY, sum = 0.0f, o[kLaneDims];
 #pragma unroll
-            for (int w = 0; w < S::kWk; ++w) top = fmaxf(top, s_ml[w][r].x);
+            for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, s_ml[w][r].x);
             const float safe = top == -INFINITY ? 0.0f : top;
 #pragma unroll
             for (int e = 0; e < kLaneDims; ++e) o[e] = 0.0f;
 #pragma unroll
-            for (int w = 0; w < S::kWk; ++w) {
+            for (int w = 0; w < kFewWarps; ++w) {
                 const float2 ml = s_ml[w][r];
                 const float c = exp2_fast(ml.x - safe);
                 sum = fmaf(ml.y, c, sum);
-                const float* src = merge + (r * S::kWk + w) * D + lane * kLaneDims;
+                const float* src = merge + (r * kFewWarps + w) * D + lane * kLaneDims;
 #pragma unroll
                 for (int e = 0; e < kLaneDims; ++e) o[e] = fmaf(src[e], c, o[e]);
             }
@@ -569,7 +587,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         qmm_wait(&full[stage], parity, &s_failed);
         __syncwarp();
 #pragma unroll 1
-        for (int k = 0; k < S::kWarpKeys; k += S::kStepKeys) multiply(stage, wk * S::kWarpKeys + k);
+        for (int k = 0; k < S::kWarpKeys; k += S::kStepKeys) multiply(stage, warp * S::kWarpKeys + k);
         const bool end = ++get.block == get.end;
         if (end) finish(stage);
         __syncwarp();
@@ -584,19 +602,19 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     if (threadIdx.x == 0 && s_failed) atomicExch(a.error, 8u);
 }
 
-template <typename T, int BITS, int D, int WM>
+template <typename T, int BITS, int D, int NB, int LANES = 1>
 cudaError_t launch_few(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t stream) {
-    using S = FewShape<BITS, D, WM>;
+    using S = FewShape<BITS, D, NB>;
     static PerDeviceOnce attribute;
     if (attribute.needed()) {
-        cudaError_t e = cudaFuncSetAttribute(kv_few_kernel<T, BITS, D, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
+        cudaError_t e = cudaFuncSetAttribute(kv_few_kernel<T, BITS, D, NB, LANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
         if (e != cudaSuccess) return e;
         attribute.mark();
     }
     CUtensorMap k_map{}, v_map{};
     int box_rows = 0;
     if (!kv_tensor_maps(p, S::kKeys, &k_map, &v_map, &box_rows)) box_rows = 0;
-    return launch_dependent(kv_few_kernel<T, BITS, D, WM>, dim3(static_cast<unsigned>(kFewCtasPerSm * sm_count())), dim3(kFewThreads), S::kSmem, stream,
+    return launch_dependent(kv_few_kernel<T, BITS, D, NB, LANES>, dim3(static_cast<unsigned>(S::kCtas * sm_count())), dim3(kFewThreads), S::kSmem, stream,
                             k_map, v_map, p, a, box_rows);
 }
 
@@ -608,13 +626,14 @@ cudaError_t launch_attention(const KvArgs& p, KvAttentionArgs a, cudaStream_t st
     const int64_t rows = static_cast<int64_t>(a.max_new) * (a.heads / p.kv_heads);
     a.least_rows = 1;
     a.most_rows = INT32_MAX;
-    if (rows <= kFewRows) return launch_few<T, BITS, D, 1>(p, a, stream);
+    if (rows <= 8) return launch_few<T, BITS, D, 1>(p, a, stream);
+    if (rows <= kFewRows) return launch_few<T, BITS, D, 2>(p, a, stream);
     if constexpr (BITS != 16) {
-        return launch_few<T, BITS, D, 4>(p, a, stream);
+        return launch_few<T, BITS, D, 2, 32>(p, a, stream);
     } else {
         if (p.batch > 1) {                                        // sequences of few rows among the others
             a.most_rows = kFewRows;
-            const cudaError_t e = launch_few<T, BITS, D, 1>(p, a, stream);
+            const cudaError_t e = launch_few<T, BITS, D, 2>(p, a, stream);
             if (e != cudaSuccess) return e;
             a.least_rows = kFewRows + 1;
             a.most_rows = INT32_MAX;
@@ -625,8 +644,8 @@ cudaError_t launch_attention(const KvArgs& p, KvAttentionArgs a, cudaStream_t st
 
 }  // namespace
 
-size_t kv_attention_workspace_bytes(int bits, int head_dim, int group, int64_t max_new) {
-    const size_t few = 2 * static_cast<size_t>(kFewCtasPerSm * sm_count()) * (bits == 16 ? 16 : 64) * (head_dim + 2) * sizeof(float);
+size_t kv_attention_workspace_bytes(int, int head_dim, int group, int64_t max_new) {
+    const size_t few = 2 * static_cast<size_t>(2 * sm_count()) * 16 * (head_dim + 2) * sizeof(float);
     return max_new * group <= kFewRows ? few : std::max(few, kv_many_workspace_bytes(head_dim));
 }
 
