@@ -9,7 +9,7 @@
 // 16 bits for the second product.  Loads bound it: what a step of single tokens moves is the cache, once.
 // Both products have the keys and values as their left operand and the rows as their right one, whose tiles are 8 wide: a group of four
 // query heads leaves half of a tile idle where it would leave three quarters of a left one's 16, and scores, outputs and exponentials
-// take half the registers and instructions (long 4-bit contexts 254 -> NNN us).
+// take half the registers and instructions (long 4-bit contexts 254 -> 208 us; with a third CTA per SM 189).
 // A row's maximum moves only when a score exceeds it by 2^8, so that outputs are seldom rescaled and the lanes that share a row seldom
 // have to agree; until then probabilities reach 256, which 16 bits hold as well as 1.
 //
@@ -31,7 +31,7 @@ constexpr int kFewOver = 1;
 
 template <int BITS, int D, int NB>
 struct FewShape {
-    static constexpr int kCtas = 2;                                // per SM
+    static constexpr int kCtas = BITS == 4 && NB == 1 ? 3 : 2;      // per SM
     static constexpr int kKeys = BITS == 16 ? 64 : 128;            // of a block
     static constexpr int kWarpKeys = kKeys / kFewWarps;            // they share the rows and take different keys
     static constexpr int kStepKeys = std::min(kWarpKeys, 32);      // of a warp's step
@@ -121,7 +121,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     extern __shared__ __align__(128) unsigned char smem_raw[];
     __shared__ int64_t s_sum[kFewThreads / LANES + 1];
     __shared__ KvTable<kFewTable> s_table;
-    __shared__ Cursor s_cursor;
+    __shared__ Cursor s_cursor, s_put[kFewWarps], s_get[kFewWarps];
     __shared__ float2 s_ml[kFewWarps][S::kRows];
     __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages];
     __shared__ bool s_last;
@@ -142,10 +142,10 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     // ---- copies ------------------------------------------------------------------------------------------------------
     const int parts = box_rows > 0 ? S::kKeys / box_rows : 0;
     // a warp asks for the block at `at`; where the place was used before, once all warps are through with it
-    auto copy_block = [&](const Cursor& at, int stage, bool wait, uint32_t parity) {
+    auto copy_block = [&](const Cursor& at, int block, int stage, bool wait, uint32_t parity) {
         const int chunk = lane % S::kChunks, row0 = lane / S::kChunks;
         constexpr int kRowStep = 32 / S::kChunks;
-        const int first = at.seg.low + at.block * S::kKeys;
+        const int first = at.seg.low + block * S::kKeys;
         // Lane i looks up the i-th part of the block: a tensor copy where every key of it is a token that some row of the sequence
         // sees (and so holds numbers), row by row with zeros where not.
         const int low = a.window > 0 ? max(0, at.seq.first_pos + 1 - a.window) : 0;
@@ -205,13 +205,34 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         if (lane == 0) mbar_expect_tx(&full[stage], static_cast<uint32_t>(__popc(whole) * box_rows * 2 * (S::kRowBytes + (BITS == 16 ? 0 : 4))));
         __syncwarp();
     };
-    Cursor put = s_cursor;                                        // copies (put) run ahead of the products (get)
+    // Copies (put) run ahead of the products (get).  Every warp keeps both places for itself in shared memory and in registers only which
+    // blocks of the segment are left.
+    Cursor& put = s_put[warp];
+    Cursor& get = s_get[warp];
+    auto next_segment = [&](Cursor& c) {
+        Cursor next = c;
+        const bool ok = next.next_segment(work);
+        __syncwarp();
+        c = next;                                                 // the same from all lanes
+        __syncwarp();
+        return ok;
+    };
+    put = s_cursor;
+    get = s_cursor;
+    __syncwarp();
+    int put_block = put.block, put_end = put.end;
     bool more = true;                                             // put stands at a block
+    auto step_put = [&]() {
+        if (++put_block < put_end) return true;
+        if (!next_segment(put)) return false;
+        put_block = put.block;
+        put_end = put.end;
+        return true;
+    };
     for (int i = 0; i < S::kStages - 1 && more; ++i) {
-        if (i % kFewWarps == warp) copy_block(put, i, false, 0);
-        more = put.step(work);
+        if (i % kFewWarps == warp) copy_block(put, put_block, i, false, 0);
+        more = step_put();
     }
-    Cursor get = s_cursor;
 
     // ---- state of a segment ---------------------------------------------------------------------------------------------
     // A lane holds the queries of row 8 b + g; scores, sums and outputs of rows 8 b + 2 t and the next (e = 0, 1).
@@ -282,7 +303,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     };
 
     // ---- a step of a warp's keys ----------------------------------------------------------------------------------------
-    auto multiply = [&](int stage, int wrow) {
+    auto multiply = [&](int stage, int wrow, int block_key) {
         const uint32_t keys = base + stage * S::kStageBytes, values = keys + S::kTileBytes;
         // matrices of a load: (octet of keys, chunk) = (0, 0) (1, 0) (0, 1) (1, 1), or (0, 0) (0, 1) (1, 0) (1, 1)
         const int row_a = (lane & 7) + ((lane >> 3) & 1) * 8, chunk_a = lane >> 4, row_b = (lane & 7) + (lane >> 4) * 8, chunk_b = (lane >> 3) & 1;
@@ -350,7 +371,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             for (int k = 0; k < kSub; ++k) { vs[k][0] *= unit_inverse; vs[k][1] *= unit_inverse; }
         }
         // masks, maximum, probabilities
-        const int first = get.seg.low + get.block * S::kKeys + wrow + g;
+        const int first = block_key + wrow + g;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -575,26 +596,30 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
 
     // ---- the run ------------------------------------------------------------------------------------------------------
     begin();
+    int block_key = get.seg.low + get.block * S::kKeys, left = get.end - get.block;      // first key of the block; blocks of the segment
     uint32_t parity = 0;
     for (int stage = 0, turn = S::kStages - 1;; ++turn) {
         if (more) {
             // into the place of the block before: used by it in the round before this one where stage is 0
             const bool used = turn >= S::kStages;
             const int to = stage == 0 ? S::kStages - 1 : stage - 1;
-            if (turn % kFewWarps == warp) copy_block(put, to, used, stage == 0 ? parity ^ 1u : parity);
-            more = put.step(work);
+            if (turn % kFewWarps == warp) copy_block(put, put_block, to, used, stage == 0 ? parity ^ 1u : parity);
+            more = step_put();
         }
         qmm_wait(&full[stage], parity, &s_failed);
         __syncwarp();
 #pragma unroll 1
-        for (int k = 0; k < S::kWarpKeys; k += S::kStepKeys) multiply(stage, warp * S::kWarpKeys + k);
-        const bool end = ++get.block == get.end;
+        for (int k = 0; k < S::kWarpKeys; k += S::kStepKeys) multiply(stage, warp * S::kWarpKeys + k, block_key);
+        block_key += S::kKeys;
+        const bool end = --left == 0;
         if (end) finish(stage);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[stage]);
         if (end) {
-            if (!get.next_segment(work)) break;
+            if (!next_segment(get)) break;
             begin();
+            block_key = get.seg.low + get.block * S::kKeys;
+            left = get.end - get.block;
         }
         if (++stage == S::kStages) { stage = 0; parity ^= 1u; }
     }
@@ -645,7 +670,7 @@ cudaError_t launch_attention(const KvArgs& p, KvAttentionArgs a, cudaStream_t st
 }  // namespace
 
 size_t kv_attention_workspace_bytes(int, int head_dim, int group, int64_t max_new) {
-    const size_t few = 2 * static_cast<size_t>(2 * sm_count()) * 16 * (head_dim + 2) * sizeof(float);
+    const size_t few = 2 * static_cast<size_t>(3 * sm_count()) * 16 * (head_dim + 2) * sizeof(float);
     return max_new * group <= kFewRows ? few : std::max(few, kv_many_workspace_bytes(head_dim));
 }
 
