@@ -85,19 +85,6 @@ __device__ __forceinline__ uint32_t tile_next(uint32_t at, int c) {
     return (at ^ static_cast<uint32_t>((c % kPiece) << 4)) + static_cast<uint32_t>(c / kPiece * KEYS * kPiece * 16);
 }
 
-// Two codes as fp16.  8 bits: bytes i and j of a word whose sign bits were flipped become 1024 + (code + 128); 4 bits: the low nibbles
-// of its halves become 1024 + (code + 8).
-__device__ __forceinline__ uint32_t less(uint32_t a, uint32_t bias) {
-    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&bias));
-    return *reinterpret_cast<const uint32_t*>(&d);
-}
-template <int I, int J> __device__ __forceinline__ uint32_t codes8(uint32_t w) { return less(prmt(w, 0x64646464u, 0x4040u | I | (J << 8)), 0x64806480u); }
-template <int I> __device__ __forceinline__ uint32_t codes4(uint32_t w) {
-    uint32_t d;
-    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(d) : "r"(w >> (4 * I)));    // (w & mask) | bias
-    return less(d, 0x64086408u);
-}
-
 // Matrices of 8 x 8 numbers of 16 bits, held as the products hold them, turned over
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     uint32_t d;
@@ -106,7 +93,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
 }
 
 // box_rows: rows of a tensor copy, a power of two that divides the page size, or 0: no tensor copies
-template <typename T, int BITS, int D, int NB, int LANES>
+template <typename T, int BITS, int D, int NB>
 __global__ void __launch_bounds__(kFewThreads, FewShape<BITS, D, NB>::kCtas)
 kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const KvArgs p, const KvAttentionArgs a,
               const int box_rows) {
@@ -119,7 +106,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     pdl_launch_dependents();
     pdl_wait();
     extern __shared__ __align__(128) unsigned char smem_raw[];
-    __shared__ int64_t s_sum[kFewThreads / LANES + 1];
+    __shared__ int64_t s_sum[kFewThreads + 1];
     __shared__ KvTable<kFewTable> s_table;
     __shared__ Cursor s_cursor, s_put[kFewWarps], s_get[kFewWarps];
     __shared__ float2 s_ml[kFewWarps][S::kRows];
@@ -136,7 +123,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     }
     const Work work(p, a, s_table);
     KvRun run;
-    if (!kv_find_run<kFewThreads, LANES>(work, s_sum, s_cursor, run)) return;
+    if (!kv_find_run<kFewThreads, 1>(work, s_sum, s_cursor, run)) return;
     const uint32_t base = smem_addr(smem);
 
     // ---- copies ------------------------------------------------------------------------------------------------------
@@ -627,19 +614,19 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     if (threadIdx.x == 0 && s_failed) atomicExch(a.error, 8u);
 }
 
-template <typename T, int BITS, int D, int NB, int LANES = 1>
+template <typename T, int BITS, int D, int NB>
 cudaError_t launch_few(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t stream) {
     using S = FewShape<BITS, D, NB>;
     static PerDeviceOnce attribute;
     if (attribute.needed()) {
-        cudaError_t e = cudaFuncSetAttribute(kv_few_kernel<T, BITS, D, NB, LANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
+        cudaError_t e = cudaFuncSetAttribute(kv_few_kernel<T, BITS, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
         if (e != cudaSuccess) return e;
         attribute.mark();
     }
     CUtensorMap k_map{}, v_map{};
     int box_rows = 0;
     if (!kv_tensor_maps(p, S::kKeys, &k_map, &v_map, &box_rows)) box_rows = 0;
-    return launch_dependent(kv_few_kernel<T, BITS, D, NB, LANES>, dim3(static_cast<unsigned>(S::kCtas * sm_count())), dim3(kFewThreads), S::kSmem, stream,
+    return launch_dependent(kv_few_kernel<T, BITS, D, NB>, dim3(static_cast<unsigned>(S::kCtas * sm_count())), dim3(kFewThreads), S::kSmem, stream,
                             k_map, v_map, p, a, box_rows);
 }
 
@@ -653,18 +640,14 @@ cudaError_t launch_attention(const KvArgs& p, KvAttentionArgs a, cudaStream_t st
     a.most_rows = INT32_MAX;
     if (rows <= 8) return launch_few<T, BITS, D, 1>(p, a, stream);
     if (rows <= kFewRows) return launch_few<T, BITS, D, 2>(p, a, stream);
-    if constexpr (BITS != 16) {
-        return launch_few<T, BITS, D, 2, 32>(p, a, stream);
-    } else {
-        if (p.batch > 1) {                                        // sequences of few rows among the others
-            a.most_rows = kFewRows;
-            const cudaError_t e = launch_few<T, BITS, D, 2>(p, a, stream);
-            if (e != cudaSuccess) return e;
-            a.least_rows = kFewRows + 1;
-            a.most_rows = INT32_MAX;
-        }
-        return launch_kv_many(p, a, stream);
+    if (p.batch > 1) {                                            // sequences of few rows among the others
+        a.most_rows = kFewRows;
+        const cudaError_t e = launch_few<T, BITS, D, 2>(p, a, stream);
+        if (e != cudaSuccess) return e;
+        a.least_rows = kFewRows + 1;
+        a.most_rows = INT32_MAX;
     }
+    return launch_kv_many(p, a, stream);
 }
 
 }  // namespace

@@ -13,7 +13,10 @@
 //
 // Four warps bring the data, a tile (a block's keys or values) each in turn, into the 128-byte swizzle that the products read: tensor
 // copies of whole pages or parts of pages where every key of the block is visible, else 16 bytes at a time with zeros for what lies
-// outside the visible range.  One thread issues the products.  Every wait is bounded; one that gives up sets the status word, all roles run on
+// outside the visible range.  One thread issues the products.  Of a quantised cache those warps load the codes and store them as
+// fp16, exactly; the key's scale multiplies its scores and the value's its probability, where m bounds their product (a row's largest
+// score plus log2 of the largest value scale of the blocks so far), so that it fits 16 bits whatever the scales' magnitude.  bf16 queries
+// enter those fp16 products multiplied by a power of two of their own.  Every wait is bounded; one that gives up sets the status word, all roles run on
 // to the end, and the kernel frees its tensor memory.
 #include "kv_work.cuh"
 
@@ -38,7 +41,9 @@ struct ManyShape {
     static constexpr int kQueryBytes = kManyRows * D * 2;
     static constexpr int kStageRow = 80;                           // a row of 32 results on its way out, 64 bytes without bank conflicts
     static constexpr int kStageBytes = kSoftmaxWarps * 32 * kStageRow;
-    static constexpr size_t kSmem = 1024 + kQueryBytes + static_cast<size_t>(kSlots) * kTileBytes + kStageBytes;
+    static constexpr int kScaleBlocks = 4;                         // blocks whose scales are kept: [key and value scales][128 keys], with codes
+    static constexpr int kScaleBytes = BITS == 16 ? 0 : kScaleBlocks * 2 * kManyKeys * 4;
+    static constexpr size_t kSmem = 1024 + kQueryBytes + static_cast<size_t>(kSlots) * kTileBytes + kStageBytes + kScaleBytes;
     static constexpr int kPartFloats = kManyRows * (D + 2);
     static constexpr uint32_t kOutCols = 2 * kScoreCols;           // first column of O_0; O_1 lies D further
 };
@@ -115,12 +120,33 @@ __device__ __forceinline__ void exp2_by_fma(Pair x, float& y0, float& y1) {
     y1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
 }
 
+__device__ __forceinline__ void scale4(uint32_t* v, const float4& f) {
+    v[0] = __float_as_uint(__uint_as_float(v[0]) * f.x);
+    v[1] = __float_as_uint(__uint_as_float(v[1]) * f.y);
+    v[2] = __float_as_uint(__uint_as_float(v[2]) * f.z);
+    v[3] = __float_as_uint(__uint_as_float(v[3]) * f.w);
+}
+
+// Eight 4-bit codes of a word as fp16 in order: the two of a byte go to the halves of a word, as 1024 + u and 1024 + 16 u
+__device__ __forceinline__ void codes4_in_order(uint32_t w, uint32_t (&v)[4]) {
+    const uint32_t by = 0x2c003c00u, less_bits = 0xd480e408u;        // 1 and 1/16; -1032 and -72
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t b;
+        const uint32_t both = prmt(w, 0u, 0x4040u | i | (i << 8));
+        asm("lop3.b32 %0, %1, 0x00f0000f, 0x64006400, 0xea;" : "=r"(b) : "r"(both));       // (both & mask) | bias
+        const __half2 d = __hfma2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&by), *reinterpret_cast<const __half2*>(&less_bits));
+        v[i] = *reinterpret_cast<const uint32_t*>(&d);
+    }
+}
+
 // box_rows: rows of a tensor copy, a power of two that divides the page size, or 0: no tensor copies
 template <typename T, int BITS, int D>
 __global__ void __launch_bounds__(kManyThreads, 1)
 kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const KvArgs p, const KvAttentionArgs a,
                const int box_rows) {
     using S = ManyShape<BITS, D>;
+    using M = std::conditional_t<BITS == 16, T, __half>;          // type of the products
     using Work = KvWork<kManyRows, kManyKeys, kManyOver>;
     using Cursor = KvCursor<kManyRows, kManyKeys, kManyOver>;
     constexpr int kChunks = D / 8;
@@ -130,7 +156,8 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     __shared__ KvTable<kManyTable> s_table;
     __shared__ int64_t s_sum[kManyThreads / 32 + 1];
     __shared__ Cursor s_cursor;
-    __shared__ __align__(8) uint64_t kv_full[S::kSlots], kv_free[S::kSlots], s_full[2], p_half[2], p_full[2], o_full[2], q_full[2], drained;
+    __shared__ __align__(8) uint64_t kv_full[S::kSlots], kv_free[S::kSlots], s_full[2], p_half[2], p_full[2], o_full[2], q_full[2], drained, scales_full[S::kScaleBlocks];
+    __shared__ float s_top[S::kScaleBlocks], s_q_scale[BITS != 16 && !std::is_same_v<T, __half> ? kManyRows : 1];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int s_last[2];
     __shared__ volatile int s_failed;
@@ -141,11 +168,13 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     if (!kv_find_run<kManyThreads, 32>(work, s_sum, s_cursor, run)) return;
     unsigned char* const queries = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     unsigned char* const tiles = queries + S::kQueryBytes;
+    float* const block_scales = reinterpret_cast<float*>(tiles + S::kSlots * S::kTileBytes + S::kStageBytes);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kSlots; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], 1); }
         for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 1); mbar_init(&p_half[x], kManyTile); mbar_init(&p_full[x], kManyTile); mbar_init(&o_full[x], 1); mbar_init(&q_full[x], kManyTile); }
         mbar_init(&drained, 1);
+        for (int i = 0; i < S::kScaleBlocks; ++i) mbar_init(&scales_full[i], 2);
         s_failed = 0;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -163,10 +192,14 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         const uint32_t scores = tmem + lanes + x * kScoreCols, probs = scores + kScoreCols / 2, outs = tmem + lanes + S::kOutCols + x * D;
         Cursor at = s_cursor;
         uint32_t s_par = 0, o_par = 0;
+        int block_count = 0, next_count = 0;                      // blocks of the run before this segment's; before the next one's
         bool more = true;                                         // `at` is a segment of this CTA's
         // the cursor at the next segment that has rows of this tile, from where it is
         auto settle = [&]() {
-            while (more && x == 1 && work.rows_of(at.seq) - at.tile * kManyRows <= kManyTile) more = at.next_segment(work);
+            while (more && x == 1 && work.rows_of(at.seq) - at.tile * kManyRows <= kManyTile) {
+                next_count += at.end - at.block;
+                more = at.next_segment(work);
+            }
         };
         // the warp's 32 rows of queries, neighbouring lanes a row; rows past the last are zeros
         auto ask_queries = [&]() {
@@ -181,7 +214,31 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 const T* src = static_cast<const T*>(a.q) + (live ? (at.seq.first_row + token) * a.q_stride +
                                                                        static_cast<int64_t>(at.head * work.group + head) * D + chunk * 8
                                                                   : 0);
-                copy16_fill(dst + many_at(kManyTile, q, chunk), src, live);
+                if constexpr (std::is_same_v<T, M>) {
+                    copy16_fill(dst + many_at(kManyTile, q, chunk), src, live);
+                } else {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (live) v = *reinterpret_cast<const uint4*>(src);
+                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    float top = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 f = KvType<T>::unpack(w[k]);
+                        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    }
+#pragma unroll
+                    for (int d = kChunks / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    const int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
+                    // |e| <= 133: in two factors, each a normal number
+                    const float f0 = ldexpf(1.0f, -e / 2), f1 = ldexpf(1.0f, -e - -e / 2);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 f = KvType<T>::unpack(w[k]);
+                        w[k] = KvType<M>::pack(f.x * f0 * f1, f.y * f0 * f1);
+                    }
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + many_at(kManyTile, q, chunk)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                    if (chunk == 0) s_q_scale[x * kManyTile + q] = ldexpf(a.scale_log2e, e);
+                }
                 q += kStep;
                 row += kStep;
                 head += kStep;
@@ -201,20 +258,30 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         }
         while (more) {
             {
+                block_count = next_count;
                 const Cursor here = at;
                 const int row = here.tile * kManyRows + x * kManyTile + r, n = here.end - here.block;
                 const int position = row < work.rows_of(here.seq) ? here.seq.first_pos + row / work.group : -1;
                 const int end = min(position + 1, work.capacity), start = a.window > 0 ? position + 1 - a.window : 0;
-                float m = -INFINITY, l = 0.0f;
+                float m = -INFINITY, l = 0.0f, row_scale = a.scale_log2e;
+                if constexpr (!std::is_same_v<T, M>) {
+                    __syncwarp();
+                    row_scale = s_q_scale[x * kManyTile + r];                  // the warp's own lanes wrote it
+                    __syncwarp();
+                }
 #pragma unroll 1
                 for (int j = 0; j < n; ++j) {
                     const int first = here.seg.low + (here.block + j) * kManyKeys;
                     const int e = end - first, b = start - first;              // visible: columns b .. e - 1
                     qmm_wait(&s_full[x], s_par, &s_failed);
                     s_par ^= 1u;
+                    const int kept = (block_count + j) % S::kScaleBlocks;      // the block's scales
+                    const float* const key_scales = block_scales + kept * 2 * kManyKeys;
+                    if constexpr (BITS != 16) qmm_wait(&scales_full[kept], ((block_count + j) / S::kScaleBlocks) & 1, &s_failed);
                     __syncwarp();
                     fence_after();
                     if (j + 1 == n) {                             // the products that read the queries are done: the next segment's may come
+                        next_count = block_count + n;
                         more = at.next_segment(work);
                         settle();
                         if (more) ask_queries();
@@ -227,6 +294,14 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                         tmem_ld32(scores + col, v0);
                         tmem_ld32(scores + col + 32, v1);
                         tmem_wait_ld();
+                        if constexpr (BITS != 16) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {
+                                const float4 k0 = *reinterpret_cast<const float4*>(key_scales + col + i), k1 = *reinterpret_cast<const float4*>(key_scales + col + 32 + i);
+                                scale4(&v0[i], k0);
+                                scale4(&v1[i], k1);
+                            }
+                        }
                         if (masked) {
                             auto seen = [&](int from) {           // bit i: column from + i is visible
                                 const int hi = min(max(e - from, 0), 32), lo = min(max(b - from, 0), 32);
@@ -252,7 +327,8 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                         }
                         top = fmaxf(top, fmaxf(t0, t1));
                     }
-                    top *= a.scale_log2e;
+                    top *= row_scale;
+                    if constexpr (BITS != 16) top += s_top[kept];
                     const bool moves = top > m + 8.0f;                           // also from -inf
                     if (__any_sync(0xffffffffu, moves)) {
                         const float to = moves ? top : m;
@@ -279,7 +355,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                         }
                     }
                     // the upper columns are in registers; their probabilities go where those scores lay, then the lower ones'
-                    const Pair scale2(a.scale_log2e, a.scale_log2e), shift2(m == -INFINITY ? 0.0f : -m, m == -INFINITY ? 0.0f : -m);
+                    const Pair scale2(row_scale, row_scale), shift2(m == -INFINITY ? 0.0f : -m, m == -INFINITY ? 0.0f : -m);
                     Pair l2(0.0f, 0.0f);
                     // every fourth pair of exponentials runs on the multiply-add pipe, which the other pipe would wait for
                     auto put = [&](auto mixed, const uint32_t (&v)[32], int col) {
@@ -296,7 +372,12 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                                 x1 = exp2_fast(x1);
                             }
                             l2 = add2(l2, Pair(x0, x1));
-                            w[i] = KvType<T>::pack(x0, x1);
+                            if constexpr (BITS != 16) {
+                                const float2 vs = *reinterpret_cast<const float2*>(key_scales + kManyKeys + col + 2 * i);
+                                x0 *= vs.x;
+                                x1 *= vs.y;
+                            }
+                            w[i] = KvType<M>::pack(x0, x1);
                         }
                         __syncwarp();
                         tmem_st16(probs + col / 2, w);
@@ -437,6 +518,83 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         bool more = w < 2 || at.step(work);
         for (int tile = w; more; tile += kLoadWarps) {
             const int slot = tile % S::kSlots, first = at.seg.low + at.block * kManyKeys;
+            if constexpr (BITS != 16) {
+                // every lane finds four keys; codes come 16 bytes a lane and leave as fp16
+                int64_t place[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = first + 32 * i + lane;
+                    place[i] = key >= at.seg.key0 && key < at.seg.key1 ? kv_place(p, at.b, key) : -1;
+                    if (place[i] >= 0) place[i] += static_cast<int64_t>(at.head) * p.page_size;
+                }
+                if (tile >= S::kSlots) {
+                    qmm_wait(&kv_free[slot], (tile / S::kSlots - 1) & 1u, &s_failed);
+                    __syncwarp();
+                }
+                const int kept = (tile >> 1) % S::kScaleBlocks;
+                float* const scales = block_scales + kept * 2 * kManyKeys + (w & 1) * kManyKeys;
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float f = place[i] >= 0 ? __ldg((w & 1 ? p.v_scale : p.k_scale) + place[i]) : 0.0f;
+                    scales[32 * i + lane] = f;
+                    top = fmaxf(top, f);
+                }
+                if (w & 1) {
+#pragma unroll
+                    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    // values below 2^-100 are as good as zero
+                    if (lane == 0) s_top[kept] = log2f(fmaxf(top, 7.8886091e-31f));
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&scales_full[kept]);
+                constexpr int kRowBytes = D * BITS / 8, kLanesPerRow = kRowBytes / 16, kAtOnce = 32 / kLanesPerRow, kTurns = kManyKeys / kAtOnce;
+                constexpr int kInFlight = 8;
+                const int piece = lane % kLanesPerRow, sub = lane / kLanesPerRow;
+                const char* const codes = static_cast<const char*>(w & 1 ? p.v : p.k) + piece * 16;
+                const uint32_t dst = tile_base + slot * S::kTileBytes;
+#pragma unroll 1
+                for (int t0 = 0; t0 < kTurns; t0 += kInFlight) {
+                    uint4 v[kInFlight];
+#pragma unroll
+                    for (int u = 0; u < kInFlight; ++u) {
+                        const int row = (t0 + u) * kAtOnce + sub, of = row >> 5;
+                        const int64_t own = of == 0 ? place[0] : of == 1 ? place[1] : of == 2 ? place[2] : place[3];
+                        const int64_t from = __shfl_sync(0xffffffffu, own, row & 31);
+                        v[u] = make_uint4(0, 0, 0, 0);
+                        if (from >= 0) v[u] = __ldg(reinterpret_cast<const uint4*>(codes + from * kRowBytes));
+                    }
+#pragma unroll
+                    for (int u = 0; u < kInFlight; ++u) {
+                        const int row = (t0 + u) * kAtOnce + sub;
+                        const uint32_t words[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+                        constexpr int kOut = BITS == 8 ? 2 : 4;              // 16-byte chunks of fp16
+                        uint32_t h[4 * kOut];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if constexpr (BITS == 8) {
+                                const uint32_t x = words[k] ^ 0x80808080u;
+                                h[2 * k] = codes8<0, 1>(x);
+                                h[2 * k + 1] = codes8<2, 3>(x);
+                            } else {
+                                uint32_t four[4];
+                                codes4_in_order(words[k], four);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) h[4 * k + i] = four[i];
+                            }
+                        }
+#pragma unroll
+                        for (int c = 0; c < kOut; ++c)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + many_at(kManyKeys, row, piece * kOut + c)), "r"(h[4 * c]),
+                                         "r"(h[4 * c + 1]), "r"(h[4 * c + 2]), "r"(h[4 * c + 3]) : "memory");
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&kv_full[slot]);
+                more = at.step(work) && at.step(work);
+                continue;
+            }
             // Lane i looks up the i-th part of the block: a tensor copy where every key of it is a token that some row of the sequence
             // sees (and so holds numbers), row by row with zeros where not.
             const int low = a.window > 0 ? max(0, at.seq.first_pos + 1 - a.window) : 0;
@@ -486,7 +644,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         }
     } else if (elect_one()) {
         // ================= products =================
-        constexpr uint32_t kFormat = std::is_same_v<T, __half> ? 0u : 1u;
+        constexpr uint32_t kFormat = std::is_same_v<M, __half> ? 0u : 1u;
         constexpr uint32_t kBase = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((128u >> 4) << 24);
         constexpr uint32_t kScoreDesc = kBase | ((static_cast<uint32_t>(kManyKeys) >> 3) << 17);
         constexpr uint32_t kValueDesc = kBase | (1u << 16) | ((static_cast<uint32_t>(D) >> 3) << 17);    // values: N is the contiguous axis
@@ -581,7 +739,7 @@ cudaError_t launch_many(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t 
     }
     CUtensorMap k_map{}, v_map{};
     int box_rows = 0;
-    if (!kv_tensor_maps(p, kManyKeys, &k_map, &v_map, &box_rows)) box_rows = 0;
+    if (BITS != 16 || !kv_tensor_maps(p, kManyKeys, &k_map, &v_map, &box_rows)) box_rows = 0;
     return launch_dependent(kv_many_kernel<T, BITS, D>, dim3(static_cast<unsigned>(sm_count())), dim3(kManyThreads), S::kSmem, stream, k_map, v_map, p, a,
                             box_rows);
 }
@@ -591,8 +749,16 @@ cudaError_t launch_many(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t 
 size_t kv_many_workspace_bytes(int head_dim) { return 2 * static_cast<size_t>(sm_count()) * kManyRows * (head_dim + 2) * sizeof(float); }
 
 cudaError_t launch_kv_many(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t stream) {
-    if (p.dtype == kF16) return p.head_dim == 128 ? launch_many<__half, 16, 128>(p, a, stream) : launch_many<__half, 16, 64>(p, a, stream);
-    return p.head_dim == 128 ? launch_many<__nv_bfloat16, 16, 128>(p, a, stream) : launch_many<__nv_bfloat16, 16, 64>(p, a, stream);
+#define B200_KV_CASE(T, BITS, D) \
+    if (p.bits == BITS && p.head_dim == D) return launch_many<T, BITS, D>(p, a, stream);
+#define B200_KV_CASES(T)                                                      \
+    B200_KV_CASE(T, 16, 128) B200_KV_CASE(T, 16, 64) B200_KV_CASE(T, 8, 128) \
+    B200_KV_CASE(T, 8, 64) B200_KV_CASE(T, 4, 128) B200_KV_CASE(T, 4, 64)
+    if (p.dtype == kF16) { B200_KV_CASES(__half) }
+    else { B200_KV_CASES(__nv_bfloat16) }
+#undef B200_KV_CASES
+#undef B200_KV_CASE
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace b200exl3

@@ -250,6 +250,19 @@ __device__ __forceinline__ void copy4_fill(uint32_t dst, const void* src, bool l
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// Two codes as fp16.  8 bits: bytes i and j of a word whose sign bits were flipped become 1024 + (code + 128); 4 bits: the low nibbles
+// of its halves become 1024 + (code + 8).
+__device__ __forceinline__ uint32_t less(uint32_t a, uint32_t bias) {
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+template <int I, int J> __device__ __forceinline__ uint32_t codes8(uint32_t w) { return less(prmt(w, 0x64646464u, 0x4040u | I | (J << 8)), 0x64806480u); }
+template <int I> __device__ __forceinline__ uint32_t codes4(uint32_t w) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(d) : "r"(w >> (4 * I)));    // (w & mask) | bias
+    return less(d, 0x64086408u);
+}
+
 // `rows` rows of the pool, 128 bytes of each at most (column c0 on), into shared memory by the tensor-copy unit
 __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int c0, int row, uint64_t* bar) {
     asm volatile(
