@@ -29,7 +29,13 @@ namespace {
 
 constexpr int kManyKeys = 128, kManyTile = 128, kManyRows = 2 * kManyTile;
 constexpr int kSoftmaxWarps = 8, kLoadWarps = 4;
-constexpr int kManyThreads = 32 * (kSoftmaxWarps + kLoadWarps + 1);
+constexpr int kManyThreads = 32 * (kSoftmaxWarps + kLoadWarps + 4);   // the last four: one issues the products
+// Registers of a thread, of the launch's 128: the row threads hold 64 scores and more, and what spills goes far (shared memory leaves no
+// first-level cache).  256 * 160 + 128 * 96 + 128 * 96 <= 512 * 128.
+constexpr int kSoftmaxRegisters = 160, kLoadRegisters = 96, kIssueRegisters = 96;
+static_assert(8 * kSoftmaxRegisters + 4 * kLoadRegisters + 4 * kIssueRegisters <= 16 * 128, "registers");
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int kManyTable = 512;
 constexpr int kManyOver = 3;
 constexpr uint32_t kScoreCols = 128;               // tensor-memory columns of S_x; P_x lies in their second half
@@ -140,6 +146,17 @@ __device__ __forceinline__ void codes4_in_order(uint32_t w, uint32_t (&v)[4]) {
     }
 }
 
+// Wait that gives up after about a quarter of a second of polls, or at once when another role has; inlined, since the register split
+// leaves no room for a call.
+__device__ __forceinline__ void many_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+    if (mbar_try_wait(bar, parity)) return;
+    const unsigned long long t0 = global_ns();
+    while (!mbar_try_wait_for(bar, parity, 20000)) {
+        if (*failed) return;
+        if (global_ns() - t0 > 250000000ull) *failed = 1;
+    }
+}
+
 // box_rows: rows of a tensor copy, a power of two that divides the page size, or 0: no tensor copies
 template <typename T, int BITS, int D>
 __global__ void __launch_bounds__(kManyThreads, 1)
@@ -155,7 +172,8 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ KvTable<kManyTable> s_table;
     __shared__ int64_t s_sum[kManyThreads / 32 + 1];
-    __shared__ Cursor s_cursor;
+    // every warp's place, and a row warp's segment at hand: in registers they would push out scores
+    __shared__ Cursor s_cursor, s_at[kSoftmaxWarps + kLoadWarps + 1], s_here[kSoftmaxWarps];
     __shared__ __align__(8) uint64_t kv_full[S::kSlots], kv_free[S::kSlots], s_full[2], p_half[2], p_full[2], o_full[2], q_full[2], drained, scales_full[S::kScaleBlocks];
     __shared__ float s_top[S::kScaleBlocks], s_q_scale[BITS != 16 && !std::is_same_v<T, __half> ? kManyRows : 1];
     __shared__ uint32_t tmem_base_slot;
@@ -184,13 +202,26 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_base_slot;
+    // a warp's cursor moved by all its lanes, to the same place
+    auto next_segment = [&](Cursor& c) {
+        Cursor next = c;
+        const bool ok = next.next_segment(work);
+        __syncwarp();
+        c = next;
+        __syncwarp();
+        return ok;
+    };
 
     if (warp < kSoftmaxWarps) {
         // ================= rows: one thread each =================
+        more_registers<kSoftmaxRegisters>();
         const int x = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t scores = tmem + lanes + x * kScoreCols, probs = scores + kScoreCols / 2, outs = tmem + lanes + S::kOutCols + x * D;
-        Cursor at = s_cursor;
+        Cursor& at = s_at[warp];
+        Cursor& here = s_here[warp];
+        at = s_cursor;
+        __syncwarp();
         uint32_t s_par = 0, o_par = 0;
         int block_count = 0, next_count = 0;                      // blocks of the run before this segment's; before the next one's
         bool more = true;                                         // `at` is a segment of this CTA's
@@ -198,7 +229,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         auto settle = [&]() {
             while (more && x == 1 && work.rows_of(at.seq) - at.tile * kManyRows <= kManyTile) {
                 next_count += at.end - at.block;
-                more = at.next_segment(work);
+                more = next_segment(at);
             }
         };
         // the warp's 32 rows of queries, neighbouring lanes a row; rows past the last are zeros
@@ -259,10 +290,13 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         while (more) {
             {
                 block_count = next_count;
-                const Cursor here = at;
+                here = at;
+                __syncwarp();
                 const int row = here.tile * kManyRows + x * kManyTile + r, n = here.end - here.block;
                 const int position = row < work.rows_of(here.seq) ? here.seq.first_pos + row / work.group : -1;
-                const int end = min(position + 1, work.capacity), start = a.window > 0 ? position + 1 - a.window : 0;
+                // visible keys from the first block's first one on
+                const int key0 = here.seg.low + here.block * kManyKeys;
+                const int end = min(position + 1, work.capacity) - key0, start = (a.window > 0 ? position + 1 - a.window : 0) - key0;
                 float m = -INFINITY, l = 0.0f, row_scale = a.scale_log2e;
                 if constexpr (!std::is_same_v<T, M>) {
                     __syncwarp();
@@ -271,18 +305,17 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 }
 #pragma unroll 1
                 for (int j = 0; j < n; ++j) {
-                    const int first = here.seg.low + (here.block + j) * kManyKeys;
-                    const int e = end - first, b = start - first;              // visible: columns b .. e - 1
-                    qmm_wait(&s_full[x], s_par, &s_failed);
+                    const int e = end - j * kManyKeys, b = start - j * kManyKeys;      // visible: columns b .. e - 1
+                    many_wait(&s_full[x], s_par, &s_failed);
                     s_par ^= 1u;
                     const int kept = (block_count + j) % S::kScaleBlocks;      // the block's scales
                     const float* const key_scales = block_scales + kept * 2 * kManyKeys;
-                    if constexpr (BITS != 16) qmm_wait(&scales_full[kept], ((block_count + j) / S::kScaleBlocks) & 1, &s_failed);
+                    if constexpr (BITS != 16) many_wait(&scales_full[kept], ((block_count + j) / S::kScaleBlocks) & 1, &s_failed);
                     __syncwarp();
                     fence_after();
                     if (j + 1 == n) {                             // the products that read the queries are done: the next segment's may come
                         next_count = block_count + n;
-                        more = at.next_segment(work);
+                        more = next_segment(at);
                         settle();
                         if (more) ask_queries();
                     }
@@ -401,7 +434,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 }
                 if (more) tell_queries();
                 // ---- the segment's rows, or this CTA's part of them
-                qmm_wait(&o_full[x], o_par, &s_failed);
+                many_wait(&o_full[x], o_par, &s_failed);
                 o_par ^= 1u;
                 __syncwarp();
                 fence_after();
@@ -508,16 +541,27 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         }
     } else if (warp < kSoftmaxWarps + kLoadWarps) {
         // ================= copies: every warp a tile of its own (even blocks' keys, their values, odd blocks' keys, their values) =================
+        fewer_registers<kLoadRegisters>();
         const int w = warp - kSoftmaxWarps, lane = threadIdx.x & 31;
         constexpr int kRowStep = 32 / kChunks;
         const int chunk = lane % kChunks, row0 = lane / kChunks;
         const int parts = box_rows > 0 ? kManyKeys / box_rows : 0;
         const uint32_t tile_base = smem_addr(tiles);
         const char* const pool = static_cast<const char*>(w & 1 ? p.v : p.k) + chunk * 16;
-        Cursor at = s_cursor;
-        bool more = w < 2 || at.step(work);
+        Cursor& at = s_at[warp];
+        at = s_cursor;
+        __syncwarp();
+        int block = at.block, block_end = at.end;                 // of the segment at hand
+        auto step = [&]() {
+            if (++block < block_end) return true;
+            if (!next_segment(at)) return false;
+            block = at.block;
+            block_end = at.end;
+            return true;
+        };
+        bool more = w < 2 || step();
         for (int tile = w; more; tile += kLoadWarps) {
-            const int slot = tile % S::kSlots, first = at.seg.low + at.block * kManyKeys;
+            const int slot = tile % S::kSlots, first = at.seg.low + block * kManyKeys;
             if constexpr (BITS != 16) {
                 // every lane finds four keys; codes come 16 bytes a lane and leave as fp16
                 int64_t place[4];
@@ -528,7 +572,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                     if (place[i] >= 0) place[i] += static_cast<int64_t>(at.head) * p.page_size;
                 }
                 if (tile >= S::kSlots) {
-                    qmm_wait(&kv_free[slot], (tile / S::kSlots - 1) & 1u, &s_failed);
+                    many_wait(&kv_free[slot], (tile / S::kSlots - 1) & 1u, &s_failed);
                     __syncwarp();
                 }
                 const int kept = (tile >> 1) % S::kScaleBlocks;
@@ -549,7 +593,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&scales_full[kept]);
                 constexpr int kRowBytes = D * BITS / 8, kLanesPerRow = kRowBytes / 16, kAtOnce = 32 / kLanesPerRow, kTurns = kManyKeys / kAtOnce;
-                constexpr int kInFlight = 8;
+                constexpr int kInFlight = kTurns < 16 ? kTurns : 16;
                 const int piece = lane % kLanesPerRow, sub = lane / kLanesPerRow;
                 const char* const codes = static_cast<const char*>(w & 1 ? p.v : p.k) + piece * 16;
                 const uint32_t dst = tile_base + slot * S::kTileBytes;
@@ -561,8 +605,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                         const int row = (t0 + u) * kAtOnce + sub, of = row >> 5;
                         const int64_t own = of == 0 ? place[0] : of == 1 ? place[1] : of == 2 ? place[2] : place[3];
                         const int64_t from = __shfl_sync(0xffffffffu, own, row & 31);
-                        v[u] = make_uint4(0, 0, 0, 0);
-                        if (from >= 0) v[u] = __ldg(reinterpret_cast<const uint4*>(codes + from * kRowBytes));
+                        v[u] = __ldg(reinterpret_cast<const uint4*>(codes + (from < 0 ? 0 : from * kRowBytes)));     // its scale is zero where there is none
                     }
 #pragma unroll
                     for (int u = 0; u < kInFlight; ++u) {
@@ -592,7 +635,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&kv_full[slot]);
-                more = at.step(work) && at.step(work);
+                more = step() && step();
                 continue;
             }
             // Lane i looks up the i-th part of the block: a tensor copy where every key of it is a token that some row of the sequence
@@ -606,7 +649,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             }
             const uint32_t whole = __ballot_sync(0xffffffffu, from >= 0);
             if (tile >= S::kSlots) {
-                qmm_wait(&kv_free[slot], (tile / S::kSlots - 1) & 1u, &s_failed);
+                many_wait(&kv_free[slot], (tile / S::kSlots - 1) & 1u, &s_failed);
                 __syncwarp();
             }
             const uint32_t dst = tile_base + slot * S::kTileBytes;
@@ -640,9 +683,11 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             // the copies' bytes may arrive before they are announced: the phase ends with this arrival at the earliest
             if (lane == 0) mbar_expect_tx(&kv_full[slot], static_cast<uint32_t>(__popc(whole) * box_rows * D * 2));
             __syncwarp();
-            more = at.step(work) && at.step(work);
+            more = step() && step();
         }
-    } else if (elect_one()) {
+    } else {
+        fewer_registers<kIssueRegisters>();
+        if (warp == kSoftmaxWarps + kLoadWarps && elect_one()) {
         // ================= products =================
         constexpr uint32_t kFormat = std::is_same_v<M, __half> ? 0u : 1u;
         constexpr uint32_t kBase = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((128u >> 4) << 24);
@@ -650,11 +695,12 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         constexpr uint32_t kValueDesc = kBase | (1u << 16) | ((static_cast<uint32_t>(D) >> 3) << 17);    // values: N is the contiguous axis
         const uint64_t q_desc = umma_desc(smem_addr(queries)), k_desc = umma_desc(smem_addr(tiles));
         const uint64_t v_desc = umma_desc_values(smem_addr(tiles), kManyKeys * 128);
-        Cursor at = s_cursor;
+        Cursor& at = s_at[warp];
+        at = s_cursor;
         int tile = 0;                                             // tiles consumed
         uint32_t p_par[2] = {0, 0}, q_par[2] = {0, 0};
         auto wait_tile = [&](int i) {
-            qmm_wait(&kv_full[i % S::kSlots], (i / S::kSlots) & 1u, &s_failed);
+            many_wait(&kv_full[i % S::kSlots], (i / S::kSlots) & 1u, &s_failed);
             fence_after();
         };
         auto score = [&](int x, int slot) {
@@ -671,7 +717,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             const uint64_t vd = v_desc + slot * (S::kTileBytes >> 4);
 #pragma unroll
             for (int h = 1; h >= 0; --h) {
-                qmm_wait(h ? &p_half[x] : &p_full[x], p_par[x], &s_failed);
+                many_wait(h ? &p_half[x] : &p_full[x], p_par[x], &s_failed);
                 fence_after();
 #pragma unroll
                 for (int k = h * (kManyKeys / 32); k < (h + 1) * (kManyKeys / 32); ++k)
@@ -685,7 +731,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             const bool two = rows - at.tile * kManyRows > kManyTile;
             wait_tile(tile);
             for (int x = 0; x < (two ? 2 : 1); ++x) {
-                qmm_wait(&q_full[x], q_par[x], &s_failed);
+                many_wait(&q_full[x], q_par[x], &s_failed);
                 q_par[x] ^= 1u;
                 fence_after();
                 score(x, tile % S::kSlots);
@@ -715,7 +761,8 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             }
         } while (at.next_segment(work));
         umma_commit(&drained);
-        qmm_wait(&drained, 0, &s_failed);
+        many_wait(&drained, 0, &s_failed);
+        }
     }
     __syncwarp();
     fence_before();
