@@ -29,13 +29,14 @@ namespace {
 
 constexpr int kManyKeys = 128, kManyTile = 128, kManyRows = 2 * kManyTile;
 constexpr int kSoftmaxWarps = 8, kLoadWarps = 4;
-constexpr int kManyThreads = 32 * (kSoftmaxWarps + kLoadWarps + 4);   // the last four: one issues the products
+constexpr int kManyThreads = 32 * (kSoftmaxWarps + kLoadWarps + 4);   // the last four: one issues the products, two bring queries
 // Registers of a thread, of the launch's 128: the row threads hold 64 scores and more, and what spills goes far (shared memory leaves no
 // first-level cache).  256 * 160 + 128 * 96 + 128 * 96 <= 512 * 128.
 constexpr int kSoftmaxRegisters = 160, kLoadRegisters = 96, kIssueRegisters = 96;
 static_assert(8 * kSoftmaxRegisters + 4 * kLoadRegisters + 4 * kIssueRegisters <= 16 * 128, "registers");
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+constexpr int kQueryWarp = kSoftmaxWarps + kLoadWarps + 1;         // and two bring the queries
 constexpr int kManyTable = 512;
 constexpr int kManyOver = 3;
 constexpr uint32_t kScoreCols = 128;               // tensor-memory columns of S_x; P_x lies in their second half
@@ -105,32 +106,12 @@ struct Pair {
 __device__ __forceinline__ Pair fma2(Pair a, const Pair& b, const Pair& c) { asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(a.v) : "l"(b.v), "l"(c.v)); return a; }
 __device__ __forceinline__ Pair add2(Pair a, const Pair& b) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v)); return a; }
 
-// 2^x of two numbers <= 2^7 on the multiply-add pipe: the nearest whole number goes into the exponent, the rest, |f| <= 1/2, through a
-// polynomial (least squares of the relative error, reweighted to equal ripples: 1.6e-7).  Below 2^-126 the result stays there.
-__device__ __forceinline__ void exp2_by_fma(Pair x, float& y0, float& y1) {
+__device__ __forceinline__ Pair mul2(Pair a, const Pair& b) { asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v)); return a; }
+__device__ __forceinline__ void scale2(uint32_t& v0, uint32_t& v1, float f0, float f1) {
     float x0, x1;
-    x.get(x0, x1);
-    x = Pair(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
-    const Pair magic(12582912.0f, 12582912.0f), unmagic(-12582912.0f, -12582912.0f), minus(-1.0f, -1.0f);
-    const Pair t = add2(x, magic), f = fma2(add2(t, unmagic), minus, x);
-    Pair y(0.00132764940f, 0.00132764940f);
-    y = fma2(y, f, Pair(0.00967553636f, 0.00967553636f));
-    y = fma2(y, f, Pair(0.0555071309f, 0.0555071309f));
-    y = fma2(y, f, Pair(0.240221202f, 0.240221202f));
-    y = fma2(y, f, Pair(0.693146944f, 0.693146944f));
-    y = fma2(y, f, Pair(1.00000012f, 1.00000012f));
-    float t0, t1;
-    t.get(t0, t1);
-    y.get(y0, y1);
-    y0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
-    y1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
-}
-
-__device__ __forceinline__ void scale4(uint32_t* v, const float4& f) {
-    v[0] = __float_as_uint(__uint_as_float(v[0]) * f.x);
-    v[1] = __float_as_uint(__uint_as_float(v[1]) * f.y);
-    v[2] = __float_as_uint(__uint_as_float(v[2]) * f.z);
-    v[3] = __float_as_uint(__uint_as_float(v[3]) * f.w);
+    mul2(Pair(__uint_as_float(v0), __uint_as_float(v1)), Pair(f0, f1)).get(x0, x1);
+    v0 = __float_as_uint(x0);
+    v1 = __float_as_uint(x1);
 }
 
 // Eight 4-bit codes of a word as fp16 in order: the two of a byte go to the halves of a word, as 1024 + u and 1024 + 16 u
@@ -173,9 +154,9 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     __shared__ KvTable<kManyTable> s_table;
     __shared__ int64_t s_sum[kManyThreads / 32 + 1];
     // every warp's place, and a row warp's segment at hand: in registers they would push out scores
-    __shared__ Cursor s_cursor, s_at[kSoftmaxWarps + kLoadWarps + 1], s_here[kSoftmaxWarps];
-    __shared__ __align__(8) uint64_t kv_full[S::kSlots], kv_free[S::kSlots], s_full[2], p_half[2], p_full[2], o_full[2], q_full[2], drained, scales_full[S::kScaleBlocks];
-    __shared__ float s_top[S::kScaleBlocks], s_q_scale[BITS != 16 && !std::is_same_v<T, __half> ? kManyRows : 1];
+    __shared__ Cursor s_cursor, s_at[kSoftmaxWarps + kLoadWarps + 3], s_here[kSoftmaxWarps];
+    __shared__ __align__(8) uint64_t kv_full[S::kSlots], kv_free[S::kSlots], s_full[2], p_half[2], p_full[2], o_full[2], q_full[2], q_free[2], drained, scales_full[S::kScaleBlocks];
+    __shared__ float s_top[S::kScaleBlocks], s_q_scale[2][BITS != 16 && !std::is_same_v<T, __half> ? kManyRows : 1];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int s_last[2];
     __shared__ volatile int s_failed;
@@ -190,7 +171,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kSlots; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], 1); }
-        for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 1); mbar_init(&p_half[x], kManyTile); mbar_init(&p_full[x], kManyTile); mbar_init(&o_full[x], 1); mbar_init(&q_full[x], kManyTile); }
+        for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 2); mbar_init(&p_half[x], kManyTile); mbar_init(&p_full[x], kManyTile); mbar_init(&o_full[x], 1); mbar_init(&q_full[x], 1); mbar_init(&q_free[x], 1); }
         mbar_init(&drained, 1);
         for (int i = 0; i < S::kScaleBlocks; ++i) mbar_init(&scales_full[i], 2);
         s_failed = 0;
@@ -223,6 +204,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         at = s_cursor;
         __syncwarp();
         uint32_t s_par = 0, o_par = 0;
+        int segment_count = 0;                                    // segments of this tile before
         int block_count = 0, next_count = 0;                      // blocks of the run before this segment's; before the next one's
         bool more = true;                                         // `at` is a segment of this CTA's
         // the cursor at the next segment that has rows of this tile, from where it is
@@ -232,61 +214,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 more = next_segment(at);
             }
         };
-        // the warp's 32 rows of queries, neighbouring lanes a row; rows past the last are zeros
-        auto ask_queries = [&]() {
-            constexpr int kStep = 32 / kChunks;
-            const int lane = threadIdx.x & 31, chunk = lane % kChunks, rows = work.rows_of(at.seq);
-            int q = (warp & 3) * 32 + lane / kChunks;
-            int row = at.tile * kManyRows + x * kManyTile + q, token = row / work.group, head = row - token * work.group;
-            const uint32_t dst = smem_addr(queries) + x * (S::kQueryBytes / 2);
-#pragma unroll 1
-            for (int i = 0; i < 32 / kStep; ++i) {
-                const bool live = row < rows;
-                const T* src = static_cast<const T*>(a.q) + (live ? (at.seq.first_row + token) * a.q_stride +
-                                                                       static_cast<int64_t>(at.head * work.group + head) * D + chunk * 8
-                                                                  : 0);
-                if constexpr (std::is_same_v<T, M>) {
-                    copy16_fill(dst + many_at(kManyTile, q, chunk), src, live);
-                } else {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (live) v = *reinterpret_cast<const uint4*>(src);
-                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                    float top = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float2 f = KvType<T>::unpack(w[k]);
-                        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-                    }
-#pragma unroll
-                    for (int d = kChunks / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    const int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
-                    // |e| <= 133: in two factors, each a normal number
-                    const float f0 = ldexpf(1.0f, -e / 2), f1 = ldexpf(1.0f, -e - -e / 2);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float2 f = KvType<T>::unpack(w[k]);
-                        w[k] = KvType<M>::pack(f.x * f0 * f1, f.y * f0 * f1);
-                    }
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + many_at(kManyTile, q, chunk)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-                    if (chunk == 0) s_q_scale[x * kManyTile + q] = ldexpf(a.scale_log2e, e);
-                }
-                q += kStep;
-                row += kStep;
-                head += kStep;
-                while (head >= work.group) { head -= work.group; ++token; }
-            }
-            copy_commit();
-        };
-        auto tell_queries = [&]() {
-            copy_wait<0>();
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&q_full[x]);
-        };
         settle();
-        if (more) {
-            ask_queries();
-            tell_queries();
-        }
         while (more) {
             {
                 block_count = next_count;
@@ -298,11 +226,6 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 const int key0 = here.seg.low + here.block * kManyKeys;
                 const int end = min(position + 1, work.capacity) - key0, start = (a.window > 0 ? position + 1 - a.window : 0) - key0;
                 float m = -INFINITY, l = 0.0f, row_scale = a.scale_log2e;
-                if constexpr (!std::is_same_v<T, M>) {
-                    __syncwarp();
-                    row_scale = s_q_scale[x * kManyTile + r];                  // the warp's own lanes wrote it
-                    __syncwarp();
-                }
 #pragma unroll 1
                 for (int j = 0; j < n; ++j) {
                     const int e = end - j * kManyKeys, b = start - j * kManyKeys;      // visible: columns b .. e - 1
@@ -310,58 +233,65 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                     s_par ^= 1u;
                     const int kept = (block_count + j) % S::kScaleBlocks;      // the block's scales
                     const float* const key_scales = block_scales + kept * 2 * kManyKeys;
+                    // written with the queries; two segments' worth, so that the next one's do not overtake a row
+                    if (!std::is_same_v<T, M> && j == 0) row_scale = s_q_scale[segment_count & 1][x * kManyTile + r];
                     if constexpr (BITS != 16) many_wait(&scales_full[kept], ((block_count + j) / S::kScaleBlocks) & 1, &s_failed);
                     __syncwarp();
                     fence_after();
-                    if (j + 1 == n) {                             // the products that read the queries are done: the next segment's may come
+                    if (j + 1 == n) {
                         next_count = block_count + n;
                         more = next_segment(at);
                         settle();
-                        if (more) ask_queries();
                     }
-                    // columns of a pair of loads that the row does not see
-                    const bool masked = __any_sync(0xffffffffu, e < kManyKeys || b > 0);
-                    uint32_t v0[32], v1[32];
-                    auto load = [&](int col) {
+                    // the block in two forms, with and without hidden columns: a test between loads and arithmetic costs a sixth of the time
+                    auto block = [&](auto with_hidden) {
+                    constexpr bool kMasked = decltype(with_hidden)::value;
+                    // 64 scores at a time, 32 where scales come on top: longer loops miss the instruction cache
+                    constexpr int kWide = BITS == 16 ? 2 : 1, kCols = 32 * kWide;
+                    uint32_t v_wide[kWide][32];
+                    auto load = [&](int col0) {
                         __syncwarp();
-                        tmem_ld32(scores + col, v0);
-                        tmem_ld32(scores + col + 32, v1);
+#pragma unroll
+                        for (int h = 0; h < kWide; ++h) tmem_ld32(scores + col0 + 32 * h, v_wide[h]);
                         tmem_wait_ld();
+#pragma unroll
+                        for (int h = 0; h < kWide; ++h) {
+                        uint32_t (&v)[32] = v_wide[h];
+                        const int col = col0 + 32 * h;
                         if constexpr (BITS != 16) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 4) {
-                                const float4 k0 = *reinterpret_cast<const float4*>(key_scales + col + i), k1 = *reinterpret_cast<const float4*>(key_scales + col + 32 + i);
-                                scale4(&v0[i], k0);
-                                scale4(&v1[i], k1);
+                                const float4 k = *reinterpret_cast<const float4*>(key_scales + col + i);
+                                scale2(v[i], v[i + 1], k.x, k.y);
+                                scale2(v[i + 2], v[i + 3], k.z, k.w);
                             }
                         }
-                        if (masked) {
-                            auto seen = [&](int from) {           // bit i: column from + i is visible
-                                const int hi = min(max(e - from, 0), 32), lo = min(max(b - from, 0), 32);
-                                return (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & (lo == 32 ? 0u : 0xffffffffu << lo);
-                            };
-                            const uint32_t m0 = seen(col), m1 = seen(col + 32);
+                        if constexpr (kMasked) {
+                            const int hi = min(max(e - col, 0), 32), lo = min(max(b - col, 0), 32);
+                            // bit i: column col + i is visible
+                            const uint32_t seen = (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & (lo == 32 ? 0u : 0xffffffffu << lo);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                v0[i] = m0 & (1u << i) ? v0[i] : 0xff800000u;
-                                v1[i] = m1 & (1u << i) ? v1[i] : 0xff800000u;
-                            }
+                            for (int i = 0; i < 32; ++i) v[i] = seen & (1u << i) ? v[i] : 0xff800000u;
+                        }
                         }
                     };
                     float top = -INFINITY;
 #pragma unroll 1
-                    for (int col = 0; col < kManyKeys; col += 64) {
+                    for (int col = 0; col < kManyKeys; col += kCols) {
                         load(col);
                         float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            t0 = fmaxf(t0, fmaxf(__uint_as_float(v0[i]), __uint_as_float(v0[i + 1])));
-                            t1 = fmaxf(t1, fmaxf(__uint_as_float(v1[i]), __uint_as_float(v1[i + 1])));
-                        }
+                        for (int h = 0; h < kWide; ++h)
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {
+                                t0 = fmaxf(t0, fmaxf(__uint_as_float(v_wide[h][i]), __uint_as_float(v_wide[h][i + 1])));
+                                t1 = fmaxf(t1, fmaxf(__uint_as_float(v_wide[h][i + 2]), __uint_as_float(v_wide[h][i + 3])));
+                            }
                         top = fmaxf(top, fmaxf(t0, t1));
                     }
                     top *= row_scale;
                     if constexpr (BITS != 16) top += s_top[kept];
+                    bool reload = false;
                     const bool moves = top > m + 8.0f;                           // also from -inf
                     if (__any_sync(0xffffffffu, moves)) {
                         const float to = moves ? top : m;
@@ -369,6 +299,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                         m = to;
                         l *= factor;
                         if (j > 0) {
+                            reload = true;                            // the outputs' way through the registers
 #pragma unroll 1
                             for (int c = 0; c < D; c += 32) {
                                 __syncwarp();
@@ -384,60 +315,50 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                                 tmem_st16(outs + c, o0);
                                 tmem_st16(outs + c + 16, o1);
                             }
-                            load(kManyKeys - 64);
                         }
                     }
-                    // the upper columns are in registers; their probabilities go where those scores lay, then the lower ones'
-                    const Pair scale2(row_scale, row_scale), shift2(m == -INFINITY ? 0.0f : -m, m == -INFINITY ? 0.0f : -m);
-                    Pair l2(0.0f, 0.0f);
-                    // every fourth pair of exponentials runs on the multiply-add pipe, which the other pipe would wait for
-                    auto put = [&](auto mixed, const uint32_t (&v)[32], int col) {
-                        uint32_t w[16];
+                    // from the upper columns down: probabilities go where scores lay that were read before
+                    const Pair scales2(row_scale, row_scale), shift2(m == -INFINITY ? 0.0f : -m, m == -INFINITY ? 0.0f : -m);
+                    Pair l2(0.0f, 0.0f), l3(0.0f, 0.0f);
+#pragma unroll 1
+                    for (int col = kManyKeys - kCols; col >= 0; col -= kCols) {
+                        if (kWide == 1 || col + kCols < kManyKeys || reload) load(col);       // 64 at a time: the upper ones are still here
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            float x0, x1;
-                            const Pair x = fma2(Pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, shift2);
-                            if (decltype(mixed)::value && i % 4 == 3) {
-                                exp2_by_fma(x, x0, x1);
-                            } else {
-                                x.get(x0, x1);
+                        for (int h = kWide - 1; h >= 0; --h) {
+                            const uint32_t (&v)[32] = v_wide[h];
+                            uint32_t p2[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                float x0, x1;
+                                fma2(Pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scales2, shift2).get(x0, x1);
                                 x0 = exp2_fast(x0);
                                 x1 = exp2_fast(x1);
+                                if (i & 1) l3 = add2(l3, Pair(x0, x1)); else l2 = add2(l2, Pair(x0, x1));
+                                if constexpr (BITS != 16) {
+                                    const float2 vs = *reinterpret_cast<const float2*>(key_scales + kManyKeys + col + 32 * h + 2 * i);
+                                    x0 *= vs.x;
+                                    x1 *= vs.y;
+                                }
+                                p2[i] = KvType<M>::pack(x0, x1);
                             }
-                            l2 = add2(l2, Pair(x0, x1));
-                            if constexpr (BITS != 16) {
-                                const float2 vs = *reinterpret_cast<const float2*>(key_scales + kManyKeys + col + 2 * i);
-                                x0 *= vs.x;
-                                x1 *= vs.y;
-                            }
-                            w[i] = KvType<M>::pack(x0, x1);
+                            __syncwarp();
+                            tmem_st16(probs + (col + 32 * h) / 2, p2);
                         }
-                        __syncwarp();
-                        tmem_st16(probs + col / 2, w);
-                    };
-                    auto put_all = [&](auto mixed) {
-#pragma unroll 1
-                        for (int col = kManyKeys - 64;; col -= 64) {
-                            put(mixed, v1, col + 32);
-                            put(mixed, v0, col);
+                        if ((col & 32) == 0) {                        // a half is there
                             tmem_wait_st();
                             fence_before();
                             mbar_arrive(col == 0 ? &p_full[x] : &p_half[x]);
-                            if (col == 0) break;
-                            load(col - 64);
                         }
-                    };
-                    if (masked) put_all(std::false_type{}); else put_all(std::true_type{});
+                    }
+                    l2 = add2(l2, l3);
                     float l0, l1;
                     l2.get(l0, l1);
                     l += l0 + l1;
+                    };
+                    if (__any_sync(0xffffffffu, e < kManyKeys || b > 0)) block(std::true_type{}); else block(std::false_type{});
                 }
-                if (more) tell_queries();
                 // ---- the segment's rows, or this CTA's part of them
-                many_wait(&o_full[x], o_par, &s_failed);
-                o_par ^= 1u;
-                __syncwarp();
-                fence_after();
+                ++segment_count;
                 const int64_t first_unit = here.base + kManyOver;
                 const int c0 = run.cta_of(first_unit), c1 = run.cta_of(first_unit + here.seg.blocks - 1);
                 auto part_of = [&](int c) { return a.parts + (2 * c + (c == c0 ? 1 : 0)) * static_cast<int64_t>(S::kPartFloats); };
@@ -472,6 +393,10 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 };
                 const float inverse = kv_inverse(l);
                 float4* const mine = whole ? nullptr : reinterpret_cast<float4*>(part_of(blockIdx.x)) + pr;      // [four results][row]
+                many_wait(&o_full[x], o_par, &s_failed);
+                o_par ^= 1u;
+                __syncwarp();
+                fence_after();
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     uint32_t v[32];
@@ -593,24 +518,30 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&scales_full[kept]);
                 constexpr int kRowBytes = D * BITS / 8, kLanesPerRow = kRowBytes / 16, kAtOnce = 32 / kLanesPerRow, kTurns = kManyKeys / kAtOnce;
-                constexpr int kInFlight = kTurns < 16 ? kTurns : 16;
+                constexpr int kBatch = 4, kBatches = kTurns / kBatch;          // two batches of loads are ahead of the one that is turned
+                static_assert(kTurns % kBatch == 0 && kBatches >= 2, "batches");
                 const int piece = lane % kLanesPerRow, sub = lane / kLanesPerRow;
                 const char* const codes = static_cast<const char*>(w & 1 ? p.v : p.k) + piece * 16;
                 const uint32_t dst = tile_base + slot * S::kTileBytes;
-#pragma unroll 1
-                for (int t0 = 0; t0 < kTurns; t0 += kInFlight) {
-                    uint4 v[kInFlight];
+                auto ask = [&](uint4 (&v)[kBatch], int batch) {
 #pragma unroll
-                    for (int u = 0; u < kInFlight; ++u) {
-                        const int row = (t0 + u) * kAtOnce + sub, of = row >> 5;
+                    for (int u = 0; u < kBatch; ++u) {
+                        const int row = (batch * kBatch + u) * kAtOnce + sub, of = row >> 5;
                         const int64_t own = of == 0 ? place[0] : of == 1 ? place[1] : of == 2 ? place[2] : place[3];
                         const int64_t from = __shfl_sync(0xffffffffu, own, row & 31);
                         v[u] = __ldg(reinterpret_cast<const uint4*>(codes + (from < 0 ? 0 : from * kRowBytes)));     // its scale is zero where there is none
                     }
+                };
+                uint4 v0[kBatch], v1[kBatch], v2[kBatch];
+                ask(v0, 0);
+                ask(v1, 1);
+#pragma unroll 1
+                for (int batch = 0; batch < kBatches; ++batch) {
+                    if (batch + 2 < kBatches) ask(v2, batch + 2);
 #pragma unroll
-                    for (int u = 0; u < kInFlight; ++u) {
-                        const int row = (t0 + u) * kAtOnce + sub;
-                        const uint32_t words[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+                    for (int u = 0; u < kBatch; ++u) {
+                        const int row = (batch * kBatch + u) * kAtOnce + sub;
+                        const uint32_t words[4] = {v0[u].x, v0[u].y, v0[u].z, v0[u].w};
                         constexpr int kOut = BITS == 8 ? 2 : 4;              // 16-byte chunks of fp16
                         uint32_t h[4 * kOut];
 #pragma unroll
@@ -631,6 +562,8 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + many_at(kManyKeys, row, piece * kOut + c)), "r"(h[4 * c]),
                                          "r"(h[4 * c + 1]), "r"(h[4 * c + 2]), "r"(h[4 * c + 3]) : "memory");
                     }
+#pragma unroll
+                    for (int u = 0; u < kBatch; ++u) { v0[u] = v1[u]; v1[u] = v2[u]; }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -711,6 +644,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 umma_f16_ss(tmem + x * kScoreCols, qd + off, kd + off, kScoreDesc, k > 0);
             }
             umma_commit(&s_full[x]);
+            mbar_arrive(&s_full[x]);                              // and passes on what this thread has waited for: the rows' scales beside their queries
         };
         auto weigh = [&](int x, int slot, bool accumulate) {
             // the probabilities of the upper keys come first
@@ -735,6 +669,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 q_par[x] ^= 1u;
                 fence_after();
                 score(x, tile % S::kSlots);
+                if (n == 1) umma_commit(&q_free[x]);
             }
             umma_commit(&kv_free[tile % S::kSlots]);
             for (int j = 0; j < n; ++j) {
@@ -745,14 +680,19 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 if (more) {
                     wait_tile(kt);
                     score(0, kt % S::kSlots);
+                    if (j + 2 == n) umma_commit(&q_free[0]);
                 } else {
                     umma_commit(&o_full[0]);
                 }
                 if (two) {
                     weigh(1, vt % S::kSlots, j > 0);
                     umma_commit(&kv_free[vt % S::kSlots]);
-                    if (more) score(1, kt % S::kSlots);
-                    else umma_commit(&o_full[1]);
+                    if (more) {
+                        score(1, kt % S::kSlots);
+                        if (j + 2 == n) umma_commit(&q_free[1]);
+                    } else {
+                        umma_commit(&o_full[1]);
+                    }
                 } else {
                     umma_commit(&kv_free[vt % S::kSlots]);
                 }
@@ -762,6 +702,66 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         } while (at.next_segment(work));
         umma_commit(&drained);
         many_wait(&drained, 0, &s_failed);
+        } else if (warp == kQueryWarp || warp == kQueryWarp + 1) {
+            // ================= queries of a tile: neighbouring lanes a row; rows past the last are zeros =================
+            const int x = warp - kQueryWarp, lane = threadIdx.x & 31, chunk = lane % kChunks;
+            constexpr int kStep = 32 / kChunks;
+            const uint32_t dst = smem_addr(queries) + x * (S::kQueryBytes / 2);
+            Cursor& at = s_at[warp];
+            at = s_cursor;
+            __syncwarp();
+            int loaded = 0;
+            do {
+                const int rows = work.rows_of(at.seq);
+                if (x == 1 && rows - at.tile * kManyRows <= kManyTile) continue;
+                const int row0 = at.tile * kManyRows + x * kManyTile, token0 = row0 / work.group, past = row0 - token0 * work.group;
+                const float per_token = 1.0f / static_cast<float>(work.group);
+                const T* const base = static_cast<const T*>(a.q) + (at.seq.first_row + token0) * a.q_stride +
+                                      static_cast<int64_t>(at.head * work.group) * D + chunk * 8;
+                // the products of this tile's segment before have read their queries
+                if (loaded > 0) many_wait(&q_free[x], (loaded - 1) & 1, &s_failed);
+                __syncwarp();
+#pragma unroll 8
+                for (int i = 0; i < kManyTile / kStep; ++i) {
+                    const int q = i * kStep + lane / kChunks;
+                    const bool live = row0 + q < rows;
+                    // (past + q) / group: half a row away from where fp32 could round it over an edge
+                    const int token = __float2int_rz((static_cast<float>(past + q) + 0.5f) * per_token);
+                    const T* src = base + (live ? token * a.q_stride + (past + q - token * work.group) * D : 0);
+                    if (!live) src = static_cast<const T*>(a.q);
+                    if constexpr (std::is_same_v<T, M>) {
+                        copy16_fill(dst + many_at(kManyTile, q, chunk), src, live);
+                    } else {
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (live) v = *reinterpret_cast<const uint4*>(src);
+                        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                        float top = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float2 f = KvType<T>::unpack(w[k]);
+                            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                        }
+#pragma unroll
+                        for (int d = kChunks / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
+                        // |e| <= 133: in two factors, each a normal number
+                        const float f0 = ldexpf(1.0f, -e / 2), f1 = ldexpf(1.0f, -e - -e / 2);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float2 f = KvType<T>::unpack(w[k]);
+                            w[k] = KvType<M>::pack(f.x * f0 * f1, f.y * f0 * f1);
+                        }
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + many_at(kManyTile, q, chunk)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                        if (chunk == 0) s_q_scale[loaded & 1][x * kManyTile + q] = ldexpf(a.scale_log2e, e);
+                    }
+                }
+                copy_commit();
+                copy_wait<0>();
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[x]);
+                ++loaded;
+            } while (next_segment(at));
         }
     }
     __syncwarp();
