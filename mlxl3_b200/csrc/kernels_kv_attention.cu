@@ -69,15 +69,6 @@ __device__ __forceinline__ void mma_rows(float (&d)[4], const uint32_t (&a)[4], 
     }
 }
 
-// Where a 16-byte chunk of a tile's row lies, as the tensor copies put it: pieces of up to 128 bytes of all rows, one after the other; in
-// a piece rows of 128 bytes swap their chunks by the row's number, shorter ones by the number of the 128 bytes they are in, so that eight
-// rows' same chunk uses all banks.
-template <int CHUNKS, int KEYS>
-__device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
-    constexpr int kPiece = CHUNKS >= 8 ? 8 : CHUNKS, kShift = CHUNKS >= 8 ? 0 : (CHUNKS == 4 ? 1 : 2);
-    return static_cast<uint32_t>((chunk / kPiece * KEYS + row) * kPiece + ((chunk % kPiece) ^ ((row >> kShift) & (kPiece - 1)))) * 16;
-}
-
 // The same for chunk c + of, c even and of 0 or 1, from the place of chunk `of`: the swizzle is an exclusive or.
 template <int CHUNKS, int KEYS>
 __device__ __forceinline__ uint32_t tile_next(uint32_t at, int c) {

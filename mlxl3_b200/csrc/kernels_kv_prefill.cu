@@ -155,7 +155,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     __shared__ int64_t s_sum[kManyThreads / 32 + 1];
     // every warp's place, and a row warp's segment at hand: in registers they would push out scores
     __shared__ Cursor s_cursor, s_at[kSoftmaxWarps + kLoadWarps + 3], s_here[kSoftmaxWarps];
-    __shared__ __align__(8) uint64_t kv_full[S::kSlots], kv_free[S::kSlots], s_full[2], p_half[2], p_full[2], o_full[2], q_full[2], q_free[2], drained, scales_full[S::kScaleBlocks];
+    __shared__ __align__(8) uint64_t kv_full[S::kSlots], kv_free[S::kSlots], s_full[2], p_half[2], p_full[2], o_full[2], q_full[2], q_free[2], drained, scales_full[S::kScaleBlocks], raw_full[S::kSlots];
     __shared__ float s_top[S::kScaleBlocks], s_q_scale[2][BITS != 16 && !std::is_same_v<T, __half> ? kManyRows : 1];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int s_last[2];
@@ -170,7 +170,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     float* const block_scales = reinterpret_cast<float*>(tiles + S::kSlots * S::kTileBytes + S::kStageBytes);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kSlots; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], 1); }
+        for (int s = 0; s < S::kSlots; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], 1); mbar_init(&raw_full[s], 1); }
         for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 2); mbar_init(&p_half[x], kManyTile); mbar_init(&p_full[x], kManyTile); mbar_init(&o_full[x], 1); mbar_init(&q_full[x], 1); mbar_init(&q_free[x], 1); }
         mbar_init(&drained, 1);
         for (int i = 0; i < S::kScaleBlocks; ++i) mbar_init(&scales_full[i], 2);
@@ -487,90 +487,6 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         bool more = w < 2 || step();
         for (int tile = w; more; tile += kLoadWarps) {
             const int slot = tile % S::kSlots, first = at.seg.low + block * kManyKeys;
-            if constexpr (BITS != 16) {
-                // every lane finds four keys; codes come 16 bytes a lane and leave as fp16
-                int64_t place[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = first + 32 * i + lane;
-                    place[i] = key >= at.seg.key0 && key < at.seg.key1 ? kv_place(p, at.b, key) : -1;
-                    if (place[i] >= 0) place[i] += static_cast<int64_t>(at.head) * p.page_size;
-                }
-                if (tile >= S::kSlots) {
-                    many_wait(&kv_free[slot], (tile / S::kSlots - 1) & 1u, &s_failed);
-                    __syncwarp();
-                }
-                const int kept = (tile >> 1) % S::kScaleBlocks;
-                float* const scales = block_scales + kept * 2 * kManyKeys + (w & 1) * kManyKeys;
-                float top = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float f = place[i] >= 0 ? __ldg((w & 1 ? p.v_scale : p.k_scale) + place[i]) : 0.0f;
-                    scales[32 * i + lane] = f;
-                    top = fmaxf(top, f);
-                }
-                if (w & 1) {
-#pragma unroll
-                    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    // values below 2^-100 are as good as zero
-                    if (lane == 0) s_top[kept] = log2f(fmaxf(top, 7.8886091e-31f));
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&scales_full[kept]);
-                constexpr int kRowBytes = D * BITS / 8, kLanesPerRow = kRowBytes / 16, kAtOnce = 32 / kLanesPerRow, kTurns = kManyKeys / kAtOnce;
-                constexpr int kBatch = 4, kBatches = kTurns / kBatch;          // two batches of loads are ahead of the one that is turned
-                static_assert(kTurns % kBatch == 0 && kBatches >= 2, "batches");
-                const int piece = lane % kLanesPerRow, sub = lane / kLanesPerRow;
-                const char* const codes = static_cast<const char*>(w & 1 ? p.v : p.k) + piece * 16;
-                const uint32_t dst = tile_base + slot * S::kTileBytes;
-                auto ask = [&](uint4 (&v)[kBatch], int batch) {
-#pragma unroll
-                    for (int u = 0; u < kBatch; ++u) {
-                        const int row = (batch * kBatch + u) * kAtOnce + sub, of = row >> 5;
-                        const int64_t own = of == 0 ? place[0] : of == 1 ? place[1] : of == 2 ? place[2] : place[3];
-                        const int64_t from = __shfl_sync(0xffffffffu, own, row & 31);
-                        v[u] = __ldg(reinterpret_cast<const uint4*>(codes + (from < 0 ? 0 : from * kRowBytes)));     // its scale is zero where there is none
-                    }
-                };
-                uint4 v0[kBatch], v1[kBatch], v2[kBatch];
-                ask(v0, 0);
-                ask(v1, 1);
-#pragma unroll 1
-                for (int batch = 0; batch < kBatches; ++batch) {
-                    if (batch + 2 < kBatches) ask(v2, batch + 2);
-#pragma unroll
-                    for (int u = 0; u < kBatch; ++u) {
-                        const int row = (batch * kBatch + u) * kAtOnce + sub;
-                        const uint32_t words[4] = {v0[u].x, v0[u].y, v0[u].z, v0[u].w};
-                        constexpr int kOut = BITS == 8 ? 2 : 4;              // 16-byte chunks of fp16
-                        uint32_t h[4 * kOut];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if constexpr (BITS == 8) {
-                                const uint32_t x = words[k] ^ 0x80808080u;
-                                h[2 * k] = codes8<0, 1>(x);
-                                h[2 * k + 1] = codes8<2, 3>(x);
-                            } else {
-                                uint32_t four[4];
-                                codes4_in_order(words[k], four);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) h[4 * k + i] = four[i];
-                            }
-                        }
-#pragma unroll
-                        for (int c = 0; c < kOut; ++c)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + many_at(kManyKeys, row, piece * kOut + c)), "r"(h[4 * c]),
-                                         "r"(h[4 * c + 1]), "r"(h[4 * c + 2]), "r"(h[4 * c + 3]) : "memory");
-                    }
-#pragma unroll
-                    for (int u = 0; u < kBatch; ++u) { v0[u] = v1[u]; v1[u] = v2[u]; }
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&kv_full[slot]);
-                more = step() && step();
-                continue;
-            }
             // Lane i looks up the i-th part of the block: a tensor copy where every key of it is a token that some row of the sequence
             // sees (and so holds numbers), row by row with zeros where not.
             const int low = a.window > 0 ? max(0, at.seq.first_pos + 1 - a.window) : 0;
@@ -586,36 +502,120 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 __syncwarp();
             }
             const uint32_t dst = tile_base + slot * S::kTileBytes;
-            if (from >= 0) {
-                const int row = static_cast<int>(from) + at.head * p.page_size;
+            if constexpr (BITS == 16) {
+                if (from >= 0) {
+                    const int row = static_cast<int>(from) + at.head * p.page_size;
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h)
-                    tma_rows(dst + h * kManyKeys * 128 + lane * box_rows * 128, w & 1 ? &v_map : &k_map, h * 128, row, &kv_full[slot]);
-            }
-            __syncwarp();
-            if (__popc(whole) < parts || parts == 0) {
+                    for (int h = 0; h < D / 64; ++h)
+                        tma_rows(dst + h * kManyKeys * 128 + lane * box_rows * 128, w & 1 ? &v_map : &k_map, h * 128, row, &kv_full[slot]);
+                }
+                __syncwarp();
+                if (__popc(whole) < parts || parts == 0) {
+#pragma unroll 1
+                    for (int k0 = 0; k0 < kManyKeys; k0 += 32) {  // 32 keys: lane i finds key k0 + i
+                        const int key = first + k0 + lane;
+                        int64_t place = -1;
+                        if (key >= at.seg.key0 && key < at.seg.key1) place = kv_place(p, at.b, key);
+                        if (place >= 0) place += static_cast<int64_t>(at.head) * p.page_size;
+#pragma unroll
+                        for (int i = 0; i < 32 / kRowStep; ++i) {
+                            const int r = row0 + i * kRowStep;
+                            const int64_t row = __shfl_sync(0xffffffffu, place, r);
+                            if (parts == 0 || !(whole >> ((k0 + r) / box_rows) & 1u))
+                                copy16_fill(dst + many_at(kManyKeys, k0 + r, chunk), pool + (row < 0 ? 0 : row * (D * 2)), row >= 0);
+                        }
+                    }
+                    copy_commit();
+                    copy_wait<0>();
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                // the copies' bytes may arrive before they are announced: the phase ends with this arrival at the earliest
+                if (lane == 0) mbar_expect_tx(&kv_full[slot], static_cast<uint32_t>(__popc(whole) * box_rows * D * 2));
+                __syncwarp();
+            } else {
+                // Codes come into the end of the tile's own place, row by row what the tensor copies would bring, and are turned into fp16
+                // from the first row on: a row's fp16 covers no codes of rows behind it.
+                constexpr int kRowBytes = D * BITS / 8, kPieces = kRowBytes / 16;
+                const uint32_t raw = dst + S::kTileBytes - kManyKeys * kRowBytes;
+                const int kept = (tile >> 1) % S::kScaleBlocks;
+                float* const scales = block_scales + kept * 2 * kManyKeys + (w & 1) * kManyKeys;
+                if (from >= 0) tma_rows(raw + lane * box_rows * kRowBytes, w & 1 ? &v_map : &k_map, 0, static_cast<int>(from) + at.head * p.page_size, &raw_full[slot]);
+                __syncwarp();
+                float top = 0.0f;
 #pragma unroll 1
                 for (int k0 = 0; k0 < kManyKeys; k0 += 32) {      // 32 keys: lane i finds key k0 + i
                     const int key = first + k0 + lane;
                     int64_t place = -1;
                     if (key >= at.seg.key0 && key < at.seg.key1) place = kv_place(p, at.b, key);
                     if (place >= 0) place += static_cast<int64_t>(at.head) * p.page_size;
+                    const float f = place >= 0 ? __ldg((w & 1 ? p.v_scale : p.k_scale) + place) : 0.0f;       // hidden keys have none
+                    scales[k0 + lane] = f;
+                    top = fmaxf(top, f);
+                    if (__popc(whole) < parts || parts == 0) {
+                        constexpr int kStep = 32 / kPieces;
 #pragma unroll
-                    for (int i = 0; i < 32 / kRowStep; ++i) {
-                        const int r = row0 + i * kRowStep;
-                        const int64_t row = __shfl_sync(0xffffffffu, place, r);
-                        if (parts == 0 || !(whole >> ((k0 + r) / box_rows) & 1u))
-                            copy16_fill(dst + many_at(kManyKeys, k0 + r, chunk), pool + (row < 0 ? 0 : row * (D * 2)), row >= 0);
+                        for (int i = 0; i < 32 / kStep; ++i) {
+                            const int r = i * kStep + lane / kPieces, piece = lane % kPieces;
+                            const int64_t row = __shfl_sync(0xffffffffu, place, r);
+                            if (parts == 0 || !(whole >> ((k0 + r) / box_rows) & 1u))
+                                copy16_fill(raw + tile_at<kPieces, kManyKeys>(k0 + r, piece),
+                                            static_cast<const char*>(w & 1 ? p.v : p.k) + (row < 0 ? 0 : row * kRowBytes) + piece * 16, row >= 0);
+                        }
                     }
                 }
+                if (lane == 0) mbar_expect_tx(&raw_full[slot], static_cast<uint32_t>(__popc(whole) * box_rows * kRowBytes));
+                if (w & 1) {
+#pragma unroll
+                    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    // values below 2^-100 are as good as zero
+                    if (lane == 0) s_top[kept] = log2f(fmaxf(top, 7.8886091e-31f));
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&scales_full[kept]);
                 copy_commit();
                 copy_wait<0>();
+                many_wait(&raw_full[slot], (tile / S::kSlots) & 1u, &s_failed);
+                __syncwarp();
+                constexpr int kAtOnce = 32 / kPieces, kTurns = kManyKeys / kAtOnce, kOut = 16 / BITS;      // 16-byte chunks of fp16 out of one of codes
+                const int piece = lane % kPieces, sub = lane / kPieces;
+#pragma unroll 1
+                for (int t0 = 0; t0 < kTurns; t0 += 4) {
+                    uint32_t words[4][4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t from_at = raw + tile_at<kPieces, kManyKeys>((t0 + u) * kAtOnce + sub, piece);
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(words[u][0]), "=r"(words[u][1]), "=r"(words[u][2]), "=r"(words[u][3]) : "r"(from_at) : "memory");
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int row = (t0 + u) * kAtOnce + sub;
+                        uint32_t h[4 * kOut];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if constexpr (BITS == 8) {
+                                const uint32_t x = words[u][k] ^ 0x80808080u;
+                                h[2 * k] = codes8<0, 1>(x);
+                                h[2 * k + 1] = codes8<2, 3>(x);
+                            } else {
+                                uint32_t four[4];
+                                codes4_in_order(words[u][k], four);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) h[4 * k + i] = four[i];
+                            }
+                        }
+#pragma unroll
+                        for (int c = 0; c < kOut; ++c)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + many_at(kManyKeys, row, piece * kOut + c)), "r"(h[4 * c]),
+                                         "r"(h[4 * c + 1]), "r"(h[4 * c + 2]), "r"(h[4 * c + 3]) : "memory");
+                    }
+                    __syncwarp();
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
+                if (lane == 0) mbar_arrive(&kv_full[slot]);
             }
-            // the copies' bytes may arrive before they are announced: the phase ends with this arrival at the earliest
-            if (lane == 0) mbar_expect_tx(&kv_full[slot], static_cast<uint32_t>(__popc(whole) * box_rows * D * 2));
-            __syncwarp();
             more = step() && step();
         }
     } else {
@@ -786,7 +786,7 @@ cudaError_t launch_many(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t 
     }
     CUtensorMap k_map{}, v_map{};
     int box_rows = 0;
-    if (BITS != 16 || !kv_tensor_maps(p, kManyKeys, &k_map, &v_map, &box_rows)) box_rows = 0;
+    if (!kv_tensor_maps(p, kManyKeys, &k_map, &v_map, &box_rows)) box_rows = 0;
     return launch_dependent(kv_many_kernel<T, BITS, D>, dim3(static_cast<unsigned>(sm_count())), dim3(kManyThreads), S::kSmem, stream, k_map, v_map, p, a,
                             box_rows);
 }

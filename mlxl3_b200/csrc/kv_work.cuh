@@ -250,6 +250,15 @@ __device__ __forceinline__ void copy4_fill(uint32_t dst, const void* src, bool l
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// Where a 16-byte chunk of a tile's row lies, as the tensor copies put it: pieces of up to 128 bytes of all rows, one after the other; in
+// a piece rows of 128 bytes swap their chunks by the row's number, shorter ones by the number of the 128 bytes they are in, so that eight
+// rows' same chunk uses all banks.
+template <int CHUNKS, int KEYS>
+__device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
+    constexpr int kPiece = CHUNKS >= 8 ? 8 : CHUNKS, kShift = CHUNKS >= 8 ? 0 : (CHUNKS == 4 ? 1 : 2);
+    return static_cast<uint32_t>((chunk / kPiece * KEYS + row) * kPiece + ((chunk % kPiece) ^ ((row >> kShift) & (kPiece - 1)))) * 16;
+}
+
 // Two codes as fp16.  8 bits: bytes i and j of a word whose sign bits were flipped become 1024 + (code + 128); 4 bits: the low nibbles
 // of its halves become 1024 + (code + 8).
 __device__ __forceinline__ uint32_t less(uint32_t a, uint32_t bias) {
