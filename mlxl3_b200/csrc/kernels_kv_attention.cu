@@ -264,18 +264,17 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
                     }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int x = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
-                // |x| <= 133: in two factors, each a normal number
-                const float f0 = ldexpf(1.0f, -x / 2), f1 = ldexpf(1.0f, -x - -x / 2);
+                const KvPower power(top);
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s)
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
                         const float2 f = KvType<T>::unpack(q[b][s][w]);
-                        q[b][s][w] = KvType<M>::pack(f.x * f0 * f1, f.y * f0 * f1);
+                        q[b][s][w] = KvType<M>::pack(f.x * power.down0 * power.down1, f.y * power.down0 * power.down1);
                     }
 #pragma unroll
-                for (int e = 0; e < 2; ++e) row_scale[b][e] = ldexpf(row_scale[b][e], __shfl_sync(0xffffffffu, x, (2 * t + e) * 4));
+                for (int e = 0; e < 2; ++e)
+                    row_scale[b][e] = row_scale[b][e] * __shfl_sync(0xffffffffu, power.up0, (2 * t + e) * 4) * __shfl_sync(0xffffffffu, power.up1, (2 * t + e) * 4);
             }
         }
     };

@@ -540,19 +540,22 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 const uint32_t raw = dst + S::kTileBytes - kManyKeys * kRowBytes;
                 const int kept = (tile >> 1) % S::kScaleBlocks;
                 float* const scales = block_scales + kept * 2 * kManyKeys + (w & 1) * kManyKeys;
-                if (from >= 0) tma_rows(raw + lane * box_rows * kRowBytes, w & 1 ? &v_map : &k_map, 0, static_cast<int>(from) + at.head * p.page_size, &raw_full[slot]);
+                if (from >= 0) {
+                    const int row = static_cast<int>(from) + at.head * p.page_size;
+                    tma_rows(raw + lane * box_rows * kRowBytes, w & 1 ? &v_map : &k_map, 0, row, &raw_full[slot]);
+                    bulk_copy_g2s(scales + lane * box_rows, (w & 1 ? p.v_scale : p.k_scale) + row, box_rows * 4, &raw_full[slot]);
+                }
                 __syncwarp();
-                float top = 0.0f;
+                if (__popc(whole) < parts || parts == 0) {
 #pragma unroll 1
-                for (int k0 = 0; k0 < kManyKeys; k0 += 32) {      // 32 keys: lane i finds key k0 + i
-                    const int key = first + k0 + lane;
-                    int64_t place = -1;
-                    if (key >= at.seg.key0 && key < at.seg.key1) place = kv_place(p, at.b, key);
-                    if (place >= 0) place += static_cast<int64_t>(at.head) * p.page_size;
-                    const float f = place >= 0 ? __ldg((w & 1 ? p.v_scale : p.k_scale) + place) : 0.0f;       // hidden keys have none
-                    scales[k0 + lane] = f;
-                    top = fmaxf(top, f);
-                    if (__popc(whole) < parts || parts == 0) {
+                    for (int k0 = 0; k0 < kManyKeys; k0 += 32) {  // 32 keys: lane i finds key k0 + i
+                        if (parts > 0 && box_rows >= 32 && (whole >> (k0 / box_rows) & 1u)) continue;
+                        const int key = first + k0 + lane;
+                        int64_t place = -1;
+                        if (key >= at.seg.key0 && key < at.seg.key1) place = kv_place(p, at.b, key);
+                        if (place >= 0) place += static_cast<int64_t>(at.head) * p.page_size;
+                        if (parts == 0 || !(whole >> ((k0 + lane) / box_rows) & 1u))
+                            scales[k0 + lane] = place >= 0 ? __ldg((w & 1 ? p.v_scale : p.k_scale) + place) : 0.0f;      // hidden keys have none
                         constexpr int kStep = 32 / kPieces;
 #pragma unroll
                         for (int i = 0; i < 32 / kStep; ++i) {
@@ -563,9 +566,15 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                                             static_cast<const char*>(w & 1 ? p.v : p.k) + (row < 0 ? 0 : row * kRowBytes) + piece * 16, row >= 0);
                         }
                     }
+                    copy_commit();
+                    copy_wait<0>();
                 }
-                if (lane == 0) mbar_expect_tx(&raw_full[slot], static_cast<uint32_t>(__popc(whole) * box_rows * kRowBytes));
+                if (lane == 0) mbar_expect_tx(&raw_full[slot], static_cast<uint32_t>(__popc(whole) * box_rows * (kRowBytes + 4)));
+                __syncwarp();
+                many_wait(&raw_full[slot], (tile / S::kSlots) & 1u, &s_failed);
+                __syncwarp();
                 if (w & 1) {
+                    float top = fmaxf(fmaxf(scales[lane], scales[lane + 32]), fmaxf(scales[lane + 64], scales[lane + 96]));
 #pragma unroll
                     for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                     // values below 2^-100 are as good as zero
@@ -573,10 +582,6 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&scales_full[kept]);
-                copy_commit();
-                copy_wait<0>();
-                many_wait(&raw_full[slot], (tile / S::kSlots) & 1u, &s_failed);
-                __syncwarp();
                 constexpr int kAtOnce = 32 / kPieces, kTurns = kManyKeys / kAtOnce, kOut = 16 / BITS;      // 16-byte chunks of fp16 out of one of codes
                 const int piece = lane % kPieces, sub = lane / kPieces;
 #pragma unroll 1
@@ -721,38 +726,45 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 // the products of this tile's segment before have read their queries
                 if (loaded > 0) many_wait(&q_free[x], (loaded - 1) & 1, &s_failed);
                 __syncwarp();
-#pragma unroll 8
-                for (int i = 0; i < kManyTile / kStep; ++i) {
-                    const int q = i * kStep + lane / kChunks;
-                    const bool live = row0 + q < rows;
+                auto source = [&](int q, bool live) {             // row q of the tile
                     // (past + q) / group: half a row away from where fp32 could round it over an edge
                     const int token = __float2int_rz((static_cast<float>(past + q) + 0.5f) * per_token);
-                    const T* src = base + (live ? token * a.q_stride + (past + q - token * work.group) * D : 0);
-                    if (!live) src = static_cast<const T*>(a.q);
-                    if constexpr (std::is_same_v<T, M>) {
-                        copy16_fill(dst + many_at(kManyTile, q, chunk), src, live);
-                    } else {
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (live) v = *reinterpret_cast<const uint4*>(src);
-                        uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                        float top = 0.0f;
+                    return live ? base + token * a.q_stride + (past + q - token * work.group) * D : static_cast<const T*>(a.q);
+                };
+                if constexpr (std::is_same_v<T, M>) {
+#pragma unroll 8
+                    for (int q = lane / kChunks; q < kManyTile; q += kStep) {
+                        const bool live = row0 + q < rows;
+                        copy16_fill(dst + many_at(kManyTile, q, chunk), source(q, live), live);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int q0 = lane / kChunks; q0 < kManyTile; q0 += 8 * kStep) {
+                        uint4 v[8];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float2 f = KvType<T>::unpack(w[k]);
-                            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                        for (int i = 0; i < 8; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(source(q0 + i * kStep, row0 + q0 + i * kStep < rows)));
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int q = q0 + i * kStep;
+                            uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                            float top = 0.0f;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float2 f = KvType<T>::unpack(w[k]);
+                                top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                            }
+#pragma unroll
+                            for (int d = kChunks / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                            const KvPower power(top);
+                            const bool live = row0 + q < rows;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float2 f = KvType<T>::unpack(w[k]);
+                                w[k] = live ? KvType<M>::pack(f.x * power.down0 * power.down1, f.y * power.down0 * power.down1) : 0u;
+                            }
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + many_at(kManyTile, q, chunk)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                            if (chunk == 0) s_q_scale[loaded & 1][x * kManyTile + q] = a.scale_log2e * power.up0 * power.up1;
                         }
-#pragma unroll
-                        for (int d = kChunks / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        const int e = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
-                        // |e| <= 133: in two factors, each a normal number
-                        const float f0 = ldexpf(1.0f, -e / 2), f1 = ldexpf(1.0f, -e - -e / 2);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float2 f = KvType<T>::unpack(w[k]);
-                            w[k] = KvType<M>::pack(f.x * f0 * f1, f.y * f0 * f1);
-                        }
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + many_at(kManyTile, q, chunk)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-                        if (chunk == 0) s_q_scale[loaded & 1][x * kManyTile + q] = ldexpf(a.scale_log2e, e);
                     }
                 }
                 copy_commit();

@@ -241,6 +241,19 @@ __device__ __forceinline__ float exp2_fast(float x) {             // 2 ulp; exp2
 // 1 / sum of a row; a row that sees nothing is zero
 __device__ __forceinline__ float kv_inverse(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
 
+// The power of two that brings a row's largest magnitude to [1, 2), and its inverse, in two factors each: all of them are normal numbers.
+struct KvPower {
+    float down0, down1, up0, up1;
+    __device__ __forceinline__ explicit KvPower(float top) {
+        const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127, half = e >> 1;        // -127 for 0
+        down0 = power(-half);
+        down1 = power(half - e);
+        up0 = power(half);
+        up1 = power(e - half);
+    }
+    static __device__ __forceinline__ float power(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+};
+
 __device__ __forceinline__ void copy16_fill(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
