@@ -15,6 +15,7 @@
 // Both kernels are bound by memory (and short calls by the chain row_start -> length -> page table -> data): 16 or 8 lanes hold a
 // vector, 8 dimensions each, so that every access is 16 bytes (8 or 4 for codes) and a vector one coalesced piece.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_work.cuh"
 
@@ -73,8 +74,17 @@ __device__ __forceinline__ double kv_abs_max(double m, double x) { x = fabs(x); 
 __device__ __forceinline__ float kv_abs_max(float m, float x) { x = fabsf(x); return x > m || x != x ? x : m; }
 __device__ __forceinline__ double kv_divide(double a, double b) { return __ddiv_rn(a, b); }
 __device__ __forceinline__ float kv_divide(float a, float b) { return __fdiv_rn(a, b); }
-__device__ __forceinline__ int kv_round(double x) { return __double2int_rn(x); }
-__device__ __forceinline__ int kv_round(float x) { return __float2int_rn(x); }
+// The whole number nearest to t, |t| < 2^20, and t's distance from it
+__device__ __forceinline__ int kv_nearest(double t, double& off) {
+    const double r = __dadd_rn(t, 6755399441055744.0);            // 1.5 * 2^52
+    off = t - __dsub_rn(r, 6755399441055744.0);
+    return __double2loint(r);
+}
+__device__ __forceinline__ int kv_nearest(float t, float& off) {
+    const float r = __fadd_rn(t, 12582912.0f);                    // 1.5 * 2^23
+    off = t - __fsub_rn(r, 12582912.0f);
+    return static_cast<int>(__float_as_uint(r) << 10) >> 10;
+}
 
 // Codes of eight dimensions of a vector that LANES neighbouring lanes hold, and its scale.  A NaN or an infinity anywhere is the
 // scale, with codes of 0: the whole vector reads as NaN.
@@ -88,10 +98,17 @@ __device__ __forceinline__ void kv_quantise(const F (&x)[8], uint32_t (&words)[2
     for (int d = LANES / 2; d >= 1; d >>= 1) top = kv_abs_max(top, __shfl_xor_sync(0xffffffffu, top, d));
     scale = static_cast<float>(kv_divide(top, static_cast<F>(M)));
     words[0] = words[1] = 0;
+    // x M / top by the inverse of top; where that comes near the middle between two codes (its error is below 2^-16 or 2^-44) the
+    // quotient itself decides
+    const bool sound = top > 0 && top < static_cast<F>(INFINITY);
+    const F inverse = sound ? kv_divide(static_cast<F>(M), top) : static_cast<F>(0), near = static_cast<F>(0.5) - (sizeof(F) == 4 ? static_cast<F>(1e-4) : static_cast<F>(1e-9));
+    const bool small = inverse > static_cast<F>(sizeof(F) == 4 ? 1e38 : 1e300);       // the inverse of a subnormal: every quotient itself
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        int code = top > 0 && top < static_cast<F>(INFINITY) ? kv_round(kv_divide(x[i] * static_cast<F>(M), top)) : 0;
-        code = max(-M, min(M, code));
+        F off;
+        int code = kv_nearest(small ? static_cast<F>(0) : x[i] * inverse, off);
+        if (sound && (small || fabs(off) > near)) code = kv_nearest(kv_divide(x[i] * static_cast<F>(M), top), off);
+        if (!sound) code = 0;
         if constexpr (BITS == 8) words[i >> 2] |= static_cast<uint32_t>(code & 0xff) << (8 * (i & 3));
         else words[0] |= static_cast<uint32_t>(code + 8) << (4 * i);
     }
@@ -106,12 +123,15 @@ __device__ __forceinline__ void kv_store_codes(void* pool, float* scales, int64_
 }
 
 template <typename T, int BITS, int D, int ROWS>
-__global__ void __launch_bounds__(kKvThreads)
+__global__ void __launch_bounds__(kKvThreads, 4)
 kv_append_kernel(const KvArgs p, const KvAppendArgs a) {
-    constexpr int LANES = D / 8, kGroups = kKvThreads / LANES;
+    // every row has warps of its own, all of which get their share of q, k and v
+    constexpr int LANES = D / 8, kRowThreads = kKvThreads / ROWS, kGroups = kRowThreads / LANES, kAtOnce = 4;
+    static_assert(kRowThreads % 32 == 0, "whole warps");
     __shared__ int s_start[kKvStarts + 1];
     __shared__ KvRow s_row[ROWS];
-    __shared__ double s_cos[ROWS][D / 2], s_sin[ROWS][D / 2];
+    __shared__ double2 s_turn[ROWS][BITS == 16 ? 1 : D / 2];      // cosine and sine
+    __shared__ float2 s_turn_f[ROWS][D / 2];
     pdl_launch_dependents();
     pdl_wait();
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * ROWS;
@@ -122,108 +142,113 @@ kv_append_kernel(const KvArgs p, const KvAppendArgs a) {
         const double turns = static_cast<double>(s_row[r].pos) * __ldg(a.turns + j);
         double sn, cs;
         sincospi(2.0 * (turns - rint(turns)), &sn, &cs);
-        s_cos[r][j] = cs * a.magnitude;
-        s_sin[r][j] = sn * a.magnitude;
+        cs *= a.magnitude;
+        sn *= a.magnitude;
+        s_turn_f[r][j] = make_float2(static_cast<float>(cs), static_cast<float>(sn));
+        if constexpr (BITS != 16) s_turn[r][j] = make_double2(cs, sn);
     }
     __syncthreads();
-    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES, group = threadIdx.x % kRowThreads / LANES;
     const int vectors = a.heads + 2 * p.kv_heads;
     const int d0 = lane * 8;
     // this lane's partner in the half layout: the same place of the other half of the rotated dimensions
     const int half_lanes = a.rotated / 16;
     const bool rotates = d0 < a.rotated, upper = lane >= half_lanes;
     const int partner = !rotates || a.interleaved ? lane : (upper ? lane - half_lanes : lane + half_lanes);
-    const int pair0 = a.interleaved ? d0 / 2 : (upper ? d0 - pairs : d0);
-    // whole warps go round together (the shuffles); a group without a vector holds zeros and stores nothing
-    const int total = ROWS * vectors;
-    for (int first = 0; first < total; first += kGroups) {
-        const int item = first + group;
-        const int r = min(item / vectors, ROWS - 1), vec = item - r * vectors;
+    const int pair0 = !rotates ? 0 : a.interleaved ? d0 / 2 : (upper ? d0 - pairs : d0);
+    {
+        const int r = threadIdx.x / kRowThreads;
         const KvRow at = s_row[r];
+        if (at.pos < 0) return;                                   // the same for all of the row's warps
         const int64_t row = row0 + r;
-        const bool is_q = vec < a.heads, is_k = !is_q && vec < a.heads + p.kv_heads;
-        const int head = is_q ? vec : (is_k ? vec - a.heads : vec - a.heads - p.kv_heads);
-        const bool live = item < total && at.pos >= 0 && (is_q || at.place >= 0);
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (live) {
-            const T* src = is_q ? static_cast<const T*>(a.q) + row * a.q_stride
-                                : (is_k ? static_cast<const T*>(a.k) + row * a.k_stride : static_cast<const T*>(a.v) + row * a.v_stride);
-            w = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(head) * D + d0);
-        }
-        uint32_t own[4] = {w.x, w.y, w.z, w.w}, other[4];
+        // the lane's dimensions are the same of every head, and so are its angles
+        float2 turn_f[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) other[i] = __shfl_sync(0xffffffffu, own[i], partner, LANES);
-        // x[i] of dimension d0 + i turned, in F
-        auto turn = [&](auto zero, auto (&x)[8]) {
-            using F = decltype(zero);
+        for (int i = 0; i < 8; ++i) turn_f[i] = rotates ? s_turn_f[r][a.interleaved ? pair0 + i / 2 : pair0 + i] : make_float2(1.0f, 0.0f);
+#pragma unroll 1
+        for (int first = 0; first < vectors; first += kAtOnce * kGroups) {
+            uint4 loaded[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = KvType<T>::unpack(own[i]);
-                x[2 * i] = f.x;
-                x[2 * i + 1] = f.y;
-            }
-            if (!rotates || pairs == 0) return;
-            if (a.interleaved) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const F c = static_cast<F>(s_cos[r][pair0 + i]), s = static_cast<F>(s_sin[r][pair0 + i]), u = x[2 * i], v = x[2 * i + 1];
-                    x[2 * i] = u * c - v * s;
-                    x[2 * i + 1] = u * s + v * c;
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int vec = first + u * kGroups + group;
+                loaded[u] = make_uint4(0, 0, 0, 0);
+                if (vec < vectors) {
+                    const T* src = vec < a.heads ? static_cast<const T*>(a.q) + row * a.q_stride + static_cast<int64_t>(vec) * D
+                                   : vec < a.heads + p.kv_heads ? static_cast<const T*>(a.k) + row * a.k_stride + static_cast<int64_t>(vec - a.heads) * D
+                                                                : static_cast<const T*>(a.v) + row * a.v_stride + static_cast<int64_t>(vec - a.heads - p.kv_heads) * D;
+                    loaded[u] = *reinterpret_cast<const uint4*>(src + d0);
                 }
-            } else {
+            }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = KvType<T>::unpack(other[i]);
-                    const F y[2] = {f.x, f.y};
+            for (int u = 0; u < kAtOnce; ++u) {
+                // whole warps go round together (the shuffles); a group without a vector holds zeros and stores nothing
+                if (first + u * kGroups >= vectors) break;
+                const int vec = first + u * kGroups + group;
+                const bool is_q = vec < a.heads, is_k = !is_q && vec < a.heads + p.kv_heads;
+                const int head = is_q ? vec : (is_k ? vec - a.heads : vec - a.heads - p.kv_heads);
+                const bool live = vec < vectors && (is_q || at.place >= 0);
+                const uint32_t own[4] = {loaded[u].x, loaded[u].y, loaded[u].z, loaded[u].w};
+                uint32_t other[4];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const F c = static_cast<F>(s_cos[r][pair0 + 2 * i + e]), s = static_cast<F>(s_sin[r][pair0 + 2 * i + e]), u = x[2 * i + e];
-                        x[2 * i + e] = upper ? y[e] * s + u * c : u * c - y[e] * s;
+                for (int i = 0; i < 4; ++i) other[i] = __shfl_sync(0xffffffffu, own[i], partner, LANES);
+                // x[i] of dimension d0 + i turned, in F
+                auto turn = [&](auto angle, auto (&x)[8]) {
+                    using F = std::remove_reference_t<decltype(x[0])>;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 f = KvType<T>::unpack(own[i]), o = KvType<T>::unpack(other[i]);
+                        x[2 * i] = f.x;
+                        x[2 * i + 1] = f.y;
+                        const auto t0 = angle(2 * i), t1 = angle(2 * i + 1);
+                        const F u0 = f.x, u1 = f.y, y0 = o.x, y1 = o.y;
+                        if (!rotates) continue;
+                        if (a.interleaved) {
+                            x[2 * i] = u0 * t0.x - u1 * t0.y;
+                            x[2 * i + 1] = u0 * t0.y + u1 * t0.x;
+                        } else if (upper) {
+                            x[2 * i] = y0 * t0.y + u0 * t0.x;
+                            x[2 * i + 1] = y1 * t1.y + u1 * t1.x;
+                        } else {
+                            x[2 * i] = u0 * t0.x - y0 * t0.y;
+                            x[2 * i + 1] = u1 * t1.x - y1 * t1.y;
+                        }
+                    }
+                };
+                auto angle_f = [&](int i) { return turn_f[i]; };
+                auto store = [&](T* dst, const float (&x)[8]) {
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(KvType<T>::pack(x[0], x[1]), KvType<T>::pack(x[2], x[3]), KvType<T>::pack(x[4], x[5]),
+                                                                KvType<T>::pack(x[6], x[7]));
+                };
+                const int64_t vector = at.place + static_cast<int64_t>(head) * p.page_size;
+                if (is_q ? live : BITS == 16 && is_k && live) {
+                    float x[8];
+                    turn(angle_f, x);
+                    store(is_q ? static_cast<T*>(a.q_out) + row * a.q_out_stride + static_cast<int64_t>(head) * D + d0 : static_cast<T*>(p.k) + vector * D + d0, x);
+                }
+                if constexpr (BITS == 16) {
+                    if (!is_q && !is_k && live) *reinterpret_cast<uint4*>(static_cast<T*>(p.v) + vector * D + d0) = loaded[u];
+                } else {
+                    // a warp may hold vectors of several kinds: all its lanes go through the shuffles of both
+                    uint32_t words[2];
+                    float scale;
+                    if (__any_sync(0xffffffffu, is_k && live)) {
+                        double x[8];
+                        turn([&](int i) { return s_turn[r][a.interleaved ? pair0 + i / 2 : pair0 + i]; }, x);
+                        kv_quantise<BITS, LANES>(x, words, scale);
+                        if (is_k && live) kv_store_codes<BITS, D>(p.k, p.k_scale, vector, lane, words, scale);
+                    }
+                    if (__any_sync(0xffffffffu, !is_q && !is_k && live)) {
+                        float x[8];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 f = KvType<T>::unpack(own[i]);
+                            x[2 * i] = f.x;
+                            x[2 * i + 1] = f.y;
+                        }
+                        kv_quantise<BITS, LANES>(x, words, scale);
+                        if (!is_q && !is_k && live) kv_store_codes<BITS, D>(p.v, p.v_scale, vector, lane, words, scale);
                     }
                 }
-            }
-        };
-        const int64_t vector = at.place + static_cast<int64_t>(head) * p.page_size;
-        auto store = [&](T* dst, const float (&x)[8]) {
-            *reinterpret_cast<uint4*>(dst) = make_uint4(KvType<T>::pack(x[0], x[1]), KvType<T>::pack(x[2], x[3]), KvType<T>::pack(x[4], x[5]),
-                                                        KvType<T>::pack(x[6], x[7]));
-        };
-        if constexpr (BITS == 16) {
-            if (!live) continue;
-            if (is_q || is_k) {
-                float x[8];
-                turn(0.0f, x);
-                store(is_q ? static_cast<T*>(a.q_out) + row * a.q_out_stride + static_cast<int64_t>(head) * D + d0 : static_cast<T*>(p.k) + vector * D + d0, x);
-            } else {
-                *reinterpret_cast<uint4*>(static_cast<T*>(p.v) + vector * D + d0) = w;
-            }
-        } else {
-            if (is_q) {
-                if (live) {
-                    float x[8];
-                    turn(0.0f, x);
-                    store(static_cast<T*>(a.q_out) + row * a.q_out_stride + static_cast<int64_t>(head) * D + d0, x);
-                }
-            }
-            // a warp may hold vectors of several kinds: all its lanes go through the shuffles of both
-            uint32_t words[2];
-            float scale;
-            if (__any_sync(0xffffffffu, is_k && live)) {
-                double x[8];
-                turn(0.0, x);
-                kv_quantise<BITS, LANES>(x, words, scale);
-                if (is_k && live) kv_store_codes<BITS, D>(p.k, p.k_scale, vector, lane, words, scale);
-            }
-            if (__any_sync(0xffffffffu, !is_q && !is_k && live)) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = KvType<T>::unpack(own[i]);
-                    x[2 * i] = f.x;
-                    x[2 * i + 1] = f.y;
-                }
-                kv_quantise<BITS, LANES>(x, words, scale);
-                if (!is_q && !is_k && live) kv_store_codes<BITS, D>(p.v, p.v_scale, vector, lane, words, scale);
             }
         }
     }
@@ -253,47 +278,61 @@ kv_read_kernel(const KvArgs p, O* __restrict__ k_out, O* __restrict__ v_out) {
     kv_locate<ROWS>(p, row0, s_start, s_row);
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
     const int vectors = 2 * p.kv_heads, total = ROWS * vectors;
-#pragma unroll 4
-    for (int item = group; item < total; item += kGroups) {
-        const int r = item / vectors, vec = item - r * vectors;
-        const bool is_k = vec < p.kv_heads;
-        const int head = is_k ? vec : vec - p.kv_heads;
-        const KvRow at = s_row[r];
-        O* out = is_k ? k_out : v_out;
-        if (at.place < 0 || out == nullptr) continue;
-        const int64_t vector = at.place + static_cast<int64_t>(head) * p.page_size;
-        const char* src = static_cast<const char*>(is_k ? p.k : p.v) + vector * (D * BITS / 8) + lane * BITS;
-        float x[8];
-        if constexpr (BITS == 16) {
-            const uint4 w = __ldcs(reinterpret_cast<const uint4*>(src));
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    constexpr int kAtOnce = 4;
+#pragma unroll 1
+    for (int first = group; first < total; first += kAtOnce * kGroups) {
+        uint4 loaded[kAtOnce];                                    // 16, 8 or 4 bytes of it
+        float scale[kAtOnce];
+        O* dst[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = KvType<T>::unpack(words[i]);
-                x[2 * i] = f.x;
-                x[2 * i + 1] = f.y;
-            }
-        } else {
-            const float scale = __ldg((is_k ? p.k_scale : p.v_scale) + vector);
-            if constexpr (BITS == 8) {
-                const uint2 w = __ldcs(reinterpret_cast<const uint2*>(src));
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    x[i] = scale * static_cast<float>(static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3))));
-            } else {
-                const uint32_t w = __ldcs(reinterpret_cast<const uint32_t*>(src));
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = scale * static_cast<float>(static_cast<int>((w >> (4 * i)) & 15u) - 8);
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int item = first + u * kGroups;
+            const int r = min(item / vectors, ROWS - 1), vec = item - r * vectors;
+            const bool is_k = vec < p.kv_heads;
+            const int head = is_k ? vec : vec - p.kv_heads;
+            const KvRow at = s_row[r];
+            O* out = is_k ? k_out : v_out;
+            dst[u] = item < total && at.place >= 0 && out != nullptr ? out + ((row0 + r) * p.kv_heads + head) * D + lane * 8 : nullptr;
+            scale[u] = 0.0f;
+            if (dst[u] == nullptr) continue;
+            const int64_t vector = at.place + static_cast<int64_t>(head) * p.page_size;
+            const char* src = static_cast<const char*>(is_k ? p.k : p.v) + vector * (D * BITS / 8) + lane * BITS;
+            if constexpr (BITS == 16) loaded[u] = __ldcs(reinterpret_cast<const uint4*>(src));
+            else {
+                if constexpr (BITS == 8) { const uint2 w = __ldcs(reinterpret_cast<const uint2*>(src)); loaded[u].x = w.x; loaded[u].y = w.y; }
+                else loaded[u].x = __ldcs(reinterpret_cast<const uint32_t*>(src));
+                scale[u] = __ldg((is_k ? p.k_scale : p.v_scale) + vector);
             }
         }
-        kv_store8(out + ((row0 + r) * p.kv_heads + head) * D + lane * 8, x);
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            if (dst[u] == nullptr) continue;
+            float x[8];
+            if constexpr (BITS == 16) {
+                const uint32_t words[4] = {loaded[u].x, loaded[u].y, loaded[u].z, loaded[u].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = KvType<T>::unpack(words[i]);
+                    x[2 * i] = f.x;
+                    x[2 * i + 1] = f.y;
+                }
+            } else if constexpr (BITS == 8) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[i] = scale[u] * static_cast<float>(static_cast<int8_t>((i < 4 ? loaded[u].x : loaded[u].y) >> (8 * (i & 3))));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = scale[u] * static_cast<float>(static_cast<int>((loaded[u].x >> (4 * i)) & 15u) - 8);
+            }
+            kv_store8(dst[u], x);
+        }
     }
 }
 
 // One row a CTA while that leaves SMs free: a short call is the latency of one row.  Eight (four appended) rows share the search
 // and fill the CTA's threads where there are many.
 template <int MANY>
-bool kv_many_rows(int64_t rows) { return rows >= static_cast<int64_t>(MANY) * 2 * sm_count(); }
+bool kv_many_rows(int64_t rows) { return rows >= static_cast<int64_t>(MANY) * sm_count(); }
 
 template <typename T, int BITS, int D>
 cudaError_t launch_append(const KvArgs& p, const KvAppendArgs& a, cudaStream_t stream) {
