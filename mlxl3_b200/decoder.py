@@ -189,6 +189,7 @@ class DenseDecoder:
         self.attn_ws = new_attention_workspace(self.heads, self.kv_heads)
         self.head_ws = DeviceBuffer(head_workspace_bytes())
         self.graph = None
+        self._chunk = None           # buffers of prefill, for the longest chunk so far
         self.store_logits = False
         self.fused = True            # norms, residual adds and SwiGLU run inside the projections' kernels; False: as kernels of their own
         self.stacked = False         # True (with fused, one GPU): o, [gate|up], down and the next block's [q|k|v] are ONE persistent launch
@@ -315,6 +316,53 @@ class DenseDecoder:
         head_argmax(b["xn"].ptr, self.head_weight.ptr, self.vocab, c.hidden, self.rank * self.vocab, b["logits"].ptr if self.store_logits else 0,
                     self.d_best_value.ptr, self.d_best_index.ptr, self.head_ws, s)
         self.launches_per_step = (5 if c.head_dim == 128 else 7) * len(self.layers) + 4
+
+    def prefill(self, tokens, pos: int = 0) -> None:
+        """Takes a chunk of a prompt in one pass: ``tokens`` at positions ``pos`` on, after whatever the cache holds before them.  The caches
+        get their rows, ``result()`` and ``logits`` (with ``store_logits``) belong to the last token, as after a ``step``.  The paged-cache
+        operators run on the decoder's own caches: one page of ``max_ctx`` rows (single GPU)."""
+        from . import kv
+        c, s = self.config, self.stream
+        tokens = np.ascontiguousarray(tokens, np.int32)
+        n = tokens.size
+        if self.tp is not None:
+            raise _lib.B200Exl3Error("prefill runs on a single GPU")
+        if tokens.ndim != 1 or n == 0 or pos < 0 or pos + n > c.max_ctx:
+            raise _lib.B200Exl3Error("prompt tokens do not fit the context")
+        if self._chunk is None or self._chunk["rows"] < n:
+            self._chunk = {name: DeviceBuffer(n * w * 2) for name, w in (
+                ("h", c.hidden), ("xn", c.hidden), ("q", self.heads * c.head_dim), ("k", self.kv_heads * c.head_dim), ("v", self.kv_heads * c.head_dim),
+                ("att", self.heads * c.head_dim), ("o", c.hidden), ("gate", self.ffn), ("up", self.ffn), ("down", c.hidden))}
+            ops = [e[name] for e in self.layers for name in ("qkv", "o", "gu", "down")]
+            self._chunk.update(rows=n, tokens=DeviceBuffer(n * 4), ws=new_workspace(max(op.workspace_bytes(n) for op in ops)),
+                               seq=DeviceBuffer.from_numpy(np.zeros(8, np.int32)), turns=DeviceBuffer.from_numpy(kv.rope_turns(c.head_dim, c.theta)))
+        b = self._chunk
+        caches = [kv.KvCache(1, c.max_ctx, self.kv_heads, c.head_dim, F16, 16, e["k_cache"].ptr, e["v_cache"].ptr) for e in self.layers]
+        if b.get("attn_rows", 0) < n:
+            b["attn_ws"], b["attn_rows"] = new_workspace(kv.attention_workspace_bytes(caches[0], self.heads, n)), n
+        b["tokens"].upload(tokens, s)
+        b["seq"].upload(np.array([0, n, pos + n, 0], np.int32), s)       # first rows, length, page table
+        s.sync()                                                          # the arrays above go away
+        batch = kv.KvBatch(b["seq"].ptr, b["seq"].ptr + 8, b["seq"].ptr + 12, 1, 1, n)
+        rope = kv.Rope(b["turns"].ptr, c.head_dim)
+        h, xn, q = b["h"].ptr, b["xn"].ptr, b["q"].ptr
+        embed(self.embed_table.ptr, b["tokens"].ptr, n, c.vocab, c.hidden, h, s)
+        pending = 0
+        for e, cache in zip(self.layers, caches):
+            rms_norm(h, pending, e["attn_norm"].ptr, n, c.hidden, c.eps, h if pending else 0, xn, s)
+            e["qkv"].forward_device(xn, F16, n, [q, b["k"].ptr, b["v"].ptr], b["ws"], s)
+            kv.append(cache, batch, b["k"].ptr, b["v"].ptr, rope, q, self.heads, q, stream=s)
+            kv.attention(cache, batch, q, self.heads, c.head_dim ** -0.5, b["att"].ptr, b["attn_ws"], n, stream=s)
+            e["o"].forward_device(b["att"].ptr, F16, n, b["o"].ptr, b["ws"], s)
+            rms_norm(h, b["o"].ptr, e["mlp_norm"].ptr, n, c.hidden, c.eps, h, xn, s)
+            e["gu"].forward_device(xn, F16, n, [b["gate"].ptr, b["up"].ptr], b["ws"], s)
+            e["down"].forward_fused_device(Prologue.swiglu(b["up"].ptr), b["gate"].ptr, n, b["down"].ptr, b["ws"], s)
+            pending = b["down"].ptr
+        last = (n - 1) * c.hidden * 2
+        rms_norm(h + last, pending + last, self.final_norm.ptr, 1, c.hidden, c.eps, self.buf["h"].ptr, self.buf["xn"].ptr, s)
+        self.hidden_name = "h"
+        head_argmax(self.buf["xn"].ptr, self.head_weight.ptr, self.vocab, c.hidden, self.rank * self.vocab, self.buf["logits"].ptr if self.store_logits else 0,
+                    self.d_best_value.ptr, self.d_best_index.ptr, self.head_ws, s)
 
     def record(self) -> None:
         self._launch()                                  # every distinct call once before recording

@@ -487,3 +487,35 @@ def test_prompt_in_pieces_equals_prompt_at_once(gpu, bits):
         outs.append((rotated, s.pool["k"], s.pool["v"]))
     for a, b in zip(*outs):
         assert np.array_equal(a, b)
+
+
+def test_decoder_prefill_equals_steps(gpu):
+    """A prompt through ``DenseDecoder.prefill`` (in one piece, and in two) against the same tokens one step at a time, and the step after it.
+    Bar: that of a decode step in tests/test_gpu_decoder.py, 3e-2 of the largest logit."""
+    from mlxl3_b200.decoder import DecoderConfig, DenseDecoder, SyntheticWeights
+    config = DecoderConfig(layers=2, hidden=512, heads=4, kv_heads=2, head_dim=128, ffn=1024, vocab=1024, k_bits=4, codebook=0, max_ctx=48)
+    weights = SyntheticWeights(config, seed=11)
+    tokens = np.random.default_rng(5).integers(0, 1024, 24).astype(np.int32)
+    steps = DenseDecoder(config, weights)
+    steps.store_logits = True
+    for i, token in enumerate(tokens):
+        steps.set_input(int(token), i)
+        steps.step()
+    want = steps.download("logits").astype(np.float32)
+    for pieces in ((24,), (1, 23), (17, 7)):
+        model = DenseDecoder(config, weights)
+        model.store_logits = True
+        done = 0
+        for n in pieces:
+            model.prefill(tokens[done:done + n], done)
+            done += n
+        got = model.download("logits").astype(np.float32)
+        assert np.abs(got - want).max() <= 3e-2 * np.abs(want).max()
+        assert want[model.result()[1]] >= want.max() - 3e-2 * np.abs(want).max()
+        for d in (model, steps):
+            d.set_input(7, 24)
+            d.step()
+        after, after_want = (d.download("logits").astype(np.float32) for d in (model, steps))
+        assert np.abs(after - after_want).max() <= 3e-2 * np.abs(after_want).max()
+    with pytest.raises(gpu.B200Exl3Error, match="do not fit"):
+        model.prefill(tokens, 30)
