@@ -269,30 +269,30 @@ __device__ __forceinline__ void kv_store8(O* dst, const float (&x)[8]) {
 template <typename T, int BITS, int D, typename O, int ROWS>
 __global__ void __launch_bounds__(kKvThreads)
 kv_read_kernel(const KvArgs p, O* __restrict__ k_out, O* __restrict__ v_out) {
-    constexpr int LANES = D / 8, kGroups = kKvThreads / LANES;
+    constexpr int LANES = D / 8, kRowThreads = kKvThreads / ROWS, kGroups = kRowThreads / LANES;
     __shared__ int s_start[kKvStarts + 1];
     __shared__ KvRow s_row[ROWS];
     pdl_launch_dependents();
     pdl_wait();
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * ROWS;
     kv_locate<ROWS>(p, row0, s_start, s_row);
-    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-    const int vectors = 2 * p.kv_heads, total = ROWS * vectors;
+    const int lane = threadIdx.x % LANES, group = threadIdx.x % kRowThreads / LANES, vectors = 2 * p.kv_heads;
+    const int r = threadIdx.x / kRowThreads;                      // every row has threads of its own
+    const KvRow at = s_row[r];
+    if (at.place < 0) return;
     constexpr int kAtOnce = 4;
 #pragma unroll 1
-    for (int first = group; first < total; first += kAtOnce * kGroups) {
+    for (int first = group; first < vectors; first += kAtOnce * kGroups) {
         uint4 loaded[kAtOnce];                                    // 16, 8 or 4 bytes of it
         float scale[kAtOnce];
         O* dst[kAtOnce];
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
-            const int item = first + u * kGroups;
-            const int r = min(item / vectors, ROWS - 1), vec = item - r * vectors;
+            const int vec = first + u * kGroups;
             const bool is_k = vec < p.kv_heads;
             const int head = is_k ? vec : vec - p.kv_heads;
-            const KvRow at = s_row[r];
             O* out = is_k ? k_out : v_out;
-            dst[u] = item < total && at.place >= 0 && out != nullptr ? out + ((row0 + r) * p.kv_heads + head) * D + lane * 8 : nullptr;
+            dst[u] = vec < vectors && out != nullptr ? out + ((row0 + r) * p.kv_heads + head) * D + lane * 8 : nullptr;
             scale[u] = 0.0f;
             if (dst[u] == nullptr) continue;
             const int64_t vector = at.place + static_cast<int64_t>(head) * p.page_size;
