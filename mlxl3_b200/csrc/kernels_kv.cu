@@ -13,7 +13,10 @@
 // rounds, unless it lies on it.  4-bit codes are stored as code + 8, the even dimension in the low half of the byte.
 //
 // Both kernels are bound by memory (and short calls by the chain row_start -> length -> page table -> data): 16 or 8 lanes hold a
-// vector, 8 dimensions each, so that every access is 16 bytes (8 or 4 for codes) and a vector one coalesced piece.
+// vector, 8 dimensions each, so that every access is 16 bytes (8 or 4 for codes) and a vector one coalesced piece.  Three prompts of 6674
+// rows, 32 heads over 8 of 128, fp16: 37 us, 68 % of the measured copy rate; with the angles read from shared memory for every vector
+// and four rows one after the other 83 us.  4000 rows into 4 bits: 50 us, bound by the instructions of the 64-bit path (four CTAs per
+// SM; three 63 with the reading back where four take 58).  60001 rows out of 4 bits: 61.5 us, 77 %.
 #include <algorithm>
 #include <type_traits>
 

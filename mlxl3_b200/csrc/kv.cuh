@@ -18,14 +18,6 @@ __device__ __forceinline__ int kv_clamp_row(const KvArgs& p, int r) {
 }
 __device__ __forceinline__ int kv_clamp_length(int n) { return n < 0 ? 0 : (n > kKvMaxTokens ? kKvMaxTokens : n); }
 
-__device__ __forceinline__ KvSeq kv_seq(const KvArgs& p, int b) {
-    KvSeq s;
-    s.first_row = kv_clamp_row(p, __ldg(p.row_start + b));
-    s.n = max(0, kv_clamp_row(p, __ldg(p.row_start + b + 1)) - s.first_row);
-    s.first_pos = kv_clamp_length(__ldg(p.length + b)) - s.n;
-    return s;
-}
-
 __device__ __forceinline__ int kv_page_index(const KvArgs& p, int pos) {
     return p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
 }

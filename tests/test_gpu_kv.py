@@ -405,6 +405,47 @@ def test_attention_scales_of_any_magnitude(gpu):
         attend(s, 4, q_factor=1.0 / k_size)
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+def test_attention_more_sequences_than_shared_memory_names(gpu, bits):
+    rng = np.random.default_rng(31)
+    few = Setup([(1, int(n)) for n in rng.integers(1, 40, 150)], F16, bits, 1, 64, 16, seed=31)
+    attend(few, 2, max_new=1)
+    many = Setup([(int(n), int(n) + 3) for n in rng.integers(0, 6, 530)], BF16, bits, 1, 64, 16, seed=32)
+    attend(many, 4, max_new=6)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_scales_that_bulk_copies_cannot_read(gpu, bits):
+    # scale arrays that lie on 4 bytes only: every key goes the slow way
+    s = Setup([(1, 200), (30, 170)], F16, bits, 2, 128, 32, seed=33)
+    for name in "kv":
+        buf = s.Buffer(s.scale[name].nbytes + 16)
+        buf.upload(s.scale[name], offset=4)
+        s.dev_scale[name] = buf
+    s.cache = s.kv.KvCache(s.pages, s.page, s.kv_heads, s.d, s.dtype, s.bits, s.dev["k"].ptr, s.dev["v"].ptr, *(s.dev_scale[n].ptr + 4 for n in "kv"))
+    attend(s, 4)
+    attend(s, 4, max_new=2)
+
+
+def test_attention_pages_outside_the_pool_read_as_zeros(gpu):
+    for bits in (16, 8):
+        s = Setup([(1, 100), (40, 90)], F16, bits, 1, 64, 16, seed=34, spare=2)
+        held = s.held
+        s.table[0, 2], s.table[1, 1] = s.pages + 5, -7
+        s.upload()
+
+        def zeros_there(name, b, t):
+            t = np.asarray(t)
+            x, bad = np.zeros((len(t), 1, 64)), (t // 16 == 2) if b == 0 else (t // 16 == 1)
+            x[~bad] = held(name, b, t[~bad])
+            return x
+        s.held = zeros_there
+        attend(s, 4, max_new=40)
+        s.seqs = s.seqs[:1]
+        s.batch = s.kv.KvBatch(s.d_start.ptr, s.d_length.ptr, s.d_table.ptr, 1, s.width, s.rows)
+        attend(s, 4, max_new=1)
+
+
 def test_attention_shares_a_workspace_and_streams(gpu):
     from mlxl3_b200.runtime import Stream
     a = Setup([(1, 900)], F16, 16, 2, 128, 16, seed=10)

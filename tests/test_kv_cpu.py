@@ -80,7 +80,7 @@ def test_reads_that_are_refused(args, message):
 
 
 @pytest.mark.parametrize("change,message", [
-    (dict(heads=3), "head counts"), (dict(heads=0), "head counts"), (dict(scale=math.nan), "scale"), (dict(window=-1), "window"), (dict(max_new=-1), "new tokens"),
+    (dict(heads=3), "head counts"), (dict(heads=0), "head counts"), (dict(scale=math.nan), "scale"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(window=-1), "window"), (dict(max_new=-1), "new tokens"),
     (dict(d_out=0), "NULL buffer"), (dict(out_stride=8), "cannot lie"), (dict(d_q=BASE + 2), "16-byte aligned"),
     (dict(workspace=Workspace(nbytes=1 << 14)), "workspace too small"), (dict(workspace=Workspace(ptr=0)), "workspace too small"),
     (dict(workspace=Workspace(ptr=BASE + 8)), "16-byte aligned")])
