@@ -560,3 +560,31 @@ def test_decoder_prefill_equals_steps(gpu):
         assert np.abs(after - after_want).max() <= 3e-2 * np.abs(after_want).max()
     with pytest.raises(gpu.B200Exl3Error, match="do not fit"):
         model.prefill(tokens, 30)
+
+
+@pytest.mark.parametrize("pdl", [0, 1, 2])
+def test_chain_of_calls_with_and_without_dependent_launch(gpu, pdl):
+    """append -> attention -> append of the outputs -> read, back to back, for a mixed batch: the same bits whether kernels start early or not."""
+    import mlxl3_b200
+    results = []
+    for option in (0, pdl):
+        s = Setup([(1, 300), (40, 400), (2, 5), (100, 100)], BF16, 8, 2, 64, 16, seed=40, tail=0)
+        up, heads, d = s.Buffer.from_numpy, 4, s.d
+        width = (heads + 4) * d
+        qkv = up(random_rows(np.random.default_rng(41), (s.rows, width), BF16))
+        turns = up(s.kv.rope_turns(64, 10000.0))
+        rope = s.kv.Rope(turns.ptr, 64, True)
+        out, k, v = s.Buffer(s.rows * heads * d * 2), s.Buffer(s.rows * 2 * d * 4), s.Buffer(s.rows * 2 * d * 4)
+        ws = s.kv.new_attention_workspace(s.cache, s.batch, heads)
+        mlxl3_b200.set_option("pdl", option)
+        try:
+            for _ in range(3):
+                s.kv.append(s.cache, s.batch, qkv.ptr + heads * d * 2, qkv.ptr + (heads + 2) * d * 2, rope, qkv.ptr, heads, qkv.ptr, width, width, width, width)
+                s.kv.attention(s.cache, s.batch, qkv.ptr, heads, 0.125, out.ptr, ws, q_stride=width)
+                s.kv.append(s.cache, s.batch, out.ptr, out.ptr + 2 * d * 2, k_stride=heads * d, v_stride=heads * d)
+                s.kv.read(s.cache, s.batch, F32, k.ptr, v.ptr)
+            results.append([b.download((b.nbytes,), np.uint8) for b in (qkv, out, k, v)])
+        finally:
+            mlxl3_b200.set_option("pdl", 0)
+    for a, b in zip(*results):
+        assert np.array_equal(a, b)
