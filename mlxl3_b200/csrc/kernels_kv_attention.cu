@@ -20,6 +20,7 @@
 #include "kv_work.cuh"
 
 #include <algorithm>
+#include <climits>
 
 namespace b200exl3 {
 
@@ -216,7 +217,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     // A lane holds the queries of row 8 b + g; scores, sums and outputs of rows 8 b + 2 t and the next (e = 0, 1).
     uint32_t q[NB][kSteps][2];
     float out[NB][kTiles][4], m[NB][2], l[NB][2], row_scale[NB][2], unit = 0.0f, unit_inverse = 0.0f;
-    int position[NB][2];                                          // -1: no row
+    int key_end[NB][2], key_start[NB][2];                         // keys that a row sees; no row sees them all, so that nothing is masked for it
     auto begin = [&]() {
         const int rows = work.rows_of(get.seq);
         unit = unit_inverse = 0.0f;
@@ -226,7 +227,9 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int r = row0 + 2 * t + e;
-                position[b][e] = r < rows ? get.seq.first_pos + r / work.group : -1;
+                const int position = get.seq.first_pos + r / work.group;
+                key_end[b][e] = r < rows ? min(position + 1, work.capacity) : INT_MAX;
+                key_start[b][e] = r < rows && a.window > 0 ? max(position + 1 - a.window, 0) : 0;
                 m[b][e] = -INFINITY;
                 l[b][e] = 0.0f;
                 row_scale[b][e] = a.scale_log2e;
@@ -353,7 +356,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int end = min(position[b][e] + 1, work.capacity) - first, start = (a.window > 0 ? position[b][e] + 1 - a.window : 0) - first;
+                const int end = key_end[b][e] - first, start = key_start[b][e] - first;
                 if (__any_sync(0xffffffffu, end < S::kStepKeys - 7 || start > 0)) {
 #pragma unroll
                     for (int k = 0; k < kSub; ++k)

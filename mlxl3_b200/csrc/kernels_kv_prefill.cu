@@ -26,6 +26,7 @@
 #include "kv_work.cuh"
 
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 namespace b200exl3 {
@@ -226,10 +227,13 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 here = at;
                 __syncwarp();
                 const int row = here.tile * kManyRows + x * kManyTile + r, n = here.end - here.block;
-                const int position = row < work.rows_of(here.seq) ? here.seq.first_pos + row / work.group : -1;
+                const bool live = row < work.rows_of(here.seq);
+                const int position = here.seq.first_pos + row / work.group;
                 // visible keys from the first block's first one on
                 const int key0 = here.seg.low + here.block * kManyKeys;
-                const int end = min(position + 1, work.capacity) - key0, start = (a.window > 0 ? position + 1 - a.window : 0) - key0;
+                // (no row sees them all, so that nothing is masked for it)
+                const int end = live ? min(position + 1, work.capacity) - key0 : INT_MAX, start = (live && a.window > 0 ? max(position + 1 - a.window, 0) : 0) - key0;
+                const bool idle = !__any_sync(0xffffffffu, live);              // a warp without rows keeps the barriers and nothing else
                 float m = -INFINITY, l = 0.0f, row_scale = a.scale_log2e;
 #pragma unroll 1
                 for (int j = 0; j < n; ++j) {
@@ -360,7 +364,14 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                     l2.get(l0, l1);
                     l += l0 + l1;
                     };
-                    if (__any_sync(0xffffffffu, e < kManyKeys || b > 0)) block(std::true_type{}); else block(std::false_type{});
+                    if (idle) {
+                        mbar_arrive(&p_half[x]);
+                        mbar_arrive(&p_full[x]);
+                    } else if (__any_sync(0xffffffffu, e < kManyKeys || b > 0)) {
+                        block(std::true_type{});
+                    } else {
+                        block(std::false_type{});
+                    }
                 }
                 // ---- the segment's rows, or this CTA's part of them
                 ++segment_count;
