@@ -71,10 +71,8 @@ def test_appends_that_are_refused(change, message):
         append(**change)
 
 
-@pytest.mark.parametrize("args,message", [((F16 + 1, BASE, 0), None), ((7, BASE, BASE), "unsupported dtype"), ((F16, 0, 0), "NULL buffer"), ((F16, BASE + 4, 0), "16-byte aligned")])
+@pytest.mark.parametrize("args,message", [((7, BASE, BASE), "unsupported dtype"), ((F16, 0, 0), "NULL buffer"), ((F16, BASE + 4, 0), "16-byte aligned")])
 def test_reads_that_are_refused(args, message):
-    if message is None:
-        return
     with pytest.raises(_lib.B200Exl3Error, match=message):
         kv.read(cache(), batch(), *args)
 
