@@ -9,8 +9,8 @@
 // 16 bits for the second product.  Loads bound it: what a step of single tokens moves is the cache, once.
 // Both products have the keys and values as their left operand and the rows as their right one, whose tiles are 8 wide: a group of four
 // query heads leaves half of a tile idle where it would leave three quarters of a left one's 16, and scores, outputs and exponentials
-// take half the registers and instructions (long 4-bit contexts 254 -> 208 us; 177 with a third CTA per SM
-// and no masks for rows that pad the tile; 64 ragged sequences of bf16 242 us, 90 % of the measured copy rate).
+// take half the registers and instructions (long 4-bit contexts 254 -> 208 us; 174 with a third CTA per SM
+// and no masks for rows that pad the tile; 64 ragged sequences of bf16 221 us, 98 % of the measured copy rate).
 // A row's maximum moves only when a score exceeds it by 2^8, so that outputs are seldom rescaled and the lanes that share a row seldom
 // have to agree; until then probabilities reach 256, which 16 bits hold as well as 1.
 //
@@ -29,7 +29,9 @@ namespace {
 
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps;
 constexpr int kFewTable = 128;
-constexpr int kFewOver = 1;
+// A segment's queries, its end and its part of a join in units of a block: us of 64 ragged sequences with 0, 1, 3, 5 and 8 of them 262,
+// 243, 225, 221 and 222, of 16 long ones in 4 bits 181, 178, 178, 174 and 175.
+constexpr int kFewOver = 5;
 
 template <int BITS, int D, int NB>
 struct FewShape {

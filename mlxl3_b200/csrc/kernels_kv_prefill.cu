@@ -45,6 +45,8 @@ template <int N> __device__ __forceinline__ void more_registers() { asm volatile
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int kQueryWarp = kSoftmaxWarps + kLoadWarps + 1;         // and two bring the queries
 constexpr int kManyTable = 512;
+// A segment's queries, masks and end in units of a block: us of a prompt of 4096 with 1, 3 and 5 of them 182, 159 and 164, of a mixed step
+// 86, 82 and 85.
 constexpr int kManyOver = 3;
 constexpr uint32_t kScoreCols = 128;               // tensor-memory columns of S_x; P_x lies in their second half
 
