@@ -342,6 +342,8 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             if (__any_sync(0xffffffffu, top > unit)) {
 #pragma unroll
                 for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                // scales below 2^-100 are as good as zero: the unit's inverse stays a number
+                top = fmaxf(top, 7.8886091e-31f);
                 // a quarter more, so that the unit seldom moves; its inverse need not be exact, only the same at the end
                 const float ratio = unit / (1.25f * top);
 #pragma unroll

@@ -1,0 +1,62 @@
+"""GPU tests of the paged key/value cache at the ends of its ranges: magnitudes of keys, values and scales, windows and lengths, numbers that
+are not finite where a row must not see them.  The bars are those of tests/test_gpu_kv.py, with the terms that a test adds written beside it.
+"""
+import numpy as np
+import pytest
+
+from oracle import kv as okv
+from tests.gpu_util import gpu  # noqa: F401
+from tests.test_gpu_kv import BF16, F16, F32, HALF_STEP, Setup, raw, values  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def run_attention(s, heads, q, window=0, max_new=0):
+    """Outputs [rows, heads, d] in 64 bits; the same bits twice, and a clean workspace header."""
+    d_q, d_out = s.Buffer.from_numpy(q), s.Buffer.from_numpy(q)
+    ws = s.kv.new_attention_workspace(s.cache, s.batch, heads, max_new)
+    got = []
+    for _ in range(2):
+        s.kv.attention(s.cache, s.batch, d_q.ptr, heads, s.d ** -0.5, d_out.ptr, ws, max_new, window)
+        got.append(d_out.download(q.shape, np.uint16))
+    assert np.array_equal(*got) and not ws.download((16384,), np.uint8).any()
+    return values(got[0], s.dtype).reshape(s.rows, heads, s.d)
+
+
+def rows_want(s, heads, q, b, window=0):
+    """(rows, what they should hold, the bar without its absolute part, visible keys) of sequence b."""
+    n, length = s.seqs[b]
+    rows = slice(int(s.start[b]), int(s.start[b]) + n)
+    low = max(0, length - n + 1 - window) if window else 0
+    keys, vals = (np.zeros((length, s.kv_heads, s.d)) for _ in range(2))
+    keys[low:], vals[low:] = s.held("k", b, np.arange(low, length)), s.held("v", b, np.arange(low, length))
+    qv = values(q[rows], s.dtype).reshape(n, heads, s.d)
+    want, mass, most, seen, _ = okv.attention(qv, keys, vals, length - n, s.d ** -0.5, window)
+    score = (s.d + 4) * 2.0 ** -23 * most
+    if s.bits != 16:
+        score = score + s.d ** -0.5 * 2.0 ** -24 * np.abs(qv).max(-1) * np.abs(keys).sum(-1).max()
+    product = s.dtype if s.bits == 16 else F16
+    bar = (np.expm1(2 * score) + 2.0 ** -20 + HALF_STEP[product] + seen * 2.0 ** -22)[..., None] * mass
+    bar = bar + HALF_STEP[s.dtype] * (np.abs(want) + bar) + (2.0 ** -25 if s.dtype == F16 else 0.0)
+    return rows, want, bar, seen
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("size", [1e-39, 1e-45])
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_value_scales_without_an_inverse(gpu, bits, size, new):
+    """Scales of the smallest numbers of fp32, some of them zero: over a whole sequence, and ahead of ordinary tokens.  A value scale is held
+    to 2^-96 or better (scales below 2^-100 are as good as zero), times the largest code, for each key."""
+    s = Setup([(new, 130), (new, 40 + new), (new, 300)], BF16, bits, 1, 64, 16, seed=50 + new, tail=0)
+    for b, last in ((0, 130), (1, 40 + new), (2, 70)):
+        t = np.arange(last)
+        at = s.table[b, t // 16], 0, t % 16
+        s.scale["v"][at] = np.where(t % 3 == 1, 0.0, size).astype(np.float32)
+        if b == 1:
+            s.scale["k"][at] = np.where(t % 5 == 1, 0.0, s.scale["k"][at])
+    s.upload()
+    q = raw(s.rng.standard_normal((s.rows, 2 * 64)), BF16)
+    got = run_attention(s, 2, q, max_new=new)
+    for b in range(3):
+        rows, want, bar, seen = rows_want(s, 2, q, b)
+        assert (np.abs(got[rows] - want) <= bar + (seen * okv.LIMIT[bits] * 2.0 ** -96)[..., None]).all()
