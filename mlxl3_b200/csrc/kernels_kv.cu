@@ -9,7 +9,7 @@
 //
 // A quantised cache holds a vector x as codes round(x m / max|x|), m = 127 or 7, and one fp32 scale max|x| / m.  The rotated k is kept
 // in 64 bits up to the code: between two codes a last bit of fp32 decides, and every element of a long cache gets its chance at it.
-// v needs no more than fp32: x m is exact there and the quotient of two 16-bit values is never closer to a border than that division
+// v needs no more than fp32: x m is exact there (from 2^100 on after a step of powers of two) and the quotient of two 16-bit values is never closer to a border than that division
 // rounds, unless it lies on it.  4-bit codes are stored as code + 8, the even dimension in the low half of the byte.
 //
 // Both kernels are bound by memory (and short calls by the chain row_start -> length -> page table -> data): 16 or 8 lanes hold a
@@ -106,11 +106,13 @@ __device__ __forceinline__ void kv_quantise(const F (&x)[8], uint32_t (&words)[2
     const bool sound = top > 0 && top < static_cast<F>(INFINITY);
     const F inverse = sound ? kv_divide(static_cast<F>(M), top) : static_cast<F>(0), near = static_cast<F>(0.5) - (sizeof(F) == 4 ? static_cast<F>(1e-4) : static_cast<F>(1e-9));
     const bool small = inverse > static_cast<F>(sizeof(F) == 4 ? 1e38 : 1e300);       // the inverse of a subnormal: every quotient itself
+    // a quotient near such a middle is that of two large numbers, where x M would leave the type: both smaller, exactly
+    const F down = sizeof(F) == 4 && top > static_cast<F>(1.2676506e30) ? static_cast<F>(0.00390625) : static_cast<F>(1);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         F off;
         int code = kv_nearest(small ? static_cast<F>(0) : x[i] * inverse, off);
-        if (sound && (small || fabs(off) > near)) code = kv_nearest(kv_divide(x[i] * static_cast<F>(M), top), off);
+        if (sound && (small || fabs(off) > near)) code = kv_nearest(kv_divide(x[i] * down * static_cast<F>(M), top * down), off);
         if (!sound) code = 0;
         if constexpr (BITS == 8) words[i >> 2] |= static_cast<uint32_t>(code & 0xff) << (8 * (i & 3));
         else words[0] |= static_cast<uint32_t>(code + 8) << (4 * i);

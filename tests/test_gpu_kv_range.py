@@ -60,3 +60,27 @@ def test_value_scales_without_an_inverse(gpu, bits, size, new):
     for b in range(3):
         rows, want, bar, seen = rows_want(s, 2, q, b)
         assert (np.abs(got[rows] - want) <= bar + (seen * okv.LIMIT[bits] * 2.0 ** -96)[..., None]).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_codes_of_the_largest_values(gpu, bits):
+    """bf16 vectors up to the largest number of the type, half of the largest (a middle between two codes: the even one) among them: equal codes."""
+    rng = np.random.default_rng(51)
+    s = Setup([(64, 64)], BF16, bits, 1, 128, 16, seed=51, tail=0)
+    x = rng.standard_normal((64, 128)) * 2.0 ** rng.integers(96, 126, (64, 1))
+    top = (1.0 + rng.integers(0, 128, 64) / 128.0) * 2.0 ** rng.integers(96, 128, 64)
+    x = np.clip(x, -top[:, None], top[:, None])
+    x[:, 3], x[:, 7], x[:, 11] = top, top / 2, -top / 2
+    x[0, 3:12] = 2.0 ** 127, 2.0 ** 126, -2.0 ** 126, 2.0 ** 125, 1.5 * 2.0 ** 126, 0.0, 1.0, 2.0 ** 119, 2.0 ** 120
+    stored = raw(x, BF16)
+    x = values(stored, BF16)
+    assert np.isfinite(x).all()
+    d_x = s.Buffer.from_numpy(stored)
+    s.kv.append(s.cache, s.batch, d_x.ptr, d_x.ptr)
+    pool, scale = s.download()
+    codes, want_scale = okv.quantise(x, bits)
+    t = np.arange(64)
+    at = s.table[0, t // 16], 0, t % 16
+    for name in "kv":
+        assert np.array_equal(okv.unpack(pool[name][at], bits), codes)
+        assert (np.abs(scale[name][at].astype(np.float64) - want_scale) <= 2.0 ** -23 * want_scale).all()
