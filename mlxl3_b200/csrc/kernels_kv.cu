@@ -9,8 +9,9 @@
 //
 // A quantised cache holds a vector x as codes round(x m / max|x|), m = 127 or 7, and one fp32 scale max|x| / m.  The rotated k is kept
 // in 64 bits up to the code: between two codes a last bit of fp32 decides, and every element of a long cache gets its chance at it.
-// v needs no more than fp32: x m is exact there (from 2^100 on after a step of powers of two) and the quotient of two 16-bit values is never closer to a border than that division
-// rounds, unless it lies on it.  4-bit codes are stored as code + 8, the even dimension in the low half of the byte.
+// v needs no more than fp32: x m is exact there (from 2^100 on after a step by a power of two) and the quotient of two 16-bit values is
+// never closer to a border than that division rounds, unless it lies on it.  4-bit codes are stored as code + 8, the even dimension in the
+// low half of the byte.
 //
 // Both kernels are bound by memory (and short calls by the chain row_start -> length -> page table -> data): 16 or 8 lanes hold a
 // vector, 8 dimensions each, so that every access is 16 bytes (8 or 4 for codes) and a vector one coalesced piece.  Three prompts of 6674

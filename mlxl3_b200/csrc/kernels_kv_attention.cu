@@ -130,7 +130,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         const int first = at.seg.low + block * S::kKeys;
         // Lane i looks up the i-th part of the block: a tensor copy where every key of it is a token that some row of the sequence
         // sees (and so holds numbers), row by row with zeros where not.
-        const int low = a.window > 0 ? max(0, at.seq.first_pos + 1 - a.window) : 0;
+        const int low = kv_seen_first(at.seq.first_pos, a.window);
         const int high = min(at.seq.first_pos + min(at.seq.n, a.max_new), work.capacity);
         int64_t from = -1;
         if (lane < parts) {
@@ -231,8 +231,8 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             for (int e = 0; e < 2; ++e) {
                 const int r = row0 + 2 * t + e;
                 const int position = get.seq.first_pos + r / work.group;
-                key_end[b][e] = r < rows ? min(position + 1, work.capacity) : INT_MAX;
-                key_start[b][e] = r < rows && a.window > 0 ? max(position + 1 - a.window, 0) : 0;
+                key_end[b][e] = r < rows ? kv_seen_end(position, work.capacity) : INT_MAX;
+                key_start[b][e] = r < rows ? kv_seen_first(position, a.window) : 0;
                 m[b][e] = -INFINITY;
                 l[b][e] = 0.0f;
                 row_scale[b][e] = a.scale_log2e;

@@ -235,7 +235,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 // visible keys from the first block's first one on
                 const int key0 = here.seg.low + here.block * kManyKeys;
                 // (no row sees them all, so that nothing is masked for it)
-                const int end = live ? min(position + 1, work.capacity) - key0 : INT_MAX, start = (live && a.window > 0 ? max(position + 1 - a.window, 0) : 0) - key0;
+                const int end = live ? kv_seen_end(position, work.capacity) - key0 : INT_MAX, start = (live ? kv_seen_first(position, a.window) : 0) - key0;
                 const bool idle = !__any_sync(0xffffffffu, live);              // a warp without rows keeps the barriers and nothing else
                 float m = -INFINITY, l = 0.0f, row_scale = a.scale_log2e;
 #pragma unroll 1
@@ -508,7 +508,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             const int slot = tile % S::kSlots, first = at.seg.low + block * kManyKeys;
             // Lane i looks up the i-th part of the block: a tensor copy where every key of it is a token that some row of the sequence
             // sees (and so holds numbers), row by row with zeros where not.
-            const int low = a.window > 0 ? max(0, at.seq.first_pos + 1 - a.window) : 0;
+            const int low = kv_seen_first(at.seq.first_pos, a.window);
             const int high = min(at.seq.first_pos + min(at.seq.n, a.max_new), work.capacity);
             int64_t from = -1;
             if (lane < parts) {

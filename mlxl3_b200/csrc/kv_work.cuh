@@ -20,6 +20,10 @@ struct KvSegment {
     int key0, key1;        // visible keys
 };
 
+// Keys that the row at `position` sees: first .. end - 1.  A sequence with more rows than tokens begins before position 0; any window.
+__device__ __forceinline__ int kv_seen_end(int position, int capacity) { return min(max(position + 1, 0), capacity); }
+__device__ __forceinline__ int kv_seen_first(int position, int window) { return window > 0 ? max(max(position + 1, 0) - window, 0) : 0; }
+
 // Sequences whose first rows and lengths a CTA keeps in shared memory; more are read where they are.
 template <int CAP>
 struct KvTable {
@@ -69,8 +73,8 @@ struct KvWork {
         const int rows = min(s.n, a.max_new) * group;
         g.first = tile * ROWS / group;
         g.last = (min(rows, (tile + 1) * ROWS) - 1) / group;
-        g.key1 = max(0, min(s.first_pos + g.last + 1, capacity));
-        g.key0 = a.window > 0 ? max(0, s.first_pos + g.first + 1 - a.window) : 0;
+        g.key1 = kv_seen_end(s.first_pos + g.last, capacity);
+        g.key0 = kv_seen_first(s.first_pos + g.first, a.window);
         g.low = g.key0 / KEYS * KEYS;
         g.blocks = max(1, (g.key1 - g.low + KEYS - 1) / KEYS);
         return g;

@@ -24,19 +24,20 @@ def run_attention(s, heads, q, window=0, max_new=0):
 
 
 def rows_want(s, heads, q, b, window=0):
-    """(rows, what they should hold, the bar without its absolute part, visible keys) of sequence b."""
+    """(rows, what they should hold, the bar, visible keys) of sequence b."""
     n, length = s.seqs[b]
     rows = slice(int(s.start[b]), int(s.start[b]) + n)
     low = max(0, length - n + 1 - window) if window else 0
     keys, vals = (np.zeros((length, s.kv_heads, s.d)) for _ in range(2))
     keys[low:], vals[low:] = s.held("k", b, np.arange(low, length)), s.held("v", b, np.arange(low, length))
     qv = values(q[rows], s.dtype).reshape(n, heads, s.d)
-    want, mass, most, seen, _ = okv.attention(qv, keys, vals, length - n, s.d ** -0.5, window)
+    want, mass, most, seen, top_v = okv.attention(qv, keys, vals, length - n, s.d ** -0.5, window)
     score = (s.d + 4) * 2.0 ** -23 * most
     if s.bits != 16:
-        score = score + s.d ** -0.5 * 2.0 ** -24 * np.abs(qv).max(-1) * np.abs(keys).sum(-1).max()
+        score = score + s.d ** -0.5 * 2.0 ** -24 * np.abs(qv).max(-1) * np.abs(keys).sum(-1).max(initial=0.0)
     product = s.dtype if s.bits == 16 else F16
     bar = (np.expm1(2 * score) + 2.0 ** -20 + HALF_STEP[product] + seen * 2.0 ** -22)[..., None] * mass
+    bar = bar + (2.0 ** -25 * seen * top_v if product == F16 else 0.0 * seen)[..., None]
     bar = bar + HALF_STEP[s.dtype] * (np.abs(want) + bar) + (2.0 ** -25 if s.dtype == F16 else 0.0)
     return rows, want, bar, seen
 
@@ -84,3 +85,17 @@ def test_codes_of_the_largest_values(gpu, bits):
     for name in "kv":
         assert np.array_equal(okv.unpack(pool[name][at], bits), codes)
         assert (np.abs(scale[name][at].astype(np.float64) - want_scale) <= 2.0 ** -23 * want_scale).all()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("seqs", [[(8, 3), (1, 5)], [(40, 30), (130, 4), (2, 0)]])
+def test_windows_beyond_every_length(gpu, bits, seqs):
+    """A window of the largest int hides nothing, also for rows ahead of their sequence's first token."""
+    s = Setup(seqs, F16, bits, 1, 64, 16, seed=52, tail=0)
+    q = raw(s.rng.standard_normal((s.rows, 2 * 64)), F16)
+    open_end = run_attention(s, 2, q)
+    for window in (2 ** 31 - 1, 2 ** 30, 200):
+        assert np.array_equal(run_attention(s, 2, q, window), open_end)
+    for b in range(len(seqs)):
+        rows, want, bar, seen = rows_want(s, 2, q, b)
+        assert (np.abs(open_end[rows] - want) <= bar).all()
