@@ -136,14 +136,24 @@ __device__ __forceinline__ void codes4_in_order(uint32_t w, uint32_t (&v)[4]) {
     }
 }
 
-// Wait that gives up after about a quarter of a second of polls, or at once when another role has; inlined, since the register split
-// leaves no room for a call.
-__device__ __forceinline__ void many_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+// What the waits of a CTA share: whether one has given up, and the block that the products are at.
+struct ManyState {
+    int failed, block;
+};
+// Wait that gives up when the products have stood still for about a quarter of a second, or at once when another role has given up: the
+// second tile's rows wait through all segments of one tile ahead of theirs.  Inlined, since the register split leaves no room for a call.
+__device__ __forceinline__ void many_wait(uint64_t* bar, uint32_t parity, volatile ManyState* state) {
     if (mbar_try_wait(bar, parity)) return;
-    const unsigned long long t0 = global_ns();
+    unsigned long long t0 = global_ns();
+    int at = state->block;
     while (!mbar_try_wait_for(bar, parity, 20000)) {
-        if (*failed) return;
-        if (global_ns() - t0 > 250000000ull) *failed = 1;
+        if (state->failed) return;
+        if (state->block != at) {
+            at = state->block;
+            t0 = global_ns();
+        } else if (global_ns() - t0 > 250000000ull) {
+            state->failed = 1;
+        }
     }
 }
 
@@ -168,7 +178,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     __shared__ float s_top[S::kScaleBlocks], s_q_scale[2][BITS != 16 && !std::is_same_v<T, __half> ? kManyRows : 1];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int s_last[2];
-    __shared__ volatile int s_failed;
+    __shared__ volatile ManyState s_state;
 
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
     const Work work(p, a, s_table);
@@ -183,7 +193,8 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 2); mbar_init(&p_half[x], kManyTile); mbar_init(&p_full[x], kManyTile); mbar_init(&o_full[x], 1); mbar_init(&q_full[x], 1); mbar_init(&q_free[x], 1); }
         mbar_init(&drained, 1);
         for (int i = 0; i < S::kScaleBlocks; ++i) mbar_init(&scales_full[i], 2);
-        s_failed = 0;
+        s_state.failed = 0;
+        s_state.block = 0;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncwarp();
@@ -241,13 +252,13 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
 #pragma unroll 1
                 for (int j = 0; j < n; ++j) {
                     const int e = end - j * kManyKeys, b = start - j * kManyKeys;      // visible: columns b .. e - 1
-                    many_wait(&s_full[x], s_par, &s_failed);
+                    many_wait(&s_full[x], s_par, &s_state);
                     s_par ^= 1u;
                     const int kept = (block_count + j) % S::kScaleBlocks;      // the block's scales
                     const float* const key_scales = block_scales + kept * 2 * kManyKeys;
                     // written with the queries; two segments' worth, so that the next one's do not overtake a row
                     if (!std::is_same_v<T, M> && j == 0) row_scale = s_q_scale[segment_count & 1][x * kManyTile + r];
-                    if constexpr (BITS != 16) many_wait(&scales_full[kept], ((block_count + j) / S::kScaleBlocks) & 1, &s_failed);
+                    if constexpr (BITS != 16) many_wait(&scales_full[kept], ((block_count + j) / S::kScaleBlocks) & 1, &s_state);
                     __syncwarp();
                     fence_after();
                     if (j + 1 == n) {
@@ -412,7 +423,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 };
                 const float inverse = kv_inverse(l);
                 float4* const mine = whole ? nullptr : reinterpret_cast<float4*>(part_of(blockIdx.x)) + pr;      // [four results][row]
-                many_wait(&o_full[x], o_par, &s_failed);
+                many_wait(&o_full[x], o_par, &s_state);
                 o_par ^= 1u;
                 __syncwarp();
                 fence_after();
@@ -517,7 +528,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             }
             const uint32_t whole = __ballot_sync(0xffffffffu, from >= 0);
             if (tile >= S::kSlots) {
-                many_wait(&kv_free[slot], (tile / S::kSlots - 1) & 1u, &s_failed);
+                many_wait(&kv_free[slot], (tile / S::kSlots - 1) & 1u, &s_state);
                 __syncwarp();
             }
             const uint32_t dst = tile_base + slot * S::kTileBytes;
@@ -590,7 +601,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 }
                 if (lane == 0) mbar_expect_tx(&raw_full[slot], static_cast<uint32_t>(__popc(whole) * box_rows * (kRowBytes + 4)));
                 __syncwarp();
-                many_wait(&raw_full[slot], (tile / S::kSlots) & 1u, &s_failed);
+                many_wait(&raw_full[slot], (tile / S::kSlots) & 1u, &s_state);
                 __syncwarp();
                 if (w & 1) {
                     float top = fmaxf(fmaxf(scales[lane], scales[lane + 32]), fmaxf(scales[lane + 64], scales[lane + 96]));
@@ -657,7 +668,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         int tile = 0;                                             // tiles consumed
         uint32_t p_par[2] = {0, 0}, q_par[2] = {0, 0};
         auto wait_tile = [&](int i) {
-            many_wait(&kv_full[i % S::kSlots], (i / S::kSlots) & 1u, &s_failed);
+            many_wait(&kv_full[i % S::kSlots], (i / S::kSlots) & 1u, &s_state);
             fence_after();
         };
         auto score = [&](int x, int slot) {
@@ -675,7 +686,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             const uint64_t vd = v_desc + slot * (S::kTileBytes >> 4);
 #pragma unroll
             for (int h = 1; h >= 0; --h) {
-                many_wait(h ? &p_half[x] : &p_full[x], p_par[x], &s_failed);
+                many_wait(h ? &p_half[x] : &p_full[x], p_par[x], &s_state);
                 fence_after();
 #pragma unroll
                 for (int k = h * (kManyKeys / 32); k < (h + 1) * (kManyKeys / 32); ++k)
@@ -689,7 +700,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             const bool two = rows - at.tile * kManyRows > kManyTile;
             wait_tile(tile);
             for (int x = 0; x < (two ? 2 : 1); ++x) {
-                many_wait(&q_full[x], q_par[x], &s_failed);
+                many_wait(&q_full[x], q_par[x], &s_state);
                 q_par[x] ^= 1u;
                 fence_after();
                 score(x, tile % S::kSlots);
@@ -722,10 +733,11 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 }
                 if (more) umma_commit(&kv_free[kt % S::kSlots]);
                 tile += 2;
+                s_state.block = tile;
             }
         } while (at.next_segment(work));
         umma_commit(&drained);
-        many_wait(&drained, 0, &s_failed);
+        many_wait(&drained, 0, &s_state);
         } else if (warp == kQueryWarp || warp == kQueryWarp + 1) {
             // ================= queries of a tile: neighbouring lanes a row; rows past the last are zeros =================
             const int x = warp - kQueryWarp, lane = threadIdx.x & 31, chunk = lane % kChunks;
@@ -743,7 +755,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 const T* const base = static_cast<const T*>(a.q) + (at.seq.first_row + token0) * a.q_stride +
                                       static_cast<int64_t>(at.head * work.group) * D + chunk * 8;
                 // the products of this tile's segment before have read their queries
-                if (loaded > 0) many_wait(&q_free[x], (loaded - 1) & 1, &s_failed);
+                if (loaded > 0) many_wait(&q_free[x], (loaded - 1) & 1, &s_state);
                 __syncwarp();
                 auto source = [&](int q, bool live) {             // row q of the tile
                     // (past + q) / group: half a row away from where fp32 could round it over an edge
@@ -803,7 +815,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         __syncwarp();
         tmem_dealloc(tmem, 512);
     }
-    if (threadIdx.x == 0 && s_failed) atomicExch(a.error, 8u);
+    if (threadIdx.x == 0 && s_state.failed) atomicExch(a.error, 8u);
 }
 
 template <typename T, int BITS, int D>

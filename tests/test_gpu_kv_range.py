@@ -99,3 +99,35 @@ def test_windows_beyond_every_length(gpu, bits, seqs):
     for b in range(len(seqs)):
         rows, want, bar, seen = rows_want(s, 2, q, b)
         assert (np.abs(open_end[rows] - want) <= bar).all()
+
+
+def test_second_tile_waits_through_a_long_run(gpu):
+    """Half a second of sequences of one tile, every CTA's run without a break, and behind them one of two tiles: its second tile's rows have
+    waited since the call began.  The long ones share a page of equal tokens: every output is their value."""
+    from mlxl3_b200 import kv
+    from mlxl3_b200.runtime import DeviceBuffer
+    length, long_ones, rows, d = 1 << 20, 6400, 33, 64
+    last = Setup([(70, 300)], F16, 8, 1, d, 512, seed=53, tail=0)
+    ends = []                                            # the last sequence's page lies behind the long ones' in pools of its own
+    for name in "kv":
+        pool, scale = DeviceBuffer(2 * length * d), DeviceBuffer.from_numpy(np.ones(2 * length, np.float32))
+        pool.fill(1)
+        pool.upload(last.pool[name][last.table[0, 0], 0], offset=length * d)
+        scale.upload(last.scale[name][last.table[0, 0], 0], offset=length * 4)
+        ends.append((pool, scale))
+    start = np.concatenate((np.arange(long_ones + 1) * rows, [long_ones * rows + 70])).astype(np.int32)
+    lengths = np.array([length] * long_ones + [300], np.int32)
+    table = np.array([0] * long_ones + [1], np.int32)
+    q = raw(last.rng.standard_normal((int(start[-1]), 2 * d)), F16)
+    d_start, d_lengths, d_table, d_q = (DeviceBuffer.from_numpy(x) for x in (start, lengths, table, q))
+    out = DeviceBuffer(q.nbytes)
+    cache = kv.KvCache(2, length, 1, d, F16, 8, ends[0][0].ptr, ends[1][0].ptr, ends[0][1].ptr, ends[1][1].ptr)
+    batch = kv.KvBatch(d_start.ptr, d_lengths.ptr, d_table.ptr, long_ones + 1, 1, int(start[-1]))
+    ws = kv.new_attention_workspace(cache, batch, 2, 70)
+    kv.attention(cache, batch, d_q.ptr, 2, d ** -0.5, out.ptr, ws, 70)
+    got = values(out.download(q.shape, np.uint16), F16)
+    assert not ws.download((16384,), np.uint8).any()
+    assert (np.abs(got[:long_ones * rows] - 1.0) <= 2.0 ** -11).all()       # half a step and the sum over 2^20 equal keys
+    last.start = last.start + long_ones * rows
+    at, want, bar, _ = rows_want(last, 2, q, 0)
+    assert (np.abs(got[at].reshape(70, 2, d) - want) <= bar).all()
