@@ -136,24 +136,24 @@ __device__ __forceinline__ void codes4_in_order(uint32_t w, uint32_t (&v)[4]) {
     }
 }
 
-// What the waits of a CTA share: whether one has given up, and the block that the products are at.
+// What the waits of a CTA share: whether one has given up, and when the products last began a block.
 struct ManyState {
-    int failed, block;
+    uint32_t failed, clock;
 };
-// Wait that gives up when the products have stood still for about a quarter of a second, or at once when another role has given up: the
-// second tile's rows wait through all segments of one tile ahead of theirs.  Inlined, since the register split leaves no room for a call.
+__device__ __forceinline__ uint32_t cycles() {
+    uint32_t c;
+    asm volatile("mov.u32 %0, %%clock;" : "=r"(c));
+    return c;
+}
+// Wait that gives up when the products have stood still for 2^29 cycles (about a third of a second), or at once when another role has given
+// up: the second tile's rows wait through all segments of one tile ahead of theirs.  Inlined, since the register split leaves no room
+// for a call.
 __device__ __forceinline__ void many_wait(uint64_t* bar, uint32_t parity, volatile ManyState* state) {
     if (mbar_try_wait(bar, parity)) return;
-    unsigned long long t0 = global_ns();
-    int at = state->block;
     while (!mbar_try_wait_for(bar, parity, 20000)) {
         if (state->failed) return;
-        if (state->block != at) {
-            at = state->block;
-            t0 = global_ns();
-        } else if (global_ns() - t0 > 250000000ull) {
-            state->failed = 1;
-        }
+        const uint32_t since = state->clock;
+        if (static_cast<int32_t>(cycles() - since) > 1 << 29) state->failed = 1;
     }
 }
 
@@ -194,7 +194,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         mbar_init(&drained, 1);
         for (int i = 0; i < S::kScaleBlocks; ++i) mbar_init(&scales_full[i], 2);
         s_state.failed = 0;
-        s_state.block = 0;
+        s_state.clock = cycles();
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncwarp();
@@ -733,7 +733,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 }
                 if (more) umma_commit(&kv_free[kt % S::kSlots]);
                 tile += 2;
-                s_state.block = tile;
+                s_state.clock = cycles();
             }
         } while (at.next_segment(work));
         umma_commit(&drained);
