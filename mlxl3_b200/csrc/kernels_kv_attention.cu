@@ -15,9 +15,8 @@
 // have to agree; until then probabilities reach 256, which 16 bits hold as well as 1.
 //
 // Codes are multiplied as they are: 8- and 4-bit codes are exact in fp16, and so is what the tensor cores add up in fp32; the key's
-// scale multiplies its scores, the value's its probability.  Those probabilities are taken relative to the largest value scale met so
-// far (`unit`), so that rounding them to fp16 costs 2^-11 of what they weigh whatever the scales' magnitude.  bf16 queries enter fp16
-// multiplied by a power of two of their own (exact but for what lies 2^-24 below the row's largest).
+// scale multiplies its scores, the value's its probability, relative to the largest such term of the row (kv_work.cuh).  bf16 queries
+// enter fp16 multiplied by a power of two of their own (exact but for what lies 2^-24 below the row's largest).
 #include "kv_work.cuh"
 
 #include <algorithm>
@@ -219,11 +218,10 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     // ---- state of a segment ---------------------------------------------------------------------------------------------
     // A lane holds the queries of row 8 b + g; scores, sums and outputs of rows 8 b + 2 t and the next (e = 0, 1).
     uint32_t q[NB][kSteps][2];
-    float out[NB][kTiles][4], m[NB][2], l[NB][2], row_scale[NB][2], unit = 0.0f, unit_inverse = 0.0f;
+    float out[NB][kTiles][4], m[NB][2], l[NB][2], row_scale[NB][2];
     int key_end[NB][2], key_start[NB][2];                         // keys that a row sees; no row sees them all, so that nothing is masked for it
     auto begin = [&]() {
         const int rows = work.rows_of(get.seq);
-        unit = unit_inverse = 0.0f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const int row0 = get.tile * S::kRows + 8 * b;
@@ -322,38 +320,22 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
                 }
             }
         const float* scales = reinterpret_cast<const float*>(smem + stage * S::kStageBytes + 2 * S::kTileBytes) + wrow + g;
-        float vs[kSub][2];
+        float vs[kSub][2], vs_log[kSub][2];
         bool rescale = false;
         float factor[NB][2];                                      // of the outputs so far
 #pragma unroll
         for (int b = 0; b < NB; ++b) factor[b][0] = factor[b][1] = 1.0f;
         if constexpr (BITS != 16) {
-            float top = 0.0f;
 #pragma unroll
             for (int k = 0; k < kSub; ++k)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const float ks = scales[k * 16 + 8 * h];
-                    vs[k][h] = scales[S::kKeys + k * 16 + 8 * h];
-                    top = fmaxf(top, vs[k][h]);
+                    vs[k][h] = scales[S::kKeys + k * 16 + 8 * h] * (1.0f / kScaleUnit);
+                    vs_log[k][h] = kv_scale_log(vs[k][h]);
 #pragma unroll
                     for (int b = 0; b < NB; ++b) { s[k][b][2 * h] *= ks; s[k][b][2 * h + 1] *= ks; }
                 }
-            if (__any_sync(0xffffffffu, top > unit)) {
-#pragma unroll
-                for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                // scales below 2^-100 are as good as zero: the unit's inverse stays a number
-                top = fmaxf(top, 7.8886091e-31f);
-                // a quarter more, so that the unit seldom moves; its inverse need not be exact, only the same at the end
-                const float ratio = unit / (1.25f * top);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) factor[b][0] = factor[b][1] = ratio;
-                unit = 1.25f * top;
-                unit_inverse = 1.0f / unit;
-                rescale = true;
-            }
-#pragma unroll
-            for (int k = 0; k < kSub; ++k) { vs[k][0] *= unit_inverse; vs[k][1] *= unit_inverse; }
         }
         // masks, maximum, probabilities
         const int first = block_key + wrow + g;
@@ -370,9 +352,15 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
                             if (k * 16 + 8 * h >= end || k * 16 + 8 * h < start) s[k][b][2 * h + e] = -INFINITY;
                 }
                 float top = -INFINITY;
+                if constexpr (BITS == 16) {
 #pragma unroll
-                for (int k = 0; k < kSub; ++k) top = fmaxf(top, fmaxf(s[k][b][e], s[k][b][2 + e]));
-                top *= row_scale[b][e];
+                    for (int k = 0; k < kSub; ++k) top = fmaxf(top, fmaxf(s[k][b][e], s[k][b][2 + e]));
+                    top *= row_scale[b][e];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kSub; ++k)
+                        top = fmaxf(top, fmaxf(fmaf(s[k][b][e], row_scale[b][e], vs_log[k][0]), fmaf(s[k][b][2 + e], row_scale[b][e], vs_log[k][1])));
+                }
                 if (__any_sync(0xffffffffu, top > m[b][e] + 8.0f)) {              // also from -inf
 #pragma unroll
                     for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -398,7 +386,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         for (int b = 0; b < NB; ++b) {
             float shift[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) shift[e] = m[b][e] == -INFINITY ? 0.0f : -m[b][e];        // a row that saw nothing yet
+            for (int e = 0; e < 2; ++e) shift[e] = m[b][e] == -INFINITY ? 0.0f : (BITS == 16 ? 0.0f : kLift) - m[b][e];        // a row that saw nothing yet
 #pragma unroll
             for (int k = 0; k < kSub; ++k)
 #pragma unroll
@@ -486,7 +474,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
 #pragma unroll
                     for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) dst[dim_of(i, h)] = BITS == 16 ? out[b][i][2 * h + e] : out[b][i][2 * h + e] * unit;
+                        for (int h = 0; h < 2; ++h) dst[dim_of(i, h)] = out[b][i][2 * h + e];
                 }
             }
         group_sync(1, 32 * kFewWarps);
@@ -512,7 +500,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
                 for (int e = 0; e < kLaneDims; ++e) o[e] = fmaf(src[e], c, o[e]);
             }
             if (c0 == c1) {
-                const float inverse = kv_inverse(sum);
+                const float inverse = kv_inverse(sum) * (BITS == 16 ? 1.0f : kScaleUnit);
 #pragma unroll
                 for (int e = 0; e < kLaneDims; ++e) o[e] *= inverse;
                 store_row(tile0 + r, o);
@@ -567,7 +555,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
                     }
 #pragma unroll
                     for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                    const float inverse = kv_inverse(sum);
+                    const float inverse = kv_inverse(sum) * (BITS == 16 ? 1.0f : kScaleUnit);
 #pragma unroll
                     for (int e = 0; e < kLaneDims; ++e) o[e] *= inverse;
                     store_row(tile0 + r, o);

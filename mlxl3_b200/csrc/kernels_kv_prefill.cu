@@ -14,9 +14,8 @@
 // Four warps bring the data, a tile (a block's keys or values) each in turn, into the 128-byte swizzle that the products read: tensor
 // copies of whole pages or parts of pages where every key of the block is visible, else 16 bytes at a time with zeros for what lies
 // outside the visible range.  One thread issues the products.  Of a quantised cache those warps load the codes and store them as
-// fp16, exactly; the key's scale multiplies its scores and the value's its probability, where m bounds their product (a row's largest
-// score plus log2 of the largest value scale of the blocks so far), so that it fits 16 bits whatever the scales' magnitude.  bf16 queries
-// enter those fp16 products multiplied by a power of two of their own.  Every wait is bounded; one that gives up sets the status word, all
+// fp16, exactly; the key's scale multiplies its scores and the value's its probability, relative to the row's largest such term
+// (kv_work.cuh).  bf16 queries enter those fp16 products multiplied by a power of two of their own.  Every wait is bounded; one that gives up sets the status word, all
 // roles run on to the end, and the kernel frees its tensor memory.
 //
 // What bounds it: for long prompts the chain score product -> softmax -> output product of the two tiles in turn, 3400 cycles a block, of which
@@ -57,8 +56,10 @@ struct ManyShape {
     static constexpr int kQueryBytes = kManyRows * D * 2;
     static constexpr int kStageRow = 80;                           // a row of 32 results on its way out, 64 bytes without bank conflicts
     static constexpr int kStageBytes = kSoftmaxWarps * 32 * kStageRow;
-    static constexpr int kScaleBlocks = 4;                         // blocks whose scales are kept: [key and value scales][128 keys], with codes
-    static constexpr int kScaleBytes = BITS == 16 ? 0 : kScaleBlocks * 2 * kManyKeys * 4;
+    // blocks whose scales are kept, with codes: [key scales, value scales, their logarithms][128 keys].  One more than in flight: a block's
+    // scales are read until the block behind it has its scores, and those free the keys' place of the block that takes the scales' place.
+    static constexpr int kScaleBlocks = kSlots / 2 + 1, kScaleFloats = 3 * kManyKeys;
+    static constexpr int kScaleBytes = BITS == 16 ? 0 : kScaleBlocks * kScaleFloats * 4;
     static constexpr size_t kSmem = 1024 + kQueryBytes + static_cast<size_t>(kSlots) * kTileBytes + kStageBytes + kScaleBytes;
     static constexpr int kPartFloats = kManyRows * (D + 2);
     static constexpr uint32_t kOutCols = 2 * kScoreCols;           // first column of O_0; O_1 lies D further
@@ -122,6 +123,12 @@ __device__ __forceinline__ void scale2(uint32_t& v0, uint32_t& v1, float f0, flo
     v0 = __float_as_uint(x0);
     v1 = __float_as_uint(x1);
 }
+__device__ __forceinline__ void term2(uint32_t& v0, uint32_t& v1, const Pair& by, float a0, float a1) {
+    float x0, x1;
+    fma2(Pair(__uint_as_float(v0), __uint_as_float(v1)), by, Pair(a0, a1)).get(x0, x1);
+    v0 = __float_as_uint(x0);
+    v1 = __float_as_uint(x1);
+}
 
 // Eight 4-bit codes of a word as fp16 in order: the two of a byte go to the halves of a word, as 1024 + u and 1024 + 16 u
 __device__ __forceinline__ void codes4_in_order(uint32_t w, uint32_t (&v)[4]) {
@@ -167,6 +174,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     using Work = KvWork<kManyRows, kManyKeys, kManyOver>;
     using Cursor = KvCursor<kManyRows, kManyKeys, kManyOver>;
     constexpr int kChunks = D / 8;
+    constexpr float kUnit = BITS == 16 ? 1.0f : kScaleUnit;      // of the outputs
     pdl_launch_dependents();
     pdl_wait();
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -175,7 +183,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     // every warp's place, and a row warp's segment at hand: in registers they would push out scores
     __shared__ Cursor s_cursor, s_at[kSoftmaxWarps + kLoadWarps + 3], s_here[kSoftmaxWarps];
     __shared__ __align__(8) uint64_t kv_full[S::kSlots], kv_free[S::kSlots], s_full[2], p_half[2], p_full[2], o_full[2], q_full[2], q_free[2], drained, scales_full[S::kScaleBlocks], raw_full[S::kSlots];
-    __shared__ float s_top[S::kScaleBlocks], s_q_scale[2][BITS != 16 && !std::is_same_v<T, __half> ? kManyRows : 1];
+    __shared__ float s_q_scale[2][BITS != 16 && !std::is_same_v<T, __half> ? kManyRows : 1];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int s_last[2];
     __shared__ volatile ManyState s_state;
@@ -255,7 +263,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                     many_wait(&s_full[x], s_par, &s_state);
                     s_par ^= 1u;
                     const int kept = (block_count + j) % S::kScaleBlocks;      // the block's scales
-                    const float* const key_scales = block_scales + kept * 2 * kManyKeys;
+                    const float* const key_scales = block_scales + kept * S::kScaleFloats;
                     // written with the queries; two segments' worth, so that the next one's do not overtake a row
                     if (!std::is_same_v<T, M> && j == 0) row_scale = s_q_scale[segment_count & 1][x * kManyTile + r];
                     if constexpr (BITS != 16) many_wait(&scales_full[kept], ((block_count + j) / S::kScaleBlocks) & 1, &s_state);
@@ -302,6 +310,16 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
 #pragma unroll 1
                     for (int col = 0; col < kManyKeys; col += kCols) {
                         load(col);
+                        if constexpr (BITS != 16) {               // terms: scores and the logarithms of the values' scales
+                            uint32_t (&v)[32] = v_wide[0];
+                            const Pair scales2(row_scale, row_scale);
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {
+                                const float4 vs_log = *reinterpret_cast<const float4*>(key_scales + 2 * kManyKeys + col + i);
+                                term2(v[i], v[i + 1], scales2, vs_log.x, vs_log.y);
+                                term2(v[i + 2], v[i + 3], scales2, vs_log.z, vs_log.w);
+                            }
+                        }
                         float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
                         for (int h = 0; h < kWide; ++h)
@@ -312,8 +330,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                             }
                         top = fmaxf(top, fmaxf(t0, t1));
                     }
-                    top *= row_scale;
-                    if constexpr (BITS != 16) top += s_top[kept];
+                    if constexpr (BITS == 16) top *= row_scale;
                     bool reload = false;
                     const bool moves = top > m + 8.0f;                           // also from -inf
                     if (__any_sync(0xffffffffu, moves)) {
@@ -341,7 +358,8 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                         }
                     }
                     // from the upper columns down: probabilities go where scores lay that were read before
-                    const Pair scales2(row_scale, row_scale), shift2(m == -INFINITY ? 0.0f : -m, m == -INFINITY ? 0.0f : -m);
+                    const float shift = m == -INFINITY ? 0.0f : (BITS == 16 ? 0.0f : kLift) - m;
+                    const Pair scales2(row_scale, row_scale), shift2(shift, shift);
                     Pair l2(0.0f, 0.0f), l3(0.0f, 0.0f);
 #pragma unroll 1
                     for (int col = kManyKeys - kCols; col >= 0; col -= kCols) {
@@ -421,7 +439,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                         if (dst[i] != nullptr)
                             *reinterpret_cast<uint4*>(dst[i] + c) = *reinterpret_cast<const uint4*>(stage + (i * 8 + lane / 4) * S::kStageRow + (lane & 3) * 16);
                 };
-                const float inverse = kv_inverse(l);
+                const float inverse = kv_inverse(l) * kUnit;
                 float4* const mine = whole ? nullptr : reinterpret_cast<float4*>(part_of(blockIdx.x)) + pr;      // [four results][row]
                 many_wait(&o_full[x], o_par, &s_state);
                 o_par ^= 1u;
@@ -466,7 +484,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                             sum = sum * exp2_fast(top - safe) + ml.y * exp2_fast(ml.x - safe);
                             top = to;
                         }
-                        const float safe = top == -INFINITY ? 0.0f : top, inv = kv_inverse(sum);
+                        const float safe = top == -INFINITY ? 0.0f : top, inv = kv_inverse(sum) * kUnit;
 #pragma unroll 1
                         for (int d = 0; d < D; d += 32) {
                             float o[32];
@@ -569,7 +587,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 constexpr int kRowBytes = D * BITS / 8, kPieces = kRowBytes / 16;
                 const uint32_t raw = dst + S::kTileBytes - kManyKeys * kRowBytes;
                 const int kept = (tile >> 1) % S::kScaleBlocks;
-                float* const scales = block_scales + kept * 2 * kManyKeys + (w & 1) * kManyKeys;
+                float* const scales = block_scales + kept * S::kScaleFloats + (w & 1) * kManyKeys;
                 if (from >= 0) {
                     const int row = static_cast<int>(from) + at.head * p.page_size;
                     tma_rows(raw + lane * box_rows * kRowBytes, w & 1 ? &v_map : &k_map, 0, row, &raw_full[slot]);
@@ -604,11 +622,12 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 many_wait(&raw_full[slot], (tile / S::kSlots) & 1u, &s_state);
                 __syncwarp();
                 if (w & 1) {
-                    float top = fmaxf(fmaxf(scales[lane], scales[lane + 32]), fmaxf(scales[lane + 64], scales[lane + 96]));
 #pragma unroll
-                    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    // values below 2^-100 are as good as zero
-                    if (lane == 0) s_top[kept] = log2f(fmaxf(top, 7.8886091e-31f));
+                    for (int i = lane; i < kManyKeys; i += 32) {
+                        const float vs = scales[i] * (1.0f / kScaleUnit);
+                        scales[i] = vs;
+                        scales[i + kManyKeys] = kv_scale_log(vs);
+                    }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&scales_full[kept]);

@@ -245,6 +245,19 @@ __device__ __forceinline__ float exp2_fast(float x) {             // 2 ulp; exp2
 // 1 / sum of a row; a row that sees nothing is zero
 __device__ __forceinline__ float kv_inverse(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
 
+// Probabilities over a quantised cache: what is rounded to fp16 for the second product is w = 2^(s + kLift - m) vs, the probability times
+// the value's scale, and m bounds s + log2 vs over the keys that the row itself sees.  So a rounding costs 2^-11 of a term, or 2^-32 of the
+// row's largest one, whatever scales other keys have; the largest w lies between 2^kLift and 2^(kLift + 8).  The sum of the probabilities has
+// 2^(s + kLift - m).  So that it fits fp32 for scales at the ends of its range too, they enter as vs / 2^16, and their logarithm is not
+// taken below -88: sums reach 2^(88 + 15) a key, and a largest term of scale 2^125 (4-bit bf16) is 2^-102.  Scales below 2^-96 lose
+// bits, as good as zero.
+constexpr float kLift = 7.0f, kScaleUnit = 65536.0f;
+__device__ __forceinline__ float kv_scale_log(float vs) {         // of a scale in that unit; NaN: the least
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(vs));
+    return fmaxf(y, -88.0f);
+}
+
 // The power of two that brings a row's largest magnitude to [1, 2), and its inverse, in two factors each: all of them are normal numbers.
 struct KvPower {
     float down0, down1, up0, up1;

@@ -23,8 +23,22 @@ def run_attention(s, heads, q, window=0, max_new=0):
     return values(got[0], s.dtype).reshape(s.rows, heads, s.d)
 
 
-def rows_want(s, heads, q, b, window=0):
-    """(rows, what they should hold, the bar, visible keys) of sequence b."""
+def largest_term(s, qv, keys, vals, first_position, scale):
+    """Largest probability times largest |value| of a key, [rows, heads]."""
+    n, heads, _ = qv.shape
+    group, out = heads // s.kv_heads, np.zeros((n, heads))
+    for i in range(n):
+        end = first_position + i + 1
+        for h in range(heads if end > 0 else 0):
+            x = scale * (keys[:end, h // group] @ qv[i, h])
+            p = np.exp(x - x.max())
+            out[i, h] = (p / p.sum() * np.abs(vals[:end, h // group]).max(-1)).max()
+    return out
+
+
+def rows_want(s, heads, q, b, window=0, by_term=False):
+    """(rows, what they should hold, the bar, visible keys) of sequence b.  by_term: fp16 products hold a term, the probability times the
+    value, to 2^-11 of itself or, subnormal, to 2^-25 in a unit of which the row's largest term makes 2^7 at least."""
     n, length = s.seqs[b]
     rows = slice(int(s.start[b]), int(s.start[b]) + n)
     low = max(0, length - n + 1 - window) if window else 0
@@ -37,7 +51,8 @@ def rows_want(s, heads, q, b, window=0):
         score = score + s.d ** -0.5 * 2.0 ** -24 * np.abs(qv).max(-1) * np.abs(keys).sum(-1).max(initial=0.0)
     product = s.dtype if s.bits == 16 else F16
     bar = (np.expm1(2 * score) + 2.0 ** -20 + HALF_STEP[product] + seen * 2.0 ** -22)[..., None] * mass
-    bar = bar + (2.0 ** -25 * seen * top_v if product == F16 else 0.0 * seen)[..., None]
+    small = 2.0 ** -32 * largest_term(s, qv, keys, vals, length - n, s.d ** -0.5) if by_term else 2.0 ** -25 * top_v
+    bar = bar + (seen * small if product == F16 else 0.0 * seen)[..., None]
     bar = bar + HALF_STEP[s.dtype] * (np.abs(want) + bar) + (2.0 ** -25 if s.dtype == F16 else 0.0)
     return rows, want, bar, seen
 
@@ -131,3 +146,38 @@ def test_second_tile_waits_through_a_long_run(gpu):
     last.start = last.start + long_ones * rows
     at, want, bar, _ = rows_want(last, 2, q, 0)
     assert (np.abs(got[at].reshape(70, 2, d) - want) <= bar).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype,d,heads,new", [(BF16, 128, 2, 1), (F16, 64, 2, 5), (BF16, 64, 4, 3), (F16, 128, 2, 40), (BF16, 64, 2, 140)])
+def test_value_scales_that_differ_between_keys(gpu, bits, dtype, d, heads, new):
+    """Value scales 2^20 apart from key to key, the largest on the last tokens, which only the last rows see: every row is held relative to
+    the terms it sees."""
+    s = Setup([(new, 260), (new, 90 + new), (new, 141)], dtype, bits, 1, d, 16, seed=54 + new, tail=0)
+    for b, (_, length) in enumerate(s.seqs):
+        t = np.arange(length)
+        power = np.select([t % 4 == 1, t % 7 == 3], [-20.0, 10.0], 0.0) - 5.0 * b
+        if b < 2:
+            power[-2:] = 12.0
+        at = s.table[b, t // 16], 0, t % 16
+        s.scale["v"][at] *= np.exp2(power).astype(np.float32)
+    s.upload()
+    q = raw(s.rng.standard_normal((s.rows, heads * d)) * 1.5, dtype)
+    got = run_attention(s, heads, q, max_new=new)
+    for b in range(3):
+        rows, want, bar, _ = rows_want(s, heads, q, b, by_term=True)
+        assert (np.abs(got[rows] - want) <= bar).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("power", [118, -70])
+@pytest.mark.parametrize("new", [1, 6, 50])
+def test_value_scales_at_the_ends_of_bf16(gpu, bits, power, new):
+    s = Setup([(new, 300), (new, new + 20)], BF16, bits, 1, 128, 16, seed=55 + new, tail=0)
+    s.scale["v"] *= np.float32(2.0 ** power)
+    s.upload()
+    q = raw(s.rng.standard_normal((s.rows, 2 * 128)) * 1.5, BF16)
+    got = run_attention(s, 2, q, max_new=new)
+    for b in range(2):
+        rows, want, bar, _ = rows_want(s, 2, q, b, by_term=True)
+        assert (np.abs(got[rows] - want) <= bar).all()
