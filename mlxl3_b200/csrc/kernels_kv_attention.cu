@@ -12,7 +12,7 @@
 // take half the registers and instructions (long 4-bit contexts 254 -> 208 us; 174 with a third CTA per SM
 // and no masks for rows that pad the tile; 64 ragged sequences of bf16 221 us, 98 % of the measured copy rate).
 // A row's maximum moves only when a score exceeds it by 2^8, so that outputs are seldom rescaled and the lanes that share a row seldom
-// have to agree; until then probabilities reach 256, which 16 bits hold as well as 1.
+// have to agree; until then they reach 256 times the unit.
 //
 // Codes are multiplied as they are: 8- and 4-bit codes are exact in fp16, and so is what the tensor cores add up in fp32; the key's
 // scale multiplies its scores, the value's its probability, relative to the largest such term of the row (kv_work.cuh).  bf16 queries
@@ -386,7 +386,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         for (int b = 0; b < NB; ++b) {
             float shift[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) shift[e] = m[b][e] == -INFINITY ? 0.0f : (BITS == 16 ? 0.0f : kLift) - m[b][e];        // a row that saw nothing yet
+            for (int e = 0; e < 2; ++e) shift[e] = m[b][e] == -INFINITY ? 0.0f : kLift<M> - m[b][e];        // a row that saw nothing yet
 #pragma unroll
             for (int k = 0; k < kSub; ++k)
 #pragma unroll

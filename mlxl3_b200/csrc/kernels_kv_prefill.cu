@@ -358,7 +358,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                         }
                     }
                     // from the upper columns down: probabilities go where scores lay that were read before
-                    const float shift = m == -INFINITY ? 0.0f : (BITS == 16 ? 0.0f : kLift) - m;
+                    const float shift = m == -INFINITY ? 0.0f : kLift<M> - m;
                     const Pair scales2(row_scale, row_scale), shift2(shift, shift);
                     Pair l2(0.0f, 0.0f), l3(0.0f, 0.0f);
 #pragma unroll 1

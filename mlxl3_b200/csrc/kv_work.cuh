@@ -245,13 +245,17 @@ __device__ __forceinline__ float exp2_fast(float x) {             // 2 ulp; exp2
 // 1 / sum of a row; a row that sees nothing is zero
 __device__ __forceinline__ float kv_inverse(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
 
-// Probabilities over a quantised cache: what is rounded to fp16 for the second product is w = 2^(s + kLift - m) vs, the probability times
-// the value's scale, and m bounds s + log2 vs over the keys that the row itself sees.  So a rounding costs 2^-11 of a term, or 2^-32 of the
-// row's largest one, whatever scales other keys have; the largest w lies between 2^kLift and 2^(kLift + 8).  The sum of the probabilities has
-// 2^(s + kLift - m).  So that it fits fp32 for scales at the ends of its range too, they enter as vs / 2^16, and their logarithm is not
-// taken below -88: sums reach 2^(88 + 15) a key, and a largest term of scale 2^125 (4-bit bf16) is 2^-102.  Scales below 2^-96 lose
-// bits, as good as zero.
-constexpr float kLift = 7.0f, kScaleUnit = 65536.0f;
+// Probabilities are rounded to 16 bits for the second product as 2^(s + lift - m), where m bounds the row's scores so far to within 8.  fp16:
+// from 2^7 to 2^15, so that what lies 2^21 below the largest still has all its bits, and all of a long context's small ones add up (2^-32
+// of the largest at worst).  bf16, whose range is that of fp32: far below one, so that sums of the type's largest values stay finite.
+template <typename M> constexpr float kLift = 7.0f;
+template <> constexpr float kLift<__nv_bfloat16> = -32.0f;
+// Over a quantised cache it is w = 2^(s + lift - m) vs, the probability times the value's scale, and m bounds s + log2 vs over the keys that
+// the row itself sees: a rounding costs 2^-11 of a term, or 2^-32 of the row's largest one, whatever scales other keys have.  The sum of
+// the probabilities has 2^(s + lift - m).  So that it fits fp32 for scales at the ends of its range too, they enter as vs / 2^16, and
+// their logarithm is not taken below -88: sums reach 2^(88 + 15) a key, and a largest term of scale 2^125 (4-bit bf16) is 2^-102.
+// Scales below 2^-96 lose bits, as good as zero.
+constexpr float kScaleUnit = 65536.0f;
 __device__ __forceinline__ float kv_scale_log(float vs) {         // of a scale in that unit; NaN: the least
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(vs));

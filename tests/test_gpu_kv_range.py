@@ -181,3 +181,38 @@ def test_value_scales_at_the_ends_of_bf16(gpu, bits, power, new):
     for b in range(2):
         rows, want, bar, _ = rows_want(s, 2, q, b, by_term=True)
         assert (np.abs(got[rows] - want) <= bar).all()
+
+
+@pytest.mark.parametrize("new,heads", [(1, 4), (30, 2)])
+def test_small_probabilities_of_a_long_context_add_up(gpu, new, heads):
+    """fp16: every sixteenth token takes its share of nearly all of the probability and has no value; the others have 2^-26 of such a share each."""
+    length, d = 20000, 64
+    s = Setup([(new, length)], F16, 16, 1, d, 64, seed=57, tail=0)
+    t = np.arange(length)
+    at = s.table[0, t // 64], 0, t % 64
+    keys, vals = np.zeros((length, d)), s.rng.uniform(500.0, 1000.0, (length, d))
+    keys[5::16, 0], vals[5::16] = 26.0 * np.log(2.0), 0.0
+    s.pool["k"][at], s.pool["v"][at] = raw(keys, F16), raw(vals, F16)
+    s.upload()
+    q = np.zeros((new, heads, d))
+    q[:, :, 0] = d ** 0.5
+    q = raw(q.reshape(new, heads * d), F16)
+    got = run_attention(s, heads, q, max_new=new)
+    rows, want, bar, seen = rows_want(s, heads, q, 0, by_term=True)
+    # a probability to 2^-32 of the largest, which is one of the shares, times the largest value
+    bar = bar + (seen * 2.0 ** -32 * 1000.0 / (length / 16))[..., None]
+    assert (want > 10 * bar).all() and (np.abs(got - want) <= bar).all()
+
+
+@pytest.mark.parametrize("new", [1, 3, 60])
+def test_sums_of_the_largest_bf16_values(gpu, new):
+    s = Setup([(new, 300), (new, new + 1000)], BF16, 16, 1, 64, 16, seed=58, tail=0)
+    for b, (_, length) in enumerate(s.seqs):
+        t = np.arange(length)
+        s.pool["v"][s.table[b, t // 16], 0, t % 16] = raw(s.rng.uniform(0.6, 0.99, (length, 64)) * 2.0 ** 128, BF16)
+    s.upload()
+    q = raw(s.rng.standard_normal((s.rows, 2 * 64)), BF16)
+    got = run_attention(s, 2, q, max_new=new)
+    for b in range(2):
+        rows, want, bar, _ = rows_want(s, 2, q, b)
+        assert (np.abs(got[rows] - want) <= bar).all()
