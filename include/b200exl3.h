@@ -500,8 +500,8 @@ int b200exl3_kv_read(const b200exl3_kv_cache* cache, const b200exl3_kv_batch* ba
 /* out[row, h] = sum_j softmax_j(scale * q[row, h] . k_j) v_j over the tokens j up to the row's own, with window > 0 the last `window` of
  * them; heads / kv_heads query heads share a key head; the row's own token has been appended before.  A row that sees no token is
  * zero.  max_new bounds the rows of one sequence (rows beyond it are not computed; 0 = `rows`): it chooses the kernel, so say 1 for a
- * step of single tokens.  Tokens that no row of a sequence sees are never used whatever they hold; the others have to be finite.
- * scale > 0.  Parts are joined in the order of the keys: a call gives the same bits every time, but where keys are cut depends on the
+ * step of single tokens.  A row takes nothing from tokens that it does not see, whatever they hold; one that sees an infinity or NaN is
+ * not finite there.  scale > 0.  Parts are joined in the order of the keys: a call gives the same bits every time, but where keys are cut depends on the
  * whole batch.  The workspace follows the rules of the linear layer's (header of zeros; one call at a time; status 8 = a wait gave up). */
 int b200exl3_kv_attention_workspace_bytes(const b200exl3_kv_cache* cache, int heads, int64_t max_new, size_t* out_bytes);
 int b200exl3_kv_attention(const b200exl3_kv_cache* cache, const b200exl3_kv_batch* batch, const void* d_q, int64_t q_stride, int heads,

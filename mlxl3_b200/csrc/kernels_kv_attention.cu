@@ -12,7 +12,7 @@
 // take half the registers and instructions (long 4-bit contexts 254 -> 208 us; 174 with a third CTA per SM
 // and no masks for rows that pad the tile; 64 ragged sequences of bf16 221 us, 98 % of the measured copy rate).
 // A row's maximum moves only when a score exceeds it by 2^8, so that outputs are seldom rescaled and the lanes that share a row seldom
-// have to agree; until then they reach 256 times the unit.
+// have to agree; what probabilities then reach is in kv_work.cuh.
 //
 // Codes are multiplied as they are: 8- and 4-bit codes are exact in fp16, and so is what the tensor cores add up in fp32; the key's
 // scale multiplies its scores, the value's its probability, relative to the largest such term of the row (kv_work.cuh).  bf16 queries
@@ -20,6 +20,7 @@
 #include "kv_work.cuh"
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 
 namespace b200exl3 {
@@ -86,8 +87,9 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     return d;
 }
 
-// box_rows: rows of a tensor copy, a power of two that divides the page size, or 0: no tensor copies
-template <typename T, int BITS, int D, int NB>
+// box_rows: rows of a tensor copy, a power of two that divides the page size, or 0: no tensor copies.  SEVERAL: sequences may have more
+// than one row, and so rows that do not see what others do.
+template <typename T, int BITS, int D, int NB, bool SEVERAL>
 __global__ void __launch_bounds__(kFewThreads, FewShape<BITS, D, NB>::kCtas)
 kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const KvArgs p, const KvAttentionArgs a,
               const int box_rows) {
@@ -106,13 +108,14 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     __shared__ float2 s_ml[kFewWarps][S::kRows];
     __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages];
     __shared__ bool s_last;
-    __shared__ volatile int s_failed;
+    __shared__ volatile int s_failed, s_odd;                      // s_odd: numbers were taken out of values
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     unsigned char* const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     if (threadIdx.x == 0) {
         // a block is there when its tensor copies are (lane 0 says how many bytes) and every lane's own copies
         for (int i = 0; i < S::kStages; ++i) { mbar_init(&full[i], 33); mbar_init(&empty[i], kFewWarps); }
         s_failed = 0;
+        s_odd = 0;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     const Work work(p, a, s_table);
@@ -130,7 +133,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         // Lane i looks up the i-th part of the block: a tensor copy where every key of it is a token that some row of the sequence
         // sees (and so holds numbers), row by row with zeros where not.
         const int low = kv_seen_first(at.seq.first_pos, a.window);
-        const int high = min(at.seq.first_pos + min(at.seq.n, a.max_new), work.capacity);
+        const int high = work.any_end(at.seq);
         int64_t from = -1;
         if (lane < parts) {
             const int key = first + lane * box_rows;
@@ -283,6 +286,36 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         }
     };
 
+    // An infinity or NaN among the values of a token would reach the rows that do not see it as 0 times itself: it is taken out of the
+    // warp's keys before the product, and added at the segment's end for the rows that see it.
+    auto look_through = [&](uint32_t values, int wrow, int block_key) {
+        constexpr int kStep = 32 / S::kChunks;
+        const int chunk = lane % S::kChunks, row0 = lane / S::kChunks;
+        uint32_t sum = 0;
+#pragma unroll 4
+        for (int r = row0; r < S::kStepKeys; r += kStep) {
+            uint32_t w[4];
+            shared_load4(values + tile_at<S::kChunks, S::kKeys>(wrow + r, chunk), w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) kv_look<T>(sum, w[j]);
+        }
+        if (__builtin_expect(!__any_sync(0xffffffffu, kv_found(sum)), 1)) return;
+        const int all0 = work.all_first(get.seq, get.seg) - block_key, all1 = work.all_end(get.seq, get.seg) - block_key;
+#pragma unroll 1
+        for (int r = wrow + row0; r < wrow + S::kStepKeys; r += kStep) {
+            if (r >= all0 && r < all1) continue;
+            const uint32_t place = values + tile_at<S::kChunks, S::kKeys>(r, chunk);
+            uint32_t w[4];
+            shared_load4(place, w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = kv_without(w[j], kv_not_finite<T>(w[j]));
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        }
+        s_odd = 1;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the place goes back to the tensor copies
+        __syncwarp();
+    };
+
     // ---- a step of a warp's keys ----------------------------------------------------------------------------------------
     auto multiply = [&](int stage, int wrow, int block_key) {
         const uint32_t keys = base + stage * S::kStageBytes, values = keys + S::kTileBytes;
@@ -330,21 +363,27 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             for (int k = 0; k < kSub; ++k)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float ks = scales[k * 16 + 8 * h];
+                    float ks = scales[k * 16 + 8 * h];
                     vs[k][h] = scales[S::kKeys + k * 16 + 8 * h] * (1.0f / kScaleUnit);
                     vs_log[k][h] = kv_scale_log(vs[k][h]);
+                    if (SEVERAL) {                                // a scale that is not finite makes the scores of its key NaN, for the rows that see it
+                        ks = fmaf(vs[k][h], 0.0f, ks);
+                        vs[k][h] = fminf(vs[k][h], FLT_MAX / kScaleUnit);
+                    }
 #pragma unroll
                     for (int b = 0; b < NB; ++b) { s[k][b][2 * h] *= ks; s[k][b][2 * h + 1] *= ks; }
                 }
         }
         // masks, maximum, probabilities
         const int first = block_key + wrow + g;
+        bool hidden = false;                                      // some row does not see some key; the same for all lanes
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int end = key_end[b][e] - first, start = key_start[b][e] - first;
                 if (__any_sync(0xffffffffu, end < S::kStepKeys - 7 || start > 0)) {
+                    hidden = true;
 #pragma unroll
                     for (int k = 0; k < kSub; ++k)
 #pragma unroll
@@ -381,6 +420,8 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
                     out[b][i][0] *= factor[b][0]; out[b][i][1] *= factor[b][1]; out[b][i][2] *= factor[b][0]; out[b][i][3] *= factor[b][1];
                 }
         }
+        if constexpr (BITS == 16)
+            if (SEVERAL && hidden && work.several(get.seq)) look_through(values, wrow, block_key);
         uint32_t pr[kSub][NB][2];                                 // probabilities as the right operand: keys 2t, 2t + 1 (+ 8) of row g
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -457,6 +498,26 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
             v[0] = f.x; v[1] = f.y;
         }
     };
+    // what was taken out of this CTA's blocks, where row r of the segment's sequence sees it (from the first such number on all segments
+    // are gone through)
+    auto add_odd = [&](int r, float (&o)[kLaneDims]) {
+        const int position = get.seq.first_pos + r / work.group, all0 = work.all_first(get.seq, get.seg), all1 = work.all_end(get.seq, get.seg);
+        const int end = min(get.seg.low + get.end * S::kKeys, kv_seen_end(position, work.capacity));
+#pragma unroll 1
+        for (int key = max(get.seg.low + get.block * S::kKeys, kv_seen_first(position, a.window)); key < end; ++key) {
+            if (key >= all0 && key < all1) key = all1;
+            const int64_t place = key < end ? kv_place(p, get.b, key) : -1;
+            if (place < 0) continue;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.v) + (place + static_cast<int64_t>(get.head) * p.page_size) * D) + lane * (kLaneDims / 2);
+#pragma unroll
+            for (int e = 0; e < kLaneDims; e += 2) {
+                const uint32_t w = __ldg(src + e / 2), top_bits = kv_not_finite<T>(w);
+                const float2 f = KvType<T>::unpack(w);
+                if (top_bits & 0x8000u) o[e] += f.x;
+                if (top_bits & 0x80000000u) o[e + 1] += f.y;
+            }
+        }
+    };
     auto finish = [&](int stage) {
         float* const merge = reinterpret_cast<float*>(smem + (S::kMergeInStage ? stage : S::kStages) * S::kStageBytes);      // [row][warp of its keys][dimension]
         const int tile0 = get.tile * S::kRows, rows_here = min(S::kRows, work.rows_of(get.seq) - tile0);
@@ -499,6 +560,8 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
 #pragma unroll
                 for (int e = 0; e < kLaneDims; ++e) o[e] = fmaf(src[e], c, o[e]);
             }
+            if constexpr (BITS == 16)
+                if (SEVERAL && __builtin_expect(s_odd, 0)) add_odd(tile0 + r, o);
             if (c0 == c1) {
                 const float inverse = kv_inverse(sum) * (BITS == 16 ? 1.0f : kScaleUnit);
 #pragma unroll
@@ -600,20 +663,25 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
     if (threadIdx.x == 0 && s_failed) atomicExch(a.error, 8u);
 }
 
-template <typename T, int BITS, int D, int NB>
-cudaError_t launch_few(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t stream) {
+template <typename T, int BITS, int D, int NB, bool SEVERAL>
+cudaError_t launch_few_rows(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t stream) {
     using S = FewShape<BITS, D, NB>;
     static PerDeviceOnce attribute;
     if (attribute.needed()) {
-        cudaError_t e = cudaFuncSetAttribute(kv_few_kernel<T, BITS, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
+        cudaError_t e = cudaFuncSetAttribute(kv_few_kernel<T, BITS, D, NB, SEVERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
         if (e != cudaSuccess) return e;
         attribute.mark();
     }
     CUtensorMap k_map{}, v_map{};
     int box_rows = 0;
     if (!kv_tensor_maps(p, S::kKeys, &k_map, &v_map, &box_rows)) box_rows = 0;
-    return launch_dependent(kv_few_kernel<T, BITS, D, NB>, dim3(static_cast<unsigned>(S::kCtas * sm_count())), dim3(kFewThreads), S::kSmem, stream,
+    return launch_dependent(kv_few_kernel<T, BITS, D, NB, SEVERAL>, dim3(static_cast<unsigned>(S::kCtas * sm_count())), dim3(kFewThreads), S::kSmem, stream,
                             k_map, v_map, p, a, box_rows);
+}
+
+template <typename T, int BITS, int D, int NB>
+cudaError_t launch_few(const KvArgs& p, const KvAttentionArgs& a, cudaStream_t stream) {
+    return a.max_new > 1 ? launch_few_rows<T, BITS, D, NB, true>(p, a, stream) : launch_few_rows<T, BITS, D, NB, false>(p, a, stream);
 }
 
 // Up to this many rows per key head the few-row kernel takes a sequence.

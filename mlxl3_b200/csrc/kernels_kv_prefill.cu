@@ -7,22 +7,26 @@
 // operand.  The two tiles share the block's keys and values and take turns: while the tensor cores multiply for one, the other's
 // exponentials are computed.  Tensor memory: S_0, S_1, O_0, O_1.
 //
-// The running maximum m of a row is moved only when a score exceeds it by 2^8 (in log2 units 8): until then probabilities may reach
-// 256, which 16 bits hold as well as 1, and O_x and the sum stay in the same unit.  When it moves, the row's thread rescales O_x in
-// tensor memory; S_x of a block being complete implies that the product before it is, so nothing else has to be waited for.
+// The running maximum m of a row is moved only when a score exceeds it by 2^8 (in log2 units 8): until then O_x and the sum stay in the
+// same unit, and probabilities in the range of their type (kv_work.cuh).  When it moves, the row's thread rescales O_x in tensor memory;
+// S_x of a block being complete implies that the product before it is, so nothing else has to be waited for.
 //
 // Four warps bring the data, a tile (a block's keys or values) each in turn, into the 128-byte swizzle that the products read: tensor
 // copies of whole pages or parts of pages where every key of the block is visible, else 16 bytes at a time with zeros for what lies
 // outside the visible range.  One thread issues the products.  Of a quantised cache those warps load the codes and store them as
 // fp16, exactly; the key's scale multiplies its scores and the value's its probability, relative to the row's largest such term
-// (kv_work.cuh).  bf16 queries enter those fp16 products multiplied by a power of two of their own.  Every wait is bounded; one that gives up sets the status word, all
-// roles run on to the end, and the kernel frees its tensor memory.
+// (kv_work.cuh).  bf16 queries enter those fp16 products multiplied by a power of two of their own.  Every wait is bounded; one that gives up
+// sets the status word, all roles run on to the end, and the kernel frees its tensor memory.
+//
+// Values of blocks that not all rows of a segment see whole are looked through for infinities and NaN by the row threads, between their
+// probabilities and the product (why: kernels_kv_attention.cu).  A mixed step with two such blocks a segment took 83 us without and takes 88,
+// the prompt 175 and 176; with the look by a warp of its own ahead of the products they took 91 and 178.
 //
 // What bounds it: for long prompts the chain score product -> softmax -> output product of the two tiles in turn, 3400 cycles a block, of which
 // the products need 2864 (a step of K = 16 takes 105 cycles with both operands in shared memory, 74 with the left one in tensor
-// memory; the pipe's own time is 64), under the power cap.  4096 tokens, 32 heads of 128 over 8, fp16: 159 to 176 us.  Segments of one
-// tile leave the other idle (their blocks dealt to both pipelines gained 4 %): 16 draft tokens of 8 sequences, five heads to a key head,
-// 8 bits: 99 us.
+// memory; the pipe's own time is 64), under the power cap.  4096 tokens, 32 heads of 128 over 8, fp16: 176 us.  Segments of one tile leave
+// the other idle (their blocks dealt to both pipelines gained 4 %): 16 draft tokens of 8 sequences, five heads to a key head, 8 bits:
+// 102 us.
 #include "kv_work.cuh"
 
 #include <algorithm>
@@ -91,6 +95,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
           "=r"(r[31])
         : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]),
@@ -187,6 +197,9 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     __shared__ uint32_t tmem_base_slot;
     __shared__ int s_last[2];
     __shared__ volatile ManyState s_state;
+    // blocks of a row warp's segment at hand with keys that some rows see and others do not: below the first number and from the second on
+    __shared__ int2 s_partly[kSoftmaxWarps];
+    __shared__ volatile int s_odd;                                // numbers were taken out of such blocks' values
 
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
     const Work work(p, a, s_table);
@@ -198,11 +211,12 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kSlots; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], 1); mbar_init(&raw_full[s], 1); }
-        for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 2); mbar_init(&p_half[x], kManyTile); mbar_init(&p_full[x], kManyTile); mbar_init(&o_full[x], 1); mbar_init(&q_full[x], 1); mbar_init(&q_free[x], 1); }
+        for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 2); mbar_init(&p_half[x], kManyTile); mbar_init(&p_full[x], kManyTile); mbar_init(&o_full[x], 2); mbar_init(&q_full[x], 1); mbar_init(&q_free[x], 1); }
         mbar_init(&drained, 1);
         for (int i = 0; i < S::kScaleBlocks; ++i) mbar_init(&scales_full[i], 2);
         s_state.failed = 0;
         s_state.clock = cycles();
+        s_odd = 0;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncwarp();
@@ -243,10 +257,53 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             }
         };
         settle();
+        // The values of the block j of the segment at hand.  The look goes over all of them: fewer instructions, whose misses are its time.
+        auto look_through = [&](int j) {
+            const int vt = 2 * (block_count + j) + 1;
+            constexpr int kStep = kManyTile / kChunks;            // a multiple of eight rows: the swizzle is the same
+            const int chunk = r % kChunks, row0 = r / kChunks;
+            uint32_t at_row = smem_addr(tiles) + vt % S::kSlots * S::kTileBytes + many_at(kManyKeys, row0, chunk);
+            many_wait(&kv_full[vt % S::kSlots], (vt / S::kSlots) & 1u, &s_state);
+            uint32_t sum = 0, sum2 = 0;
+#pragma unroll 1
+            for (int k = 0; k < kManyKeys; k += 2 * kStep, at_row += 2 * kStep * 128) {
+                uint32_t v[4], w[4];
+                shared_load4(at_row, v);
+                shared_load4(at_row + kStep * 128, w);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { kv_look<T>(sum, v[i]); kv_look<T>(sum2, w[i]); }
+            }
+            if (__builtin_expect(kv_found(sum | sum2), 0)) {
+                s_odd = 1;                                        // before the other tile's threads may find nothing left
+                __threadfence_block();
+                const int first = here.seg.low + (here.block + j) * kManyKeys;
+                const int all0 = work.all_first(here.seq, here.seg) - first, all1 = work.all_end(here.seq, here.seg) - first;
+                at_row -= kManyKeys * 128;
+#pragma unroll 1
+                for (int k = row0; k < kManyKeys; k += kStep, at_row += kStep * 128) {
+                    uint32_t v[4];
+                    if (k >= all0 && k < all1) continue;          // all rows see it
+                    shared_load4(at_row, v);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = kv_without(v[i], kv_not_finite<T>(v[i]));
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at_row), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            __syncwarp();
+        };
         while (more) {
             {
                 block_count = next_count;
                 here = at;
+                if constexpr (BITS == 16) {
+                    if (elect_one()) {
+                        const int first = at.seg.low + at.block * kManyKeys;
+                        s_partly[warp] = work.several(at.seq) ? make_int2((work.all_first(at.seq, at.seg) - first + kManyKeys - 1) / kManyKeys,
+                                                                          (work.all_end(at.seq, at.seg) - first) / kManyKeys)
+                                                              : make_int2(0, INT_MAX);
+                    }
+                }
                 __syncwarp();
                 const int row = here.tile * kManyRows + x * kManyTile + r, n = here.end - here.block;
                 const bool live = row < work.rows_of(here.seq);
@@ -271,8 +328,13 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                     fence_after();
                     if (j + 1 == n) {
                         next_count = block_count + n;
-                        more = next_segment(at);
+                                more = next_segment(at);
                         settle();
+                    }
+                    bool partly = false;                          // some rows of the segment see keys of the block that others do not
+                    if constexpr (BITS == 16) {
+                        const int2 blocks = s_partly[warp];
+                        partly = j < blocks.x || j >= blocks.y;
                     }
                     // the block in two forms, with and without hidden columns: a test between loads and arithmetic costs a sixth of the time
                     auto block = [&](auto with_hidden) {
@@ -379,6 +441,10 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                                     const float2 vs = *reinterpret_cast<const float2*>(key_scales + kManyKeys + col + 32 * h + 2 * i);
                                     x0 *= vs.x;
                                     x1 *= vs.y;
+                                    if (kMasked) {                // whatever the scale of a hidden key is
+                                        if (v[2 * i] == 0xff800000u) x0 = 0.0f;
+                                        if (v[2 * i + 1] == 0xff800000u) x1 = 0.0f;
+                                    }
                                 }
                                 p2[i] = KvType<M>::pack(x0, x1);
                             }
@@ -388,7 +454,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                         if ((col & 32) == 0) {                        // a half is there
                             tmem_wait_st();
                             fence_before();
-                            mbar_arrive(col == 0 ? &p_full[x] : &p_half[x]);
+                            if (BITS != 16 || !partly) mbar_arrive(col == 0 ? &p_full[x] : &p_half[x]);
                         }
                     }
                     l2 = add2(l2, l3);
@@ -397,12 +463,19 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                     l += l0 + l1;
                     };
                     if (idle) {
-                        mbar_arrive(&p_half[x]);
-                        mbar_arrive(&p_full[x]);
+                        partly = true;
                     } else if (__any_sync(0xffffffffu, e < kManyKeys || b > 0)) {
                         block(std::true_type{});
                     } else {
                         block(std::false_type{});
+                    }
+                    if (partly) {
+                        // An infinity or NaN among the values of a token would reach the rows that do not see it as 0 times itself.  So the
+                        // tile's threads look through such values before the product gets them; what they take out is added at the
+                        // segment's end for the rows that see it.
+                        if (BITS == 16 && (j < s_partly[warp].x || j >= s_partly[warp].y)) look_through(j);
+                        mbar_arrive(&p_half[x]);
+                        mbar_arrive(&p_full[x]);
                     }
                 }
                 // ---- the segment's rows, or this CTA's part of them
@@ -445,6 +518,39 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 o_par ^= 1u;
                 __syncwarp();
                 fence_after();
+                if (BITS == 16 && __builtin_expect(s_odd, 0)) {
+                    // values that were taken out of this CTA's blocks come back for the rows that see them (all such: from the first one on
+                    // every segment is gone through)
+                    const int row = here.tile * kManyRows + x * kManyTile + r, position = here.seq.first_pos + row / work.group;
+                    const int low = max(here.seg.low + here.block * kManyKeys, kv_seen_first(position, a.window));
+                    const int high = row < work.rows_of(here.seq) ? min(here.seg.low + here.end * kManyKeys, kv_seen_end(position, work.capacity)) : low;
+                    const int all0 = work.all_first(here.seq, here.seg), all1 = work.all_end(here.seq, here.seg);
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        __syncwarp();
+                        uint32_t o[16];
+                        tmem_ld16(outs + c, o);
+                        tmem_wait_ld();
+#pragma unroll 1
+                        for (int key = low; key < high; ++key) {
+                            if (key >= all0 && key < all1) key = all1;            // rows of the tile as it was
+                            const int64_t place = key < high ? kv_place(p, here.b, key) : -1;
+                            if (place < 0) continue;
+                            const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.v) +
+                                                                                    (place + static_cast<int64_t>(here.head) * p.page_size) * D + c);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const uint32_t w = __ldg(src + i), top_bits = kv_not_finite<T>(w);
+                                const float2 f = KvType<T>::unpack(w);
+                                if (top_bits & 0x8000u) o[2 * i] = __float_as_uint(__uint_as_float(o[2 * i]) + f.x);
+                                if (top_bits & 0x80000000u) o[2 * i + 1] = __float_as_uint(__uint_as_float(o[2 * i + 1]) + f.y);
+                            }
+                        }
+                        __syncwarp();
+                        tmem_st16(outs + c, o);
+                        tmem_wait_st();
+                    }
+                }
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     uint32_t v[32];
@@ -538,7 +644,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
             // Lane i looks up the i-th part of the block: a tensor copy where every key of it is a token that some row of the sequence
             // sees (and so holds numbers), row by row with zeros where not.
             const int low = kv_seen_first(at.seq.first_pos, a.window);
-            const int high = min(at.seq.first_pos + min(at.seq.n, a.max_new), work.capacity);
+            const int high = work.any_end(at.seq);
             int64_t from = -1;
             if (lane < parts) {
                 const int key = first + lane * box_rows;
@@ -639,7 +745,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         const uint32_t from_at = raw + tile_at<kPieces, kManyKeys>((t0 + u) * kAtOnce + sub, piece);
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(words[u][0]), "=r"(words[u][1]), "=r"(words[u][2]), "=r"(words[u][3]) : "r"(from_at) : "memory");
+                        shared_load4(from_at, words[u]);
                     }
                     __syncwarp();
 #pragma unroll
@@ -737,6 +843,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                     if (j + 2 == n) umma_commit(&q_free[0]);
                 } else {
                     umma_commit(&o_full[0]);
+                    mbar_arrive(&o_full[0]);                    // and passes on what the rows took out
                 }
                 if (two) {
                     weigh(1, vt % S::kSlots, j > 0);
@@ -746,6 +853,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                         if (j + 2 == n) umma_commit(&q_free[1]);
                     } else {
                         umma_commit(&o_full[1]);
+                        mbar_arrive(&o_full[1]);                    // and passes on what the rows took out
                     }
                 } else {
                     umma_commit(&kv_free[vt % S::kSlots]);

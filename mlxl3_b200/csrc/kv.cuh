@@ -34,6 +34,8 @@ __device__ __forceinline__ int64_t kv_place(const KvArgs& p, int b, int pos) {
 
 template <typename T> struct KvType;
 template <> struct KvType<__half> {
+    using Two = __half2;
+    static constexpr uint32_t kExponent = 0x7c007c00u, kExponentStep = 0x04000400u;
     static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
@@ -41,11 +43,27 @@ template <> struct KvType<__half> {
     }
 };
 template <> struct KvType<__nv_bfloat16> {
+    using Two = __nv_bfloat162;
+    static constexpr uint32_t kExponent = 0x7f807f80u, kExponentStep = 0x00800080u;
     static __device__ __forceinline__ float2 unpack(uint32_t w) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w)); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
 };
+// Adds zero times two numbers: a sum that began at zero stays there unless one of them is an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ void kv_look(uint32_t& sum, uint32_t w) {
+    using Two = typename KvType<T>::Two;
+    const uint32_t zero = 0;
+    const Two s = __hfma2(*reinterpret_cast<const Two*>(&w), *reinterpret_cast<const Two*>(&zero), *reinterpret_cast<const Two*>(&sum));
+    sum = *reinterpret_cast<const uint32_t*>(&s);
+}
+__device__ __forceinline__ bool kv_found(uint32_t sum) { return (sum & 0x7fff7fffu) != 0; }
+// The top bit of each of two numbers that is an infinity or NaN: one step more than the largest exponent.
+template <typename T>
+__device__ __forceinline__ uint32_t kv_not_finite(uint32_t w) { return ((w & KvType<T>::kExponent) + KvType<T>::kExponentStep) & 0x80008000u; }
+// The two numbers with zeros in those places
+__device__ __forceinline__ uint32_t kv_without(uint32_t w, uint32_t top_bits) { return w & ~((top_bits >> 15) * 0xffffu); }
 
 }  // namespace b200exl3

@@ -67,6 +67,11 @@ struct KvWork {
         const int rows = min(s.n, a.max_new) * group;
         return rows >= a.least_rows && rows <= a.most_rows ? rows : 0;
     }
+    // Keys that some row of a sequence sees end here; whether its rows see different keys; keys that all rows of a segment see
+    __device__ __forceinline__ int any_end(const KvSeq& s) const { return min(s.first_pos + min(s.n, a.max_new), capacity); }
+    __device__ __forceinline__ bool several(const KvSeq& s) const { return min(s.n, a.max_new) > 1; }
+    __device__ __forceinline__ int all_first(const KvSeq& s, const KvSegment& g) const { return kv_seen_first(s.first_pos + g.last, a.window); }
+    __device__ __forceinline__ int all_end(const KvSeq& s, const KvSegment& g) const { return kv_seen_end(s.first_pos + g.first, capacity); }
     __device__ __forceinline__ int tiles_of(const KvSeq& s) const { return (rows_of(s) + ROWS - 1) / ROWS; }
     __device__ __forceinline__ KvSegment segment(const KvSeq& s, int tile) const {
         KvSegment g;
@@ -280,6 +285,9 @@ __device__ __forceinline__ void copy16_fill(uint32_t dst, const void* src, bool 
 }
 __device__ __forceinline__ void copy4_fill(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void shared_load4(uint32_t src, uint32_t (&w)[4]) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }

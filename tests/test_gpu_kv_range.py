@@ -216,3 +216,52 @@ def test_sums_of_the_largest_bf16_values(gpu, new):
     for b in range(2):
         rows, want, bar, _ = rows_want(s, 2, q, b)
         assert (np.abs(got[rows] - want) <= bar).all()
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("dtype,d,heads,kv_heads,page,window,seqs", [
+    (F16, 128, 2, 1, 16, 0, [(4, 70), (3, 3), (1, 90), (2, 300)]), (BF16, 64, 4, 2, 32, 20, [(8, 200), (5, 129), (1, 40)]),
+    (BF16, 128, 5, 1, 7, 0, [(3, 66), (2, 130)]), (F16, 64, 2, 2, 64, 0, [(40, 300), (9, 9), (130, 130), (1, 50)]),
+    (BF16, 128, 4, 1, 16, 0, [(300, 400), (33, 200), (7, 700)]), (F16, 128, 2, 1, 24, 50, [(150, 500), (20, 140)]),
+    (BF16, 64, 4, 4, 64, 90, [(130, 400)] * 40 + [(3, 60)] * 7), (F16, 128, 3, 3, 128, 0, [(200, 256), (140, 140), (11, 128)] * 20)])
+def test_tokens_that_are_not_finite_reach_only_the_rows_that_see_them(gpu, bits, dtype, d, heads, kv_heads, page, window, seqs):
+    """Infinities and NaN in tokens that some rows of a sequence see: the other rows have the same bits as without, and so have the other
+    dimensions of the rows that see a value of them."""
+    s = Setup(seqs, dtype, bits, kv_heads, d, page, seed=59, tail=0, window=window)
+    q = raw(s.rng.standard_normal((s.rows, heads * d)), dtype)
+    most = max(n for n, _ in seqs)
+    plain = run_attention(s, heads, q, window, most)
+    kept = {n: v.copy() for n, v in (s.pool if bits == 16 else s.scale).items()}
+    for name in "vk":
+        sees = np.zeros((s.rows, 3), bool)                # by kind: +inf, NaN, -inf (codes: +inf, NaN, +inf)
+        for b, (n, length) in enumerate(seqs):
+            first = length - n
+            # the last token, one that half of the rows see, and with a window the first one, which only the first row sees
+            tokens = [(length - 1, 0), (first + n // 2, 1)] + ([(first + 1 - window, 2)] if window and first + 1 > window else [])
+            for t, kind in tokens:
+                number = (np.inf, np.nan, -np.inf)[kind]
+                at = s.table[b, t // page], slice(None), t % page
+                if bits == 16:
+                    s.pool[name][at + (5 + kind,)] = raw(np.array([number]), dtype)[0]
+                else:
+                    s.scale[name][at] = abs(number)
+                for i in range(n):
+                    if first + i >= t and (not window or first + i - t < window):
+                        sees[int(s.start[b]) + i, kind] = True
+        s.upload()
+        got = run_attention(s, heads, q, window, most)
+        any_of = sees.any(1)
+        assert any_of.any() and np.array_equal(got[~any_of], plain[~any_of])
+        if bits == 16 and name == "v":
+            others = np.ones(d, bool)
+            others[5:8] = False
+            assert np.array_equal(got[:, :, others], plain[:, :, others])
+            for kind in range(3):
+                assert np.array_equal(got[~sees[:, kind], :, 5 + kind], plain[~sees[:, kind], :, 5 + kind])
+                assert not np.isfinite(got[sees[:, kind], :, 5 + kind]).any()
+        elif name == "v":
+            assert not np.isfinite(got[any_of]).any()
+        else:                                             # an infinite key may score -inf, which is a probability of zero
+            assert np.isnan(got[sees[:, 1]]).all()
+        for n, v in kept.items():
+            (s.pool if bits == 16 else s.scale)[n][:] = v
