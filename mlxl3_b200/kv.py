@@ -33,6 +33,7 @@ class KvCache(ctypes.Structure):
                 buf = DeviceBuffer(nbytes)
                 buf.fill(0)
                 self._owned.append(buf)
+            DEFAULT_STREAM.sync()                # calls on other streams do not wait for it
             d_k, d_v, d_k_scale, d_v_scale = ([b.ptr for b in self._owned] + [0, 0])[:4]
         super().__init__(d_k, d_v, d_k_scale, d_v_scale, pages, page_size, kv_heads, head_dim, dtype, bits)
 
