@@ -330,12 +330,13 @@ class DenseDecoder:
         if tokens.ndim != 1 or n == 0 or pos < 0 or pos + n > c.max_ctx:
             raise _lib.B200Exl3Error("prompt tokens do not fit the context")
         if self._chunk is None or self._chunk["rows"] < n:
-            self._chunk = {name: DeviceBuffer(n * w * 2) for name, w in (
+            chunk = {name: DeviceBuffer(n * w * 2) for name, w in (
                 ("h", c.hidden), ("xn", c.hidden), ("q", self.heads * c.head_dim), ("k", self.kv_heads * c.head_dim), ("v", self.kv_heads * c.head_dim),
                 ("att", self.heads * c.head_dim), ("o", c.hidden), ("gate", self.ffn), ("up", self.ffn), ("down", c.hidden))}
             ops = [e[name] for e in self.layers for name in ("qkv", "o", "gu", "down")]
-            self._chunk.update(rows=n, tokens=DeviceBuffer(n * 4), ws=new_workspace(max(op.workspace_bytes(n) for op in ops)),
-                               seq=DeviceBuffer.from_numpy(np.zeros(8, np.int32)), turns=DeviceBuffer.from_numpy(kv.rope_turns(c.head_dim, c.theta)))
+            chunk.update(rows=n, tokens=DeviceBuffer(n * 4), ws=new_workspace(max(op.workspace_bytes(n) for op in ops)),
+                         seq=DeviceBuffer.from_numpy(np.zeros(8, np.int32)), turns=DeviceBuffer.from_numpy(kv.rope_turns(c.head_dim, c.theta)))
+            self._chunk = chunk                           # whole or not at all
         b = self._chunk
         caches = [kv.KvCache(1, c.max_ctx, self.kv_heads, c.head_dim, F16, 16, e["k_cache"].ptr, e["v_cache"].ptr) for e in self.layers]
         if b.get("attn_rows", 0) < n:

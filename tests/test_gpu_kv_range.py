@@ -265,3 +265,26 @@ def test_tokens_that_are_not_finite_reach_only_the_rows_that_see_them(gpu, bits,
             assert np.isnan(got[sees[:, 1]]).all()
         for n, v in kept.items():
             (s.pool if bits == 16 else s.scale)[n][:] = v
+
+
+def test_prefill_after_an_allocation_that_failed(gpu, monkeypatch):
+    from mlxl3_b200 import decoder
+    config = decoder.DecoderConfig(layers=1, hidden=256, heads=2, kv_heads=1, head_dim=128, ffn=512, vocab=512, k_bits=4, codebook=0, max_ctx=32)
+    model = decoder.DenseDecoder(config, decoder.SyntheticWeights(config, seed=3))
+    model.store_logits = True
+    tokens = np.arange(20, dtype=np.int32)
+    model.prefill(tokens[:5])
+    real = decoder.new_workspace
+
+    def out_of_memory(nbytes):
+        raise gpu.B200Exl3Error("out of memory")
+    monkeypatch.setattr(decoder, "new_workspace", out_of_memory)
+    with pytest.raises(gpu.B200Exl3Error, match="out of memory"):
+        model.prefill(tokens)
+    model.prefill(tokens[:5])                            # what was there still is
+    monkeypatch.setattr(decoder, "new_workspace", real)
+    model.prefill(tokens)
+    fresh = decoder.DenseDecoder(config, decoder.SyntheticWeights(config, seed=3))
+    fresh.store_logits = True
+    fresh.prefill(tokens)
+    assert np.array_equal(model.download("logits"), fresh.download("logits"))
