@@ -288,3 +288,51 @@ def test_prefill_after_an_allocation_that_failed(gpu, monkeypatch):
     fresh.store_logits = True
     fresh.prefill(tokens)
     assert np.array_equal(model.download("logits"), fresh.download("logits"))
+
+
+def test_lengths_and_rows_without_sense(gpu):
+    """The largest and smallest lengths, first rows before the buffers: the largest length counts as 2^30 tokens, of which the table's are seen;
+    rows of no sequence, of tokens before the first, and all pages stay as they are."""
+    heads, d = 4, 64
+    s = Setup([(5, 48), (4, 40), (3, 30)], F16, 16, 2, d, 16, seed=61, gap=2)
+    for length, first in (((1 << 31) - 1, 2), (1 << 30, 2), ((1 << 31) - 1, -(1 << 31))):
+        s.d_start.upload(np.array([first, 7, 11, 14], np.int64).astype(np.int32))
+        s.d_length.upload(np.array([length, -(1 << 31), 30], np.int64).astype(np.int32))
+        n0 = 7 - max(first, 0)
+        width = (heads + 4) * d
+        qkv = raw(s.rng.standard_normal((s.rows, width)), F16)
+        turns = s.kv.rope_turns(d, 10000.0)
+        d_qkv, d_turns = s.Buffer.from_numpy(qkv), s.Buffer.from_numpy(turns)
+        sentinel = raw(np.full((s.rows, heads * d), 9.0), F16)
+        out, read = s.Buffer.from_numpy(sentinel), s.Buffer.from_numpy(np.full((s.rows, 2, d), 5.0, np.float32))
+        batch = s.kv.KvBatch(s.d_start.ptr, s.d_length.ptr, s.d_table.ptr, 2, s.width, s.rows)           # the third sequence only reads
+        s.kv.append(s.cache, batch, d_qkv.ptr + heads * d * 2, d_qkv.ptr + (heads + 2) * d * 2, s.kv.Rope(d_turns.ptr, d), d_qkv.ptr, heads, d_qkv.ptr,
+                    width, width, width, width)
+        ws = s.kv.new_attention_workspace(s.cache, batch, heads)
+        s.kv.attention(s.cache, batch, d_qkv.ptr, heads, d ** -0.5, out.ptr, ws, q_stride=width)
+        s.kv.read(s.cache, s.batch, F32, read.ptr, 0)
+        pool, _ = s.download()
+        assert all(np.array_equal(pool[n], s.pool[n]) for n in "kv")                  # nothing lay in the table
+        rotated, got = d_qkv.download(qkv.shape, np.uint16), out.download(sentinel.shape, np.uint16)
+        ours = np.arange(s.rows)
+        ours = (ours >= max(first, 0)) & (ours < 7)
+        assert np.array_equal(rotated[~ours], qkv[~ours]) and np.array_equal(rotated[:, heads * d:], qkv[:, heads * d:])
+        keys, vals = np.zeros((64, 2, d)), np.zeros((64, 2, d))                       # the table's last page is none: zeros
+        keys[:48], vals[:48] = s.held("k", 0, np.arange(48)), s.held("v", 0, np.arange(48))
+        position = (1 << 30) - n0
+        for i, row in enumerate(np.flatnonzero(ours)):
+            q = values(rotated[row, :heads * d], F16).reshape(heads, d)
+            x = values(qkv[row, :heads * d], F16).reshape(heads, d)
+            # turns in 64 bits at 2^30 are off by 2^30 * 2^-53 of a turn; then fp32 and one rounding to fp16
+            assert np.abs(q - okv.rope(x, position + i, turns)).max() <= (2.0 ** -11 + 2.0 ** -19) * 8
+            want, mass, most, seen, top_v = okv.attention(q[None], keys, vals, position + i, d ** -0.5)
+            bar = (np.expm1(2 * (d + 4) * 2.0 ** -23 * most) + 2.0 ** -20 + 2.0 ** -11 + seen * 2.0 ** -22)[..., None] * mass + (2.0 ** -25 * seen * top_v)[..., None]
+            bar = bar + 2.0 ** -11 * (np.abs(want) + bar) + 2.0 ** -25
+            assert (seen == 64).all() and (np.abs(values(got[row], F16).reshape(1, heads, d) - want) <= bar).all()
+        assert (got[7:11] == 0).all()                                                 # a sequence without tokens
+        none = ~ours
+        none[7:11] = False
+        assert np.array_equal(got[none], sentinel[none])
+        back = read.download((s.rows, 2, d), np.float32)
+        assert np.array_equal(back[11:14], s.held("k", 2, np.array([27, 28, 29])).astype(np.float32)) and (np.delete(back, [11, 12, 13], 0) == 5.0).all()
+        assert not ws.download((16384,), np.uint8).any()
