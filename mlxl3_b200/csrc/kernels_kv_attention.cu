@@ -660,6 +660,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__
         if (++stage == S::kStages) { stage = 0; parity ^= 1u; }
     }
     __syncthreads();
+    settle_after_failure(s_failed != 0);
     if (threadIdx.x == 0 && s_failed) atomicExch(a.error, 8u);
 }
 

@@ -776,7 +776,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&kv_full[slot]);
             }
-            more = step() && step();
+            more = step() && step() && !__any_sync(0xffffffffu, s_state.failed != 0);      // then nobody waits for copies any more
         }
     } else {
         fewer_registers<kIssueRegisters>();
@@ -938,6 +938,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
     fence_before();
     __syncthreads();
     fence_after();
+    settle_after_failure(s_state.failed != 0);
     if (warp == kSoftmaxWarps + kLoadWarps) {
         __syncwarp();
         tmem_dealloc(tmem, 512);

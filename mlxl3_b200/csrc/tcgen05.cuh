@@ -63,6 +63,12 @@ static __device__ __noinline__ bool qmm_wait_slow(uint64_t* bar, uint32_t parity
 __device__ __forceinline__ bool qmm_wait(uint64_t* bar, uint32_t parity, volatile int* cta_failed) {
     return mbar_try_wait(bar, parity) || qmm_wait_slow(bar, parity, cta_failed);
 }
+// Copies and products that were still in flight when a wait gave up have to land before the CTA gives its memory back.
+__device__ __forceinline__ void settle_after_failure(bool failed) {
+    if (!failed) return;
+    const unsigned long long t0 = global_ns();
+    while (global_ns() - t0 < 2000000ull) __nanosleep(1000);
+}
 // Barrier of some warps.  Not the aligned form (`bar.sync`), which all lanes of a warp have to execute as one: lanes come here
 // from branches of their own (lane 0 from an atomic or an arrival), where nothing but a warp barrier brings them together again.
 // The same holds for the instructions marked .sync.aligned -- allocation and release of tensor memory, its loads and stores and
