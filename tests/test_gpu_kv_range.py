@@ -336,3 +336,26 @@ def test_lengths_and_rows_without_sense(gpu):
         back = read.download((s.rows, 2, d), np.float32)
         assert np.array_equal(back[11:14], s.held("k", 2, np.array([27, 28, 29])).astype(np.float32)) and (np.delete(back, [11, 12, 13], 0) == 5.0).all()
         assert not ws.download((16384,), np.uint8).any()
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_single_tokens_beside_one_that_is_not_finite(gpu, bits):
+    """A step of single tokens: a sequence that holds an infinity and one that holds a NaN are not finite, the others have the same bits."""
+    s = Setup([(1, 90), (1, 200), (1, 17), (1, 300)], BF16, bits, 2, 128, 16, seed=62, tail=0)
+    q = raw(s.rng.standard_normal((s.rows, 4 * 128)), BF16)
+    plain = run_attention(s, 4, q, max_new=1)
+    for b, t, number in ((1, 199, np.inf), (2, 3, np.nan)):
+        at = s.table[b, t // 16], slice(None), t % 16
+        if bits == 16:
+            s.pool["v"][at + (9,)] = raw(np.array([number]), BF16)[0]
+        else:
+            s.scale["v"][at] = number
+    s.upload()
+    got = run_attention(s, 4, q, max_new=1)
+    assert np.array_equal(got[[0, 3]], plain[[0, 3]])
+    odd = np.ones(128, bool)
+    if bits == 16:
+        odd[:] = False
+        odd[9] = True
+        assert np.array_equal(got[1:3][:, :, ~odd], plain[1:3][:, :, ~odd])
+    assert not np.isfinite(got[1:3][:, :, odd]).any()
