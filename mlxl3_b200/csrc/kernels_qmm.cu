@@ -639,7 +639,11 @@ qmm_kernel(const __grid_constant__ CUtensorMap xmap, const QmmArgs p) {
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");   // every warp's last access before the memory is given back
     if (tr && threadIdx.x == 0) tr[6] = global_ns();
-    settle_after_failure(s_failed != 0);
+    if (s_failed) {
+        // copies that were still in flight when a wait gave up must land before the CTA's shared memory is released
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 2000000ull) __nanosleep(1000);
+    }
     __syncwarp();
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
     if (threadIdx.x == 0 && s_failed) {

@@ -63,7 +63,8 @@ static __device__ __noinline__ bool qmm_wait_slow(uint64_t* bar, uint32_t parity
 __device__ __forceinline__ bool qmm_wait(uint64_t* bar, uint32_t parity, volatile int* cta_failed) {
     return mbar_try_wait(bar, parity) || qmm_wait_slow(bar, parity, cta_failed);
 }
-// Copies and products that were still in flight when a wait gave up have to land before the CTA gives its memory back.
+// Copies and products that were still in flight when a wait gave up have to land before the CTA gives its memory back (as at the end of
+// qmm_kernel).  Lanes leave the loop one by one: a warp barrier belongs behind it.
 __device__ __forceinline__ void settle_after_failure(bool failed) {
     if (!failed) return;
     const unsigned long long t0 = global_ns();
