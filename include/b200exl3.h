@@ -468,8 +468,9 @@ typedef struct {
 /* The sequences of a call: sequence b brings the rows d_row_start[b] .. d_row_start[b + 1] - 1 of the row buffers, which are the last
  * of its d_length[b] tokens (row i of n is token length - n + i), and token t lies in row t % page_size of page d_page_table[b,
  * t / page_size].  d_row_start ascends; `rows` bounds the row buffers.  Rows that are no sequence's and tokens before the first are left
- * as they were; tokens behind the table and pages outside the pool are never written and read as zeros (kv_read leaves their rows as
- * they were).  No two sequences of a call may append to the same row of a page. */
+ * as they were; a length above 2^30 counts as that.  Tokens behind the table and in pages outside the pool are never written, and
+ * kv_read leaves their rows as they were; to kv_attention those behind the table do not exist, and those in pages outside the pool are
+ * zeros.  No two sequences of a call may append to the same row of a page. */
 typedef struct {
     const int32_t* d_row_start;      /* [batch + 1] */
     const int32_t* d_length;         /* [batch] */
@@ -493,16 +494,19 @@ typedef struct {
 int b200exl3_kv_append(const b200exl3_kv_cache* cache, const b200exl3_kv_batch* batch, const b200exl3_rope* rope, const void* d_q,
                        int64_t q_stride, int heads, void* d_q_out, int64_t q_out_stride, const void* d_k, int64_t k_stride,
                        const void* d_v, int64_t v_stride, b200exl3_stream stream);
-/* What the cache holds for the rows of the batch: keys and values [rows, kv_heads, head_dim] in out_dtype (f16, bf16 or f32), rounded
- * once; either output may be NULL. */
+/* What the cache holds for the rows of the batch: keys and values [rows, kv_heads, head_dim], a code times its scale in fp32, in out_dtype
+ * (f16, bf16 or f32); either output may be NULL. */
 int b200exl3_kv_read(const b200exl3_kv_cache* cache, const b200exl3_kv_batch* batch, int out_dtype, void* d_k_out, void* d_v_out,
                      b200exl3_stream stream);
 /* out[row, h] = sum_j softmax_j(scale * q[row, h] . k_j) v_j over the tokens j up to the row's own, with window > 0 the last `window` of
  * them; heads / kv_heads query heads share a key head; the row's own token has been appended before.  A row that sees no token is
  * zero.  max_new bounds the rows of one sequence (rows beyond it are not computed; 0 = `rows`): it chooses the kernel, so say 1 for a
  * step of single tokens.  A row takes nothing from tokens that it does not see, whatever they hold; one that sees an infinity or NaN is
- * not finite there.  scale > 0.  Parts are joined in the order of the keys: a call gives the same bits every time, but where keys are cut depends on the
- * whole batch.  The workspace follows the rules of the linear layer's (header of zeros; one call at a time; status 8 = a wait gave up). */
+ * not finite there.  scale > 0; any window (0 = none).  Scores, sums and outputs are fp32; probabilities (over codes: times the value's
+ * scale) are rounded to the type of the products, that of a 16-bit cache or fp16 over codes, which may lose what lies 2^32 below a row's
+ * largest one; value scales below 2^-93 lose bits.  Parts are joined in the order of the keys: a call gives the same bits every time, but
+ * where keys are cut depends on the whole batch.  Pages of a multiple of eight rows are copied whole, others row by row (a step of single
+ * tokens takes twice as long).  The workspace follows the rules of the linear layer's (header of zeros; one call at a time; status 8 = a wait gave up). */
 int b200exl3_kv_attention_workspace_bytes(const b200exl3_kv_cache* cache, int heads, int64_t max_new, size_t* out_bytes);
 int b200exl3_kv_attention(const b200exl3_kv_cache* cache, const b200exl3_kv_batch* batch, const void* d_q, int64_t q_stride, int heads,
                           float scale, int window, int64_t max_new, void* d_out, int64_t out_stride, void* d_workspace,

@@ -1988,7 +1988,7 @@ int b200exl3_kv_attention_workspace_bytes(const b200exl3_kv_cache* cache, int he
     KvArgs p;
     if (!out_bytes) return fail("NULL argument");
     if (kv_args(cache, nullptr, p) || kv_attention_heads(cache, heads, max_new)) return -1;
-    *out_bytes = kCounterBytes + round256(kv_attention_workspace_bytes(p.bits, p.head_dim, heads / p.kv_heads, max_new));
+    *out_bytes = kCounterBytes + round256(kv_attention_workspace_bytes(p.head_dim, heads / p.kv_heads, max_new));
     return 0;
 }
 
@@ -2006,7 +2006,7 @@ int b200exl3_kv_attention(const b200exl3_kv_cache* cache, const b200exl3_kv_batc
     const int64_t width = static_cast<int64_t>(heads) * p.head_dim;
     if (kv_stride(q_stride, width) || kv_stride(out_stride, width)) return -1;
     if (!aligned16(d_q) || !aligned16(d_out) || !aligned16(ws)) return fail("device pointers must be 16-byte aligned");
-    const size_t need = kCounterBytes + round256(kv_attention_workspace_bytes(p.bits, p.head_dim, heads / p.kv_heads, max_new));
+    const size_t need = kCounterBytes + round256(kv_attention_workspace_bytes(p.head_dim, heads / p.kv_heads, max_new));
     if (!ws || ws_bytes < need) return fail("workspace too small: %zu bytes given, %zu needed", ws_bytes, need);
     KvAttentionArgs a{};
     a.q = d_q;

@@ -456,7 +456,7 @@ struct KvAttentionArgs {
     unsigned int* error;       // status word of the workspace
     float* parts;              // two places per CTA for its part of a segment that CTAs share
 };
-size_t kv_attention_workspace_bytes(int bits, int head_dim, int group, int64_t max_new);
+size_t kv_attention_workspace_bytes(int head_dim, int group, int64_t max_new);
 cudaError_t launch_kv_attention(const KvArgs& args, const KvAttentionArgs& attention, cudaStream_t stream);
 // sequences of many rows on the tcgen05 tensor cores (kernels_kv_prefill.cu)
 size_t kv_many_workspace_bytes(int head_dim);

@@ -707,7 +707,7 @@ cudaError_t launch_attention(const KvArgs& p, KvAttentionArgs a, cudaStream_t st
 
 }  // namespace
 
-size_t kv_attention_workspace_bytes(int, int head_dim, int group, int64_t max_new) {
+size_t kv_attention_workspace_bytes(int head_dim, int group, int64_t max_new) {
     const size_t few = 2 * static_cast<size_t>(3 * sm_count()) * 16 * (head_dim + 2) * sizeof(float);
     return max_new * group <= kFewRows ? few : std::max(few, kv_many_workspace_bytes(head_dim));
 }

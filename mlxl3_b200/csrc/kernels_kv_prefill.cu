@@ -19,12 +19,13 @@
 // sets the status word, all roles run on to the end, and the kernel frees its tensor memory.
 //
 // Values of blocks that not all rows of a segment see whole are looked through for infinities and NaN by the row threads, between their
-// probabilities and the product (why: kernels_kv_attention.cu).  A mixed step with two such blocks a segment took 83 us without and takes 88,
-// the prompt 175 and 176; with the look by a warp of its own ahead of the products they took 91 and 178.
+// probabilities and the product (why: kernels_kv_attention.cu).  A mixed step with two such blocks a segment took 83 us without and takes 86,
+// the prompt 175 and 175; with the look by a warp of its own ahead of the products they took 91 and 178.
 //
 // What bounds it: for long prompts the chain score product -> softmax -> output product of the two tiles in turn, 3400 cycles a block, of which
 // the products need 2864 (a step of K = 16 takes 105 cycles with both operands in shared memory, 74 with the left one in tensor
-// memory; the pipe's own time is 64), under the power cap.  4096 tokens, 32 heads of 128 over 8, fp16: 176 us.  Segments of one tile leave
+// memory; the pipe's own time is 64), under the power cap.  4096 tokens, 32 heads of 128 over 8, fp16: 160 us for
+// forty calls, 175 us when the power cap has settled.  Segments of one tile leave
 // the other idle (their blocks dealt to both pipelines gained 4 %): 16 draft tokens of 8 sequences, five heads to a key head, 8 bits:
 // 102 us.
 #include "kv_work.cuh"

@@ -32,7 +32,6 @@ struct KvTable {
 
 template <int ROWS, int KEYS, int OVER>
 struct KvWork {
-    static constexpr int kOver = OVER;
     const KvArgs& p;
     const KvAttentionArgs& a;
     const int* start;      // [batch + 1], [batch]
@@ -259,7 +258,7 @@ template <> constexpr float kLift<__nv_bfloat16> = -32.0f;
 // the row itself sees: a rounding costs 2^-11 of a term, or 2^-32 of the row's largest one, whatever scales other keys have.  The sum of
 // the probabilities has 2^(s + lift - m).  So that it fits fp32 for scales at the ends of its range too, they enter as vs / 2^16, and
 // their logarithm is not taken below -88: sums reach 2^(88 + 15) a key, and a largest term of scale 2^125 (4-bit bf16) is 2^-102.
-// Scales below 2^-96 lose bits, as good as zero.
+// Scales below 2^-93 lose bits, those below 2^-104 are zero.
 constexpr float kScaleUnit = 65536.0f;
 __device__ __forceinline__ float kv_scale_log(float vs) {         // of a scale in that unit; NaN: the least
     float y;
