@@ -329,7 +329,7 @@ kv_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
                     fence_after();
                     if (j + 1 == n) {
                         next_count = block_count + n;
-                                more = next_segment(at);
+                        more = next_segment(at);
                         settle();
                     }
                     bool partly = false;                          // some rows of the segment see keys of the block that others do not
