@@ -52,6 +52,7 @@ def new_attention_workspace(heads: int, kv_heads: int) -> DeviceBuffer:
     """Scratch of ``attention_decode``: it starts with arrival counters that must be zero before the first call."""
     ws = DeviceBuffer(attention_workspace_bytes(heads, kv_heads))
     ws.fill(0)
+    DEFAULT_STREAM.sync()                # calls on other streams do not wait for it
     return ws
 
 

@@ -1,7 +1,7 @@
-"""Who owns and prepares the memory of a paged key/value cache (no GPU needed)."""
+"""Who owns and prepares the memory of the key/value caches and of attention (no GPU needed)."""
 import pytest
 
-from mlxl3_b200 import kv
+from mlxl3_b200 import decoder, kv
 
 
 @pytest.mark.parametrize("bits,buffers", [(16, 2), (8, 4), (4, 4)])
@@ -30,3 +30,24 @@ def test_a_new_cache_is_zeroed_when_its_constructor_returns(monkeypatch, bits, b
     del log[:]
     kv.KvCache(3, 16, 2, 64, d_k=4096, d_v=8192)
     assert not log
+
+
+def test_a_new_attention_workspace_is_zeroed_when_the_function_returns(monkeypatch):
+    log = []
+
+    class Buffer:
+        def __init__(self, nbytes):
+            log.append("new")
+
+        def fill(self, byte):
+            log.append("fill")
+
+    class Stream:
+        handle = None
+
+        def sync(self):
+            log.append("sync")
+    monkeypatch.setattr(decoder, "DeviceBuffer", Buffer)
+    monkeypatch.setattr(decoder, "DEFAULT_STREAM", Stream())
+    decoder.new_attention_workspace(32, 8)
+    assert log == ["new", "fill", "sync"]
